@@ -360,6 +360,98 @@ TN_API int tn_sdpa_decode_step_q8(const void *qkv, const float *inv_freq, void *
                                   const int64_t *k_strides, const int64_t *v_strides, const int *pos_dev,
                                   double scale, void *stream);
 
+/* ------------------------------------------------- paged 4-bit KV cache --
+ * A KV cache in GGML Q4_0 blocks (4.5 bits an element; BlockQ4_0::from_float,
+ * vendor/candle-core/src/quantized/k_quants.rs:241-277), in pages that requests
+ * take and give back as they grow and end. The reference's cache is dense and
+ * contiguous (torchnative/python/torchnative/kernels/kv_cache.py:51-185): these
+ * entry points have no counterpart there.
+ *
+ * pool: uint8 [num_pages][kv_heads][page_size / 16][18 * head_dim], 16-byte
+ * aligned: groups of 16 tokens of one head, keys then values, codes then f16
+ * scales, in the order that the attention kernels read (kv_q4.cuh, with the bytes of a
+ * group). page_size: a power of two from 16 to 1024; head_dim 64 or 128.
+ * page_table: int32 [requests][table_stride], the first max_pages columns of
+ * which may be used: the pages of each request in order, -1 where none.
+ * lengths: int32 [requests], cached tokens. A length outside [0, max_pages *
+ * page_size] counts as the nearer end. Page ids, slots and positions are device
+ * data that no host check sees: one outside its range is never followed; its
+ * token is left out and tn_device_status reports TN_ERR_INVALID.
+ * Different pages of the table must be different pages, and slots of one append
+ * different slots, as tn_kv_pages_resize makes them. */
+
+/* Bytes of one page of one layer (-1 on a bad argument). */
+TN_API int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t page_size);
+
+/* Block tables and slot maps from request lengths, in one launch: takes every
+ * request from lengths[b] tokens to new_lengths[b] (device, not `lengths`
+ * itself), or, with new_lengths NULL, every request that has tokens to grow more.
+ * A request that shrinks gives its last pages back on the stack free_pages[0,
+ * *free_count), one that grows takes from its top; stack order is such that
+ * undoing a call restores the table and the stack. Then, for the new tokens
+ * (request by request, packed): slots[r] = page * page_size + offset,
+ * positions[r] = place in the request, and -1 for r from the last new token to
+ * max_tokens; query_start [requests + 1] the first of each request's new
+ * tokens. lengths, page_table, free_pages and *free_count are updated.
+ * A call that cannot be met changes none of them, gives no token a slot
+ * (slots and positions -1, query_start 0) and sets *status, if that is 0, to
+ * 1: not enough pages, 2: a length outside [0, max_pages * page_size], 3: more
+ * new tokens than max_tokens, 4: more free pages than num_pages. *status is
+ * never cleared here. requests <= 8192. */
+TN_API int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
+                              const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
+                              int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots,
+                              int *positions, int64_t max_tokens, int *query_start, int *status, void *stream);
+
+/* Quantises key and value rows k, v [tokens][kv_heads][head_dim] (dtype F32,
+ * F16 or BF16; element strides of token and head, unit inner stride, rows 16-byte
+ * aligned) into the pool at slots[token] (int64; a negative slot is skipped: a
+ * padded row). Codes and scales are those of tn_q4_0_quantize. */
+TN_API int tn_kv_q4_append(const void *k, const void *v, int dtype, const int64_t *k_strides,
+                           const int64_t *v_strides, int64_t tokens, const int64_t *slots, void *pool,
+                           int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size, void *stream);
+
+/* Scratch bytes of the two attention calls below (device memory of the
+ * caller's, 16-byte aligned, any contents; two calls that can run at the same
+ * time need one each). max_query: a bound on one request's query tokens. */
+TN_API int64_t tn_sdpa_q4_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t max_query);
+
+/* Attention over the cache, as tn_sdpa_flash_attention computes it over dense
+ * keys and values. q [tokens][heads][head_dim] (dtype F32, F16, BF16; strides
+ * of token and head) holds the requests' query tokens packed: those of request
+ * b are rows query_start[b] to query_start[b + 1] (device int32 [requests +
+ * 1], ascending; NULL: one row each, tokens == requests). Query token i of n of
+ * a request of lengths[b] = S tokens (its own among them, already appended)
+ * attends keys 0 to S - n + i; one that sees no key gives zeros and lse 0.
+ * Query head h reads cache head h / (heads / kv_heads). out [tokens][heads]
+ * [head_dim] in q's dtype, lse [tokens][heads] f32 or NULL; rows behind the
+ * last request's are left as they were. max_query: a bound on one request's
+ * query tokens (it chooses the kernel; every value gives the right result).
+ * scale <= 0 or NaN: 1 / sqrt(head_dim). */
+TN_API int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strides, int64_t tokens, int64_t heads,
+                            const void *pool, int64_t num_pages, int64_t kv_heads, int64_t head_dim,
+                            int64_t page_size, const int *page_table, int64_t table_stride, int64_t max_pages,
+                            const int *lengths, int64_t requests, const int *query_start, int64_t max_query,
+                            void *out, float *lse, double scale, void *workspace, int64_t workspace_bytes,
+                            void *stream);
+
+/* The attention block of one decode token of every request (bf16), as
+ * tn_sdpa_decode_step_q8 over the dense cache: from the q/k/v projection rows
+ * qkv [requests][(heads + 2 kv_heads) head_dim], rotate q and k at position
+ * lengths[b] - 1 (row of rope [rope_rows][head_dim] bf16: cosines, then sines;
+ * halves rotated against each other, f32 products and sum rounded once to
+ * bf16), append k and v to that slot in 4 bits, attend keys [0, lengths[b])
+ * and, if codes is not NULL, write out's planar Q8_0 too (the bytes of
+ * tn_q8_0_quantize_planar). A request of length 0 appends nothing and gives
+ * zeros. out [requests][heads][head_dim]; heads / kv_heads <= 8. */
+TN_API int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t rope_rows, void *pool,
+                                  int64_t num_pages, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  int64_t page_size, const int *page_table, int64_t table_stride,
+                                  int64_t max_pages, const int *lengths, int64_t requests, void *out, float *lse,
+                                  int8_t *codes, float *scales, float *offsets, double scale, void *workspace,
+                                  int64_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------ decode-step glue (bf16) --
  * The work between the hot operators in one greedy token of transformers'
  * LlamaForCausalLM (modeling_llama.py: LlamaRMSNorm, apply_rotary_pos_emb,

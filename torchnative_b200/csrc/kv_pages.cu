@@ -1,0 +1,231 @@
+// kv_pages.cu -- block tables and slot maps from request lengths.
+//
+// One call takes every request from its old length to its new one: pages of
+// requests that shrink go back on the free stack, requests that grow take pages
+// from its top, and every new token gets its slot, position and place in the
+// packed rows. All of it is prefix sums over the requests (pages given, pages
+// taken, tokens new), so the result does not depend on any order of execution.
+#include "kv_q4.cuh"
+
+namespace tn {
+
+int kv_page_shift(int64_t page_size) {
+    for (int s = 4; s <= 10; ++s)
+        if (page_size == (int64_t)1 << s) return s;
+    return -1;
+}
+
+int check_kv_pool(const char *op, const void *pool, int64_t num_pages, int64_t kv_heads, int64_t head_dim,
+                  int64_t page_size) {
+    const std::string name(op);
+    if (kv_page_shift(page_size) < 0)
+        return set_error(TN_ERR_NOT_IMPLEMENTED, name + ": a page holds 16, 32, 64, 128, 256, 512 or 1024 tokens, got " +
+                                                     std::to_string(page_size));
+    if (head_dim != 64 && head_dim != 128)
+        return set_error(TN_ERR_NOT_IMPLEMENTED, name + ": the 4-bit KV cache takes head dimensions 64 and 128, got " +
+                                                     std::to_string(head_dim));
+    if (num_pages < 0 || num_pages > INT32_MAX || kv_heads < 1 || kv_heads > 65535)
+        return set_error(TN_ERR_SHAPE, name + ": bad page or head count");
+    if ((!pool && num_pages > 0) || reinterpret_cast<uintptr_t>(pool) % 16 != 0)
+        return set_error(TN_ERR_INVALID, name + ": the pool must be a 16-byte aligned device pointer");
+    return TN_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kMaxRequests = 8192;
+
+enum : int { BAD_NONE = 0, BAD_POOL = 1, BAD_LENGTH = 2, BAD_TOKENS = 3, BAD_STACK = 4 };
+
+struct Resize {
+    int *table;
+    int64_t table_stride;
+    int max_pages;
+    int *lengths;
+    const int *new_lengths;  // NULL: every request with tokens grows by `grow`
+    int grow, requests;
+    int *free_pages, *free_count;
+    int num_pages, page_shift;
+    int64_t *slots;
+    int *positions;
+    int max_tokens;
+    int *query_start, *status;
+};
+
+__device__ __forceinline__ int pages_of(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
+
+// The last of the `n` ascending starts that is at most x (x >= starts[0] = 0).
+__device__ __forceinline__ int find(const int *starts, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// Latency bounds it: one launch, and inside it a chain of dependent loads
+// (lengths, prefix sums, stack entries).
+__global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize p) {
+    extern __shared__ int sm[];
+    const int B = p.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int *old_len = sm, *new_len = sm + B, *give_at = sm + 2 * B, *take_at = sm + 3 * B, *tok_at = sm + 4 * B;
+    __shared__ long long warp_sum[3][kThreads / 32];
+    __shared__ long long total[3];
+    __shared__ int bad_length;
+
+    pdl_launch_dependents();
+    pdl_wait();
+    if (tid == 0) bad_length = 0;
+    __syncthreads();
+    const int top0 = *p.free_count;
+    const int64_t cap = (int64_t)p.max_pages << p.page_shift;
+    // each thread takes `per` neighbouring requests
+    const int per = (B + kThreads - 1) / kThreads, b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    long long sum[3] = {0, 0, 0};
+    for (int b = b0; b < b1; ++b) {
+        const int o = p.lengths[b];
+        const long long n = p.new_lengths ? p.new_lengths[b] : (o > 0 ? (long long)o + p.grow : 0);
+        if (o < 0 || o > cap || n < 0 || n > cap) {
+            bad_length = 1;
+            old_len[b] = new_len[b] = 0;
+            continue;
+        }
+        old_len[b] = o;
+        new_len[b] = (int)n;
+        const int have = pages_of(o, p.page_shift), want = pages_of((int)n, p.page_shift);
+        sum[0] += max(0, have - want);
+        sum[1] += max(0, want - have);
+        sum[2] += max(0, (int)n - o);
+    }
+    long long before[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        long long v = sum[k];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, off);
+            if (lane >= off) v += u;
+        }
+        if (lane == 31) warp_sum[k][warp] = v;
+        before[k] = v - sum[k];
+    }
+    __syncthreads();
+    if (warp < 3) {
+        long long v = warp_sum[warp][lane];
+        const long long own = v;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, off);
+            if (lane >= off) v += u;
+        }
+        warp_sum[warp][lane] = v - own;
+        if (lane == 31) total[warp] = v;
+    }
+    __syncthreads();
+    const long long gives = total[0], takes = total[1], tokens = total[2];
+    const int bad = bad_length                                            ? BAD_LENGTH
+                    : top0 < 0 || top0 + gives > (long long)p.num_pages   ? BAD_STACK
+                    : takes > top0 + gives                                ? BAD_POOL
+                    : tokens > (long long)p.max_tokens                    ? BAD_TOKENS
+                                                                          : BAD_NONE;
+    if (bad) {  // nothing changes; no token has a slot
+        if (tid == 0 && *p.status == 0) *p.status = bad;
+        for (int b = tid; b <= B; b += kThreads) p.query_start[b] = 0;
+        for (int r = tid; r < p.max_tokens; r += kThreads) {
+            p.slots[r] = -1;
+            p.positions[r] = -1;
+        }
+        return;
+    }
+    for (int b = b0; b < b1; ++b) {
+        const int o = old_len[b], n = new_len[b];
+        const int have = pages_of(o, p.page_shift), want = pages_of(n, p.page_shift);
+        give_at[b] = (int)(before[0] + warp_sum[0][warp]);
+        take_at[b] = (int)(before[1] + warp_sum[1][warp]);
+        tok_at[b] = (int)(before[2] + warp_sum[2][warp]);
+        before[0] += max(0, have - want);
+        before[1] += max(0, want - have);
+        before[2] += max(0, n - o);
+        p.query_start[b] = tok_at[b];
+        p.lengths[b] = n;
+    }
+    const int top = top0 + (int)gives;
+    if (tid == 0) {
+        p.query_start[B] = (int)tokens;
+        *p.free_count = top - (int)takes;
+    }
+    __syncthreads();
+    // pages given back, the last one first, so that a roll-back leaves the stack as it was
+    for (int i = tid; i < (int)gives; i += kThreads) {
+        const int b = find(give_at, B, i);
+        const int64_t at = b * p.table_stride + pages_of(new_len[b], p.page_shift) + (i - give_at[b]);
+        p.free_pages[top - 1 - i] = p.table[at];
+        p.table[at] = -1;
+    }
+    __syncthreads();
+    for (int i = tid; i < (int)takes; i += kThreads) {
+        const int b = find(take_at, B, i);
+        p.table[b * p.table_stride + pages_of(old_len[b], p.page_shift) + (i - take_at[b])] = p.free_pages[top - 1 - i];
+    }
+    for (int r = tid; r < p.max_tokens; r += kThreads) {
+        int64_t slot = -1;
+        int position = -1;
+        if (r < (int)tokens) {
+            const int b = find(tok_at, B, r);
+            position = old_len[b] + r - tok_at[b];
+            const int j = position >> p.page_shift, have = pages_of(old_len[b], p.page_shift);
+            const int page = j < have ? p.table[b * p.table_stride + j] : p.free_pages[top - 1 - (take_at[b] + j - have)];
+            slot = ((int64_t)page << p.page_shift) + (position & ((1 << p.page_shift) - 1));
+        }
+        p.slots[r] = slot;
+        p.positions[r] = position;
+    }
+}
+
+}  // namespace
+}  // namespace tn
+
+extern "C" int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t page_size) {
+    if (tn::check_kv_pool("tn_kv_q4_page_bytes", nullptr, 0, kv_heads, head_dim, page_size)) return -1;
+    return kv_heads * (page_size / tn::kKvGroup) * 18 * head_dim;
+}
+
+extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
+                                  const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
+                                  int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots, int *positions,
+                                  int64_t max_tokens, int *query_start, int *status, void *stream) {
+    const std::string op("tn_kv_pages_resize");
+    const int shift = tn::kv_page_shift(page_size);
+    if (shift < 0)
+        return tn::set_error(TN_ERR_NOT_IMPLEMENTED, op + ": a page holds 16, 32, 64, 128, 256, 512 or 1024 tokens, got " +
+                                                         std::to_string(page_size));
+    if (requests < 0 || max_pages < 0 || table_stride < max_pages || num_pages < 0 || num_pages > INT32_MAX ||
+        max_tokens < 0 || max_tokens > INT32_MAX || max_pages > (int64_t)INT32_MAX >> shift)
+        return tn::set_error(TN_ERR_SHAPE, op + ": bad table, pool or token count");
+    if (grow < 0 || grow > INT32_MAX)
+        return tn::set_error(TN_ERR_SHAPE, op + ": grow must be a token count (new_lengths shrinks requests)");
+    if (requests > tn::kMaxRequests)
+        return tn::set_error(TN_ERR_NOT_IMPLEMENTED, op + ": at most " + std::to_string(tn::kMaxRequests) + " requests");
+    if (!free_count || !query_start || !status || (requests > 0 && !lengths) ||
+        (requests > 0 && max_pages > 0 && !page_table) || (num_pages > 0 && !free_pages) ||
+        (max_tokens > 0 && (!slots || !positions)))
+        return tn::set_error(TN_ERR_INVALID, op + ": null pointer");
+    if (new_lengths && new_lengths == lengths)
+        return tn::set_error(TN_ERR_INVALID, op + ": new_lengths must not be lengths");
+    tn::Resize p{page_table, table_stride, (int)max_pages, lengths, new_lengths, (int)grow, (int)requests, free_pages,
+                 free_count, (int)num_pages, shift, slots, positions, (int)max_tokens, query_start, status};
+    const int smem = (int)(5 * requests * sizeof(int));
+    if (smem > 48 * 1024 - 1024) {
+        int st = tn::check_cuda(
+            cudaFuncSetAttribute(tn::kv_pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+            "tn_kv_pages_resize", "cudaFuncSetAttribute");
+        if (st) return st;
+    }
+    return tn::launch_pdl(tn::kv_pages_resize_kernel, dim3(1), dim3(tn::kThreads), smem, tn::stream_of(stream),
+                          "tn_kv_pages_resize", p);
+}

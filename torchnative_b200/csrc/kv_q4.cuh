@@ -1,0 +1,149 @@
+// kv_q4.cuh -- the paged 4-bit KV cache: its layout in memory, and what the
+// kernels that fill and read it share.
+//
+// A pool holds pages of `page_size` tokens (a power of two from 16 on) for
+// every KV head; a page of one head is page_size / 16 groups of 16 tokens, and
+// a group is 18 * D contiguous bytes:
+//   [0, 8D)     K codes   [16 tokens][4 t][D/32 blocks] words of 8 nibbles: nibble
+//                         n < 4 of word (t, block) is element 8t + 2n of the block's
+//                         32, nibble 4 + n is element 8t + 2n + 1
+//   [8D, 9D)    K scales  [16 tokens][D/32] f16
+//   [9D, 17D)   V codes   [2 h][8 g][4 t][D/32] words of two 16-bit halves: half p
+//                         is token 8h + 2t + p, its nibble n is element 4g + n
+//   [17D, 18D)  V scales  [16 tokens][D/32] f16
+// Codes and scales are GGML Q4_0's (BlockQ4_0::from_float, k_quants.rs:241-277),
+// only their order differs. It is the order in which a warp's m16n8k16 tensor
+// instructions take them: lane 4g + t finds the 8D / 32 bytes of its K rows
+// (tokens g and g + 8) and of its V columns (tokens 2t, 2t + 1, 2t + 8, 2t + 9)
+// as whole 16-byte (D = 64: 8-byte) vectors, neighbouring lanes next to each
+// other, and each extraction mask yields the two elements of one operand
+// register. A group's bytes are a multiple of 16, so that one bulk copy brings
+// it to shared memory.
+#pragma once
+
+#include <string>
+#include <type_traits>
+
+#include "tn_common.cuh"
+
+namespace tn {
+
+constexpr int kKvGroup = 16;
+
+template <int D>
+struct KvQ4 {
+    static constexpr int NB = D / 32;           // blocks a row
+    static constexpr int GROUP_BYTES = 18 * D;  // 16 tokens of one head, K and V
+    static constexpr int K_CODES = 0, K_SCALES = 8 * D, V_CODES = 9 * D, V_SCALES = 17 * D;
+    // byte of the K word (t, block) of token `key` of a group
+    __host__ __device__ static constexpr int k_word(int key, int t, int block) {
+        return K_CODES + key * (D / 2) + (t * NB + block) * 4;
+    }
+    // byte of the 16-bit V piece (elements 4g .. 4g + 3 of a block) of token `key`
+    __host__ __device__ static constexpr int v_half(int key, int g, int block) {
+        return V_CODES + (key >> 3) * 4 * D + ((g * 4 + ((key & 7) >> 1)) * NB + block) * 4 + (key & 1) * 2;
+    }
+    __host__ __device__ static constexpr int k_scale(int key, int block) { return K_SCALES + (key * NB + block) * 2; }
+    __host__ __device__ static constexpr int v_scale(int key, int block) { return V_SCALES + (key * NB + block) * 2; }
+};
+
+// The cache as a call gives it. Page ids, lengths and slots live on the device,
+// so the kernels check them: an id outside [0, num_pages) is never followed.
+struct KvPool {
+    uint8_t *pool;
+    int num_pages, page_shift, kv_heads;
+    const int *table;  // [requests][table_stride] page ids
+    int64_t table_stride;
+    int max_pages;
+    const int *lengths;  // [requests] cached tokens
+    int requests;
+    int *err;
+
+    // The cached tokens of request b, within what its table row can name.
+    __device__ __forceinline__ int length(int b) const {
+        const int64_t cap = (int64_t)max_pages << page_shift;
+        const int n = lengths[b];
+        return n < 0 ? 0 : (n > cap ? (int)cap : n);
+    }
+    // The group of tokens [16 group, 16 group + 16) of request b, or NULL (and
+    // the device error word set) where the table names no page of the pool.
+    template <int D>
+    __device__ __forceinline__ uint8_t *group(int b, int kvh, int group) const {
+        const int page = table[b * table_stride + (group >> (page_shift - 4))];
+        if ((unsigned)page >= (unsigned)num_pages) {
+            record_device_error(err, DEV_ERR_BAD_PAGE);
+            return nullptr;
+        }
+        const int64_t at = (((int64_t)page * kv_heads + kvh) << (page_shift - 4)) +
+                           (group & ((1 << (page_shift - 4)) - 1));
+        return pool + at * KvQ4<D>::GROUP_BYTES;
+    }
+};
+
+// A launch that may begin while the kernel before it ends (programmatic
+// dependent launch): every kernel of the cache waits for that kernel's memory
+// itself, before it reads or writes anything.
+template <typename K, typename... Args>
+int launch_pdl(K kernel, dim3 grid, dim3 block, int smem, cudaStream_t stream, const char *what, Args... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what, "cudaLaunchKernelEx");
+}
+
+int check_kv_pool(const char *op, const void *pool, int64_t num_pages, int64_t kv_heads, int64_t head_dim,
+                  int64_t page_size);
+int kv_page_shift(int64_t page_size);  // log2 of a page size the cache takes, else -1
+
+// The Q4_0 code of x in a block with reciprocal scale `inv`: trunc(x * inv + 8.5)
+// in [0, 15], NaN to 0 (Rust's `as u8`, then min 15). Explicitly rounded, so
+// that no contraction changes a byte.
+__device__ __forceinline__ uint32_t q4_0_code(float x, float inv) {
+    const float v = __fadd_rn(__fmul_rn(x, inv), 8.5f);
+    return !(v > 0.0f) ? 0u : (v >= 15.0f ? 15u : __float2uint_rz(v));
+}
+
+// The element of largest magnitude of a block of 32 held 8 a lane by 4
+// neighbouring lanes in element order; the first of equals, as
+// BlockQ4_0::from_float's loop finds it (NaN never wins its comparison).
+__device__ __forceinline__ float q4_0_extreme(const float (&x)[8]) {
+    float amax = 0.0f, m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(x[i]);
+        if (amax < a) amax = a, m = x[i];
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+        const float oa = __shfl_xor_sync(0xffffffffu, amax, off), om = __shfl_xor_sync(0xffffffffu, m, off);
+        // the lower lane's element comes first: of equals it wins
+        const bool other = (threadIdx.x & off) ? !(oa < amax) : (amax < oa);
+        if (other) amax = oa, m = om;
+    }
+    return m;
+}
+
+// 8 elements a lane (lane t of the block's 4) -> the lane's K word, or its two
+// V pieces (g = 2t low, g = 2t + 1 high).
+__device__ __forceinline__ uint32_t q4_0_k_word(const float (&x)[8], float inv) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+        w |= (q4_0_code(x[2 * n], inv) << (4 * n)) | (q4_0_code(x[2 * n + 1], inv) << (16 + 4 * n));
+    return w;
+}
+__device__ __forceinline__ uint32_t q4_0_v_halves(const float (&x)[8], float inv) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= q4_0_code(x[i], inv) << (4 * i);
+    return w;
+}
+
+}  // namespace tn

@@ -48,7 +48,13 @@ int *device_error_word();
 
 // ---- device-side helpers -----------------------------------------------------
 
-enum : int { DEV_ERR_NONE = 0, DEV_ERR_WAIT_FULL = 1, DEV_ERR_WAIT_EMPTY = 2, DEV_ERR_DRAIN = 3 };
+enum : int {
+    DEV_ERR_NONE = 0,
+    DEV_ERR_WAIT_FULL = 1,
+    DEV_ERR_WAIT_EMPTY = 2,
+    DEV_ERR_DRAIN = 3,
+    DEV_ERR_BAD_PAGE = 4  // a page id, slot or position outside what the call was given: skipped, never followed
+};
 
 // ~2^31 cycles (~1 s at 1.9 GHz) before a wait gives up: the default of the
 // per-device budget (tn_set_wait_budget) that waits read next to the error

@@ -230,6 +230,9 @@ int tn_device_status(int reset) {
         int zero = 0;
         cudaMemcpy(w, &zero, sizeof(int), cudaMemcpyHostToDevice);
     }
+    if (v == tn::DEV_ERR_BAD_PAGE)
+        return tn::set_error(TN_ERR_INVALID, "torchnative_b200: a paged KV cache call met a page id, slot or position "
+                                             "outside its pool or tables (that token was skipped)");
     if (v)
         return tn::set_error(TN_ERR_TIMEOUT, "torchnative_b200: a kernel's bounded wait gave up (device code " +
                                                  std::to_string(v) + ")");

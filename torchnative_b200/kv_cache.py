@@ -1,0 +1,311 @@
+"""A paged KV cache in 4 bits, and the operators that keep and read it.
+
+The reference's cache is dense (PreallocatedCache, torchnative/python/torchnative/
+kernels/kv_cache.py:51-185: one [B, Hkv, capacity, D] buffer a layer). Here keys
+and values are GGML Q4_0 blocks (4.5 bits an element, the weights' format) in
+pages of `page_size` tokens, which requests take and give back as they grow and
+end:
+
+- `kv_pages_resize`: block tables and slot maps from request lengths
+- `kv_q4_append`: keys and values quantised into their slots
+- `sdpa_q4_cache`: attention over the cached pages, one or many tokens a request
+- `sdpa_q4_decode_step`: one decode token's rotary embedding, append and
+  attention
+- `PagedQ4Cache`: the pools, tables and lengths of a model's layers
+
+The compute is the C ABI's (include/torchnative_b200.h). No CPU path: a CPU
+tensor is refused by name.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native as N
+
+GROUP = 16  # tokens of one head that lie together
+_CODE = {torch.float32: N.TN_F32, torch.bfloat16: N.TN_BF16, torch.float16: N.TN_F16}
+_STATUS = {1: "not enough free pages", 2: "a request's length is outside [0, max_pages * page_size]",
+           3: "more new tokens than max_tokens", 4: "more free pages than the pool has"}
+
+
+def _require(op: str, device: torch.device, **tensors) -> None:
+    """Every (tensor, dtype) on `device`, contiguous, of its dtype."""
+    for name, (t, dtype) in tensors.items():
+        if t.dtype != dtype:
+            raise NotImplementedError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+        if t.device != device:
+            raise RuntimeError(f"{op}: Expected all tensors to be on the same device, but found at least two devices, "
+                               f"{device} and {t.device} ({name})")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{op}: {name} must be contiguous")
+
+
+def _require_cuda(op: str, device: torch.device) -> None:
+    if device.type != "cuda":
+        raise NotImplementedError(f"{op}: this is the CUDA arm (sm_100a); a {device.type} tensor belongs to "
+                                  "torchnative's CPU path")
+
+
+def _call(device: torch.device, fn, *args) -> None:
+    """One library call on the device's current stream; the library takes the
+    current device, which may be another one."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch._C._cuda_getDevice():
+        N.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            N.check(fn(*args, stream))
+
+
+def _table_shape(op: str, page_table: torch.Tensor, lengths: torch.Tensor):
+    if page_table.dim() != 2 or lengths.dim() != 1 or page_table.shape[0] != lengths.shape[0]:
+        raise RuntimeError(f"{op}: page_table {list(page_table.shape)} and lengths {list(lengths.shape)} do not "
+                           "describe the same requests ([requests, max_pages] and [requests])")
+    return page_table.shape
+
+
+def _pool_shape(op: str, pool: torch.Tensor):
+    """(pages, KV heads, page size, head dimension) of a pool [pages, heads, page_size / 16, 18 D]."""
+    if pool.dim() != 4 or pool.shape[3] % 18:
+        raise RuntimeError(f"{op}: a pool is [pages, kv_heads, page_size / {GROUP}, 18 * head_dim], got "
+                           f"{list(pool.shape)}")
+    pages, heads, groups, row = pool.shape
+    return pages, heads, groups * GROUP, row // 18
+
+
+def kv_q4_pool(num_pages: int, kv_heads: int, head_dim: int, page_size: int, device="cuda") -> torch.Tensor:
+    """A zeroed pool: `num_pages` pages of `page_size` tokens of every KV head."""
+    if N.lib().tn_kv_q4_page_bytes(kv_heads, head_dim, page_size) < 0:
+        raise NotImplementedError(N.last_error())
+    return torch.zeros((num_pages, kv_heads, page_size // GROUP, 18 * head_dim), dtype=torch.uint8, device=device)
+
+
+def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Tensor,
+                    free_count: torch.Tensor, status: torch.Tensor, page_size: int, max_tokens: int, *,
+                    new_lengths: torch.Tensor | None = None, grow: int = 0):
+    """Take every request from its length to `new_lengths`, or, without them,
+    grow every request that has tokens by `grow`; returns (slots int64 and
+    positions int32 [max_tokens], query_start int32 [requests + 1]) of the new
+    tokens, packed request by request, -1 behind the last. Pages come from and
+    go back to the stack free_pages[:free_count]; page_table, lengths,
+    free_pages and free_count are updated in place. Nothing waits for the GPU:
+    a call that cannot be met changes nothing, gives no token a slot and sets
+    `status` (see `PagedQ4Cache.check`)."""
+    op = "kv_pages_resize"
+    device = page_table.device
+    i32 = torch.int32
+    _require_cuda(op, device)
+    _require(op, device, page_table=(page_table, i32), lengths=(lengths, i32), free_pages=(free_pages, i32),
+             free_count=(free_count, i32), status=(status, i32))
+    requests, max_pages = _table_shape(op, page_table, lengths)
+    if free_pages.dim() != 1 or free_count.numel() != 1 or status.numel() != 1:
+        raise RuntimeError(f"{op}: free_pages is [pages], free_count and status one number each")
+    if max_tokens < 0:
+        raise RuntimeError(f"{op}: max_tokens must not be negative, got {max_tokens}")
+    new = None
+    if new_lengths is not None:
+        if grow:
+            raise RuntimeError(f"{op}: new_lengths or grow, not both")
+        _require(op, device, new_lengths=(new_lengths, i32))
+        if new_lengths.shape != lengths.shape:
+            raise RuntimeError(f"{op}: new_lengths {list(new_lengths.shape)} do not fit lengths {list(lengths.shape)}")
+        new = new_lengths.data_ptr()
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
+    positions = torch.empty(max_tokens, dtype=i32, device=device)
+    query_start = torch.empty(requests + 1, dtype=i32, device=device)
+    _call(device, N.lib().tn_kv_pages_resize, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
+          int(grow), requests, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size,
+          slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr())
+    return slots, positions, query_start
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t [tokens, heads, D] with the unit inner stride and 16-byte aligned rows the kernels read, copied if need be."""
+    es = t.element_size()
+    if (t.stride(2) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) * es % 16)
+            or (t.shape[1] > 1 and t.stride(1) * es % 16)):
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _row_strides(t: torch.Tensor):
+    """Element strides of token and head; a size-1 dimension is never stepped through."""
+    return (ctypes.c_int64 * 2)(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def kv_q4_append(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise key and value [tokens, kv_heads, D] (float32, float16 or
+    bfloat16) into the pool at `slots` (int64 [tokens], all different; a
+    negative one skips its token), in place. Codes and scales are those of
+    `torch._C._quantize(..., "q4_0")`."""
+    op = "kv_q4_append"
+    device = pool.device
+    _require_cuda(op, device)
+    _require(op, device, pool=(pool, torch.uint8), slots=(slots, torch.int64))
+    pages, heads, page_size, dim = _pool_shape(op, pool)
+    if key.dtype not in _CODE or value.dtype != key.dtype:
+        raise NotImplementedError(f"{op}: key and value must both be float32, float16 or bfloat16, got {key.dtype} and "
+                                  f"{value.dtype}")
+    if key.device != device or value.device != device:
+        raise RuntimeError(f"{op}: Expected all tensors to be on the same device")
+    tokens = slots.shape[0]
+    if slots.dim() != 1 or tuple(key.shape) != (tokens, heads, dim) or key.shape != value.shape:
+        raise RuntimeError(f"{op}: key {list(key.shape)}, value {list(value.shape)} and slots {list(slots.shape)} do "
+                           f"not fit a pool of {heads} heads of {dim}")
+    key, value = _rows(key), _rows(value)
+    _call(device, N.lib().tn_kv_q4_append, key.data_ptr(), value.data_ptr(), _CODE[key.dtype], _row_strides(key),
+          _row_strides(value), tokens, slots.data_ptr(), pool.data_ptr(), pages, heads, dim, page_size)
+
+
+def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *,
+                  query_start: torch.Tensor | None = None, max_tokens: int | None = None, scale: float | None = None):
+    """(out, logsumexp) of attention over the cache. query [tokens, heads, D]
+    holds the requests' query tokens packed, those of request b in rows
+    query_start[b] to query_start[b + 1] (None: one each); they are the last of
+    its lengths[b] cached tokens, and each sees the tokens up to its own. A
+    token that sees none gives zeros and logsumexp 0; rows behind the last
+    request's are not written. `max_tokens`, a bound on one request's query
+    tokens, chooses the kernel (None: all of them)."""
+    op = "sdpa_q4_cache"
+    device = query.device
+    _require_cuda(op, device)
+    if query.dtype not in _CODE:
+        raise NotImplementedError(f"{op}: the query must be float32, float16 or bfloat16, got {query.dtype}")
+    _require(op, device, pool=(pool, torch.uint8), page_table=(page_table, torch.int32),
+             lengths=(lengths, torch.int32))
+    pages, kv_heads, page_size, dim = _pool_shape(op, pool)
+    requests, max_pages = _table_shape(op, page_table, lengths)
+    if query.dim() != 3 or query.shape[2] != dim:
+        raise RuntimeError(f"{op}: query {list(query.shape)} must be [tokens, heads, {dim}]")
+    tokens, heads = query.shape[:2]
+    start = None
+    if query_start is not None:
+        _require(op, device, query_start=(query_start, torch.int32))
+        if query_start.numel() != requests + 1:
+            raise RuntimeError(f"{op}: query_start must have requests + 1 = {requests + 1} entries, got "
+                               f"{query_start.numel()}")
+        start = query_start.data_ptr()
+    most = 1 if start is None else tokens if max_tokens is None else min(max_tokens, tokens)
+    query = _rows(query)
+    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
+    lib = N.lib()
+    ws = torch.empty(lib.tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, dim, most), dtype=torch.uint8,
+                     device=device)
+    _call(device, lib.tn_sdpa_q4_cache, query.data_ptr(), _CODE[query.dtype], _row_strides(query), tokens, heads,
+          pool.data_ptr(), pages, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages,
+          lengths.data_ptr(), requests, start, most, out.data_ptr(), lse.data_ptr(), 0.0 if scale is None else
+          float(scale), ws.data_ptr(), ws.numel())
+    return out, lse
+
+
+def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
+                        lengths: torch.Tensor, heads: int, *, scale: float | None = None, q8=None) -> torch.Tensor:
+    """One decode token's attention block of every request, bf16: from the
+    projection rows qkv [requests, (heads + 2 kv_heads) D], rotate q and k at
+    position lengths - 1 (rows of `rope` [positions, D]: cosines, then sines),
+    append k and v there in 4 bits, attend. Returns [requests, heads, D]; q8 =
+    (codes int8 [requests, heads D], scales and offsets float32 [requests,
+    heads D / 32]) also receives its planar Q8_0, the next linear's
+    activations. A request of length 0 appends nothing and gives zeros."""
+    op = "sdpa_q4_decode_step"
+    device = qkv.device
+    _require_cuda(op, device)
+    bf = torch.bfloat16
+    _require(op, device, qkv=(qkv, bf), rope=(rope, bf), pool=(pool, torch.uint8), page_table=(page_table, torch.int32),
+             lengths=(lengths, torch.int32))
+    pages, kv_heads, page_size, dim = _pool_shape(op, pool)
+    requests, max_pages = _table_shape(op, page_table, lengths)
+    if tuple(qkv.shape) != (requests, (heads + 2 * kv_heads) * dim):
+        raise RuntimeError(f"{op}: qkv {list(qkv.shape)} must be [{requests}, {(heads + 2 * kv_heads) * dim}]")
+    if rope.dim() != 2 or rope.shape[1] != dim:
+        raise RuntimeError(f"{op}: rope {list(rope.shape)} must be [positions, {dim}]")
+    codes = scales = offsets = None
+    if q8 is not None:
+        codes, scales, offsets = q8
+        _require(op, device, codes=(codes, torch.int8), scales=(scales, torch.float32), offsets=(offsets, torch.float32))
+        if codes.numel() != requests * heads * dim or not scales.numel() == offsets.numel() == codes.numel() // 32:
+            raise RuntimeError(f"{op}: q8 must be codes [{requests}, {heads * dim}], scales and offsets "
+                               f"[{requests}, {heads * dim // 32}]")
+        codes, scales, offsets = codes.data_ptr(), scales.data_ptr(), offsets.data_ptr()
+    out = torch.empty((requests, heads, dim), dtype=bf, device=device)
+    lib = N.lib()
+    ws = torch.empty(lib.tn_sdpa_q4_workspace_bytes(requests, heads, kv_heads, dim, 1), dtype=torch.uint8,
+                     device=device)
+    _call(device, lib.tn_sdpa_q4_decode_step, qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
+          heads, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
+          out.data_ptr(), None, codes, scales, offsets, 0.0 if scale is None else float(scale), ws.data_ptr(),
+          ws.numel())
+    return out
+
+
+def kv_q4_dense(pool: torch.Tensor):
+    """(keys, values) of a pool as float32 [pages, kv_heads, page_size, D]: the
+    values its codes stand for, by plain torch operations on any device. For
+    looking into a cache; attention reads the pool itself."""
+    op = "kv_q4_dense"
+    pages, heads, page_size, dim = _pool_shape(op, pool)
+    nb = dim // 32
+    kc, ks, vc, vs = pool.split([8 * dim, dim, 8 * dim, dim], -1)
+
+    def nibbles(u):
+        return torch.stack((u & 15, u >> 4), -1).flatten(-2)
+
+    k = nibbles(kc.unflatten(-1, (16, 4, nb, 4)))[..., [0, 4, 1, 5, 2, 6, 3, 7]]  # token, t, block, element 8t + i
+    k = k.transpose(-3, -2).flatten(-2)
+    v = nibbles(vc.unflatten(-1, (2, 8, 4, nb, 2, 2)))  # h, g, t, block, p, element 4g + n
+    v = v.permute(0, 1, 2, 3, 5, 7, 6, 4, 8).flatten(3, 5).flatten(-2)
+    return tuple(((c.float() - 8.0) * s.contiguous().view(torch.float16).unflatten(-1, (16, nb)).float()[..., None])
+                 .reshape(pages, heads, page_size, dim) for c, s in ((k, ks), (v, vs)))
+
+
+class PagedQ4Cache:
+    """The 4-bit KV cache of a model: one pool a layer, and the block table,
+    lengths and free pages that all layers share. `num_pages` pages of
+    `page_size` tokens serve up to `max_requests` requests of up to
+    `max_pages` pages each."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, num_pages: int, max_requests: int, max_pages: int,
+                 page_size: int = 64, device="cuda"):
+        device = torch.device(device)
+        _require_cuda("PagedQ4Cache", device)
+        self.page_size = page_size
+        self.pools = [kv_q4_pool(num_pages, kv_heads, head_dim, page_size, device) for _ in range(layers)]
+        i32 = dict(dtype=torch.int32, device=device)
+        self.page_table = torch.full((max_requests, max_pages), -1, **i32)
+        self.lengths = torch.zeros(max_requests, **i32)
+        # the top of the stack is its end: page 0 is taken first
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
+        self.free_count = torch.full((1,), num_pages, **i32)
+        self.status = torch.zeros(1, **i32)
+
+    def nbytes(self) -> int:
+        return sum(p.numel() for p in self.pools)
+
+    def resize(self, max_tokens: int, *, new_lengths: torch.Tensor | None = None, grow: int = 0):
+        """`kv_pages_resize` of this cache: (slots, positions, query_start)."""
+        return kv_pages_resize(self.page_table, self.lengths, self.free_pages, self.free_count, self.status,
+                               self.page_size, max_tokens, new_lengths=new_lengths, grow=grow)
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor) -> None:
+        kv_q4_append(key, value, self.pools[layer], slots)
+
+    def attend(self, layer: int, query: torch.Tensor, *, query_start=None, max_tokens=None, scale=None):
+        return sdpa_q4_cache(query, self.pools[layer], self.page_table, self.lengths, query_start=query_start,
+                             max_tokens=max_tokens, scale=scale)
+
+    def decode_step(self, layer: int, qkv: torch.Tensor, rope: torch.Tensor, heads: int, *, scale=None, q8=None):
+        return sdpa_q4_decode_step(qkv, rope, self.pools[layer], self.page_table, self.lengths, heads, scale=scale,
+                                   q8=q8)
+
+    def check(self) -> None:
+        """Wait for the GPU and raise for a resize that could not be met since
+        the last check, or a page, slot or position outside its range."""
+        code = int(self.status.item())
+        self.status.zero_()
+        if code:
+            raise RuntimeError(f"kv_pages_resize: {_STATUS.get(code, code)}; that call changed nothing")
+        N.device_status()
