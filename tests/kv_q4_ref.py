@@ -54,10 +54,14 @@ def attention(q, pool, table, lengths, page_size, query_start=None, scale=None):
       the exponential, its argument and the running maximum add 2^-20 and 2^-23 |s| (arguments in float32 units of
       log 2 are subtracted once the product is rounded), so a probability is off by e = 2 max(ds + 2^-22 |s|) + 2^-20
       relative (numerator and denominator);
-      a probability times a value's scale is rounded once more: half a step of its carrier h;
+      a probability times a value's scale is rounded to the carrier, half a step of it; for bfloat16 results the
+      probability is rounded to it before as well, 2 * 2^-11 in all, an eighth of the step of the result;
       sums over n keys in at most n / 16 + 64 additions of partial sums: (n / 16 + 64) 2^-24;
+      below float16's normal numbers those roundings are half a subnormal step, 2^-25, where the row's largest
+      probability, times a scale of the larger of 1 and twice the largest scale d, stands for 2^10 at least: at most
+      2 * 2^-35 max(1, 2 d), times a code of at most 8, for every key that the row sees;
       the result is rounded to its type: half a step of its value, or half the spacing of the subnormals."""
-    h = 2.0**-22 if q.dtype == torch.float32 else 2.0**-11
+    h = {torch.float32: 2.0**-22, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-10}[q.dtype]
     step = HALF_STEP[q.dtype]
     t, hq, dim = q.shape
     scale = 1 / math.sqrt(dim) if scale is None else scale
@@ -89,7 +93,9 @@ def attention(q, pool, table, lengths, page_size, query_start=None, scale=None):
         o = p @ v
         out[rows] = o.transpose(0, 1)
         lse[rows] = torch.where(some, e, 0.0).transpose(0, 1)
-        bound[rows] = ((rel + h)[..., None] * (p @ v.abs()) + (step * o.abs()).clamp(min=HALF_SUBNORMAL[q.dtype]) + 1e-30).transpose(0, 1)
+        dmax = v.abs().amax() / 8  # the largest element of a block has code 0: eight scales
+        floor = sees.sum(-1)[:, None] * 16 * 2.0**-35 * max(1.0, 2 * dmax.item())
+        bound[rows] = ((rel + h)[..., None] * (p @ v.abs()) + floor + (step * o.abs()).clamp(min=HALF_SUBNORMAL[q.dtype]) + 1e-30).transpose(0, 1)
         lse_bound[rows] = (rel + 2.0**-22 * e.abs()).transpose(0, 1)
     return out, lse, bound, lse_bound
 

@@ -22,24 +22,6 @@ struct Append {
     int *err;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(src);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned short u = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
-            T e;
-            memcpy(&e, &u, 2);
-            x[i] = to_f32<T>(e);
-        }
-    }
-}
-
 // Work item: one block of one row, four lanes. Items run over blocks, then K
 // and V, then heads, then tokens.
 template <typename T, int D>

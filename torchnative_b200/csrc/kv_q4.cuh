@@ -102,6 +102,27 @@ int check_kv_pool(const char *op, const void *pool, int64_t num_pages, int64_t k
                   int64_t page_size);
 int kv_page_shift(int64_t page_size);  // log2 of a page size the cache takes, else -1
 
+// Eight neighbouring elements (16-byte aligned), widened.
+template <typename T>
+__device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4 *>(src);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned short u = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+            T e;
+            memcpy(&e, &u, 2);
+            x[i] = to_f32<T>(e);
+        }
+    }
+}
+
+__device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+
 // The Q4_0 code of x in a block with reciprocal scale `inv`: trunc(x * inv + 8.5)
 // in [0, 15], NaN to 0 (Rust's `as u8`, then min 15). Explicitly rounded, so
 // that no contraction changes a byte.

@@ -5,6 +5,10 @@
 //   s_j = scale * q . (d_j * (code_j - 8)),  out = sum_j e^(s_j - m) v_j / l,
 //   lse = m + log l;
 // a token that sees no key gives zeros and lse 0, as the dense operator does.
+#include <algorithm>
+#include <atomic>
+#include <chrono>
+
 #include "kv_q4.cuh"
 
 namespace tn {
@@ -21,162 +25,879 @@ struct Attend {
     float scale;
 };
 
-// The request of packed token r and the number of its keys that r sees; -1 for
-// a row behind the last request's.
-__device__ __forceinline__ int request_of(const Attend &p, int r, int *keys) {
-    int b = r, first = r, n = 1;
-    if (p.query_start) {
-        int lo = 0, hi = p.c.requests;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (p.query_start[mid] <= r)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        b = lo;
-        first = p.query_start[b];
-        n = p.query_start[b + 1] - first;
-        if (r < first || r >= first + n) return -1;
-    }
-    *keys = p.c.length(b) - n + (r - first) + 1;
-    return b;
-}
+// ---- the split kernel: few query rows against a long cache
+//
+// One unit of work is one group of 16 tokens of one (request, row tile, KV
+// head); a row tile is 8 NT of the request's query rows (tokens times the heads
+// that share the KV head). All units of a call stand in one line, and CTA c of G
+// takes units [c W / G, (c + 1) W / G): every CTA gets the same number whatever
+// the lengths, which only the device knows. Inside a CTA the units go round the
+// warps; a warp brings its groups (18 D bytes, one bulk copy each) into a ring of
+// its own and needs no other warp until an item (request, tile, head) ends.
+//
+// Per group a warp computes, with m16n8k16 tensor instructions,
+//   S^T[16 keys, 8 rows] = sum over blocks b of d_k[key, b] * (codes_b . q_b)
+//   O^T[D, 8 rows] += sum over blocks: codes_b^T . (p[key, row] * d_v[key, b])
+// so that the 4-bit codes enter the products as the small integers they are
+// (exact in f16), the tall side of both products is the cache's, and a tile of 8
+// rows wastes nothing. A code costs about 1.1 instructions to unpack: masks put
+// the nibble below a float16 exponent (1024 + c, or 64 + c for a nibble at bit
+// 4), and 1032 or 72 goes off again, for a part of K in the accumulators' start.
+// The scores' fragment is turned into the second product's operand by a register
+// transpose (movmatrix).
+//
+// p is 2^(s - ref) times 2^10, f16, where ref follows the row's maximum by more
+// than 2^5 only (a vote per group; out = O / l holds for any ref), and goes down
+// when the value scales are above 1, so that p * d_v stays in f16's range.
 
-constexpr int kSimpleThreads = 128;
-
-// One CTA for one (token, head): a thread per key, then a thread per dimension.
-template <typename T, int D>
-__global__ void __launch_bounds__(kSimpleThreads) sdpa_q4_simple_kernel(const Attend p) {
-    using Q = KvQ4<D>;
-    __shared__ float q[D], s[kSimpleThreads], part[kSimpleThreads], red[4];
-    __shared__ const uint8_t *groups[kSimpleThreads / 16];
-    const int tid = threadIdx.x, r = blockIdx.x, h = blockIdx.y, lane = tid & 31, warp = tid >> 5;
-    pdl_launch_dependents();
-    pdl_wait();
-    int keys = 0;
-    const int b = request_of(p, r, &keys);
-    if (b < 0) return;
-    for (int d = tid; d < D; d += kSimpleThreads)
-        q[d] = to_f32<T>(static_cast<const T *>(p.q)[r * p.q_token + h * p.q_head + d]);
-    constexpr int HALVES = kSimpleThreads / D;  // key halves of the second product
-    const int dim = tid % D, half = tid / D;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int j0 = 0; j0 < keys; j0 += kSimpleThreads) {
-        __syncthreads();
-        if (tid < kSimpleThreads / 16)
-            groups[tid] = j0 + tid * 16 < keys ? p.c.group<D>(b, h / p.rep, j0 / 16 + tid) : nullptr;
-        __syncthreads();
-        const uint8_t *g = groups[tid / 16];
-        float x = -INFINITY;
-        if (j0 + tid < keys && g) {
-            x = 0.0f;
-            for (int block = 0; block < Q::NB; ++block) {
-                float dot = 0.0f;
-                for (int t = 0; t < 4; ++t) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t *>(g + Q::k_word(tid & 15, t, block));
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                        dot = fmaf((float)((int)((w >> (4 * n)) & 15) - 8), q[block * 32 + t * 8 + 2 * (n & 3) + (n >> 2)],
-                                   dot);
-                }
-                x = fmaf(dot, __half2float(*reinterpret_cast<const __half *>(g + Q::k_scale(tid & 15, block))), x);
-            }
-            x *= p.scale;
-        }
-        float mx = x;
-#pragma unroll
-        for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-        if (lane == 0) red[warp] = mx;
-        __syncthreads();
-        mx = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float alpha = mx == -INFINITY ? 1.0f : expf(m - mx);
-        s[tid] = x == -INFINITY ? 0.0f : expf(x - mx);
-        m = mx;
-        __syncthreads();
-        l *= alpha;
-        o *= alpha;
-        for (int j = 0; j < kSimpleThreads; ++j) l += s[j];
-        for (int j = half; j < min(kSimpleThreads, keys - j0); j += HALVES) {
-            const uint8_t *v = groups[j / 16];
-            if (!v) continue;
-            const uint32_t w = *reinterpret_cast<const unsigned short *>(v + Q::v_half(j & 15, dim % 32 / 4, dim / 32));
-            const float d = __half2float(*reinterpret_cast<const __half *>(v + Q::v_scale(j & 15, dim / 32)));
-            o = fmaf(s[j] * d, (float)((int)((w >> (4 * (dim & 3))) & 15) - 8), o);
-        }
-    }
-    part[tid] = o;
-    __syncthreads();
-    if (tid < D) {
-        float v = 0.0f;
-        for (int i = 0; i < HALVES; ++i) v += part[i * D + tid];
-        const int64_t at = ((int64_t)r * p.heads + h) * D + tid;
-        v = l == 0.0f ? 0.0f : v / l;
-        if constexpr (sizeof(T) == 4)
-            static_cast<float *>(p.out)[at] = v;
-        else if constexpr (std::is_same<T, __half>::value)
-            static_cast<__half *>(p.out)[at] = __float2half_rn(v);
-        else
-            static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(v);
-        if (tid == 0 && p.lse) p.lse[(int64_t)r * p.heads + h] = l == 0.0f ? 0.0f : m + logf(l);
-    }
-}
-
-template <typename T, int D>
-int launch_attend(const Attend &p, cudaStream_t stream) {
-    return launch_pdl(sdpa_q4_simple_kernel<T, D>, dim3((unsigned)p.tokens, (unsigned)p.heads), dim3(kSimpleThreads), 0,
-                      stream, "tn_sdpa_q4_cache", p);
-}
-
-// Rotates the q and k heads of one projection row at the request's last
-// position and appends k and v there: q_out [B][heads][D].
 template <int D>
-__global__ void rope_append_q4_kernel(const __nv_bfloat16 *qkv, const __nv_bfloat16 *rope, int64_t rope_rows, KvPool c,
-                                      int heads, __nv_bfloat16 *q_out) {
-    using Q = KvQ4<D>;
-    __shared__ float row[D];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int b = blockIdx.y, h = blockIdx.x, W = heads + 2 * c.kv_heads, i = threadIdx.x;
-    const __nv_bfloat16 *x = qkv + ((int64_t)b * W + h) * D;
-    const int pos = c.length(b) - 1;
-    if (pos >= 0 && pos >= rope_rows) record_device_error(c.err, DEV_ERR_BAD_PAGE);
-    const int at = (int)max((int64_t)0, min((int64_t)pos, rope_rows - 1));
-    if (i < D / 2) {
-        const float cs = __bfloat162float(rope[(int64_t)at * D + i]), sn = __bfloat162float(rope[(int64_t)at * D + D / 2 + i]);
-        float a = __bfloat162float(x[i]), e = __bfloat162float(x[i + D / 2]);
-        if (h < heads + c.kv_heads) {
-            const float a2 = a * cs - e * sn, e2 = e * cs + a * sn;
-            a = a2, e = e2;
-        }
-        row[i] = __bfloat162float(__float2bfloat16_rn(a));
-        row[i + D / 2] = __bfloat162float(__float2bfloat16_rn(e));
+struct Ring {
+    static constexpr int WARPS = 8, STAGES = 4;
+    static constexpr int BYTES = WARPS * STAGES * KvQ4<D>::GROUP_BYTES;
+    static constexpr int ROW = D + 4;  // floats of a row of the merge buffer: rows 2t of a fragment differ in their banks
+    static constexpr int MERGE = WARPS * 8 * ROW * 4;
+    static constexpr int SMEM = BYTES + MERGE;
+};
+
+constexpr int kSplitThreads = 256;
+constexpr float kBias = 10.0f, kSlack = 5.0f;
+
+struct Split {
+    Attend a;
+    int min_units;        // units a CTA should have before another one is used
+    float *part_o;        // [grid][2][8 NT][D]
+    float *part_ml;       // [grid][2][8 NT][2]
+    unsigned long long *flags;  // [grid][2]
+    unsigned long long nonce;
+    // decode step
+    const __nv_bfloat16 *qkv, *rope;
+    int64_t rope_rows;
+    int8_t *codes;
+    float *scales, *offsets;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, const float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+
+// The nibbles n and n + 4 of a word as half2, n = 0 .. 3: codes minus 8, except
+// that with RAW the odd ones come as 64 + code.
+template <bool RAW>
+__device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&e)[4]) {
+    constexpr uint32_t kLow = 0x64086408u, kHigh = 0x54805480u;  // 1032, 72
+    const uint32_t u = w >> 8;
+    e[0] = sub_f16x2((w & 0x000f000fu) | 0x64006400u, kLow);
+    e[1] = (w & 0x00f000f0u) | 0x54005400u;
+    e[2] = sub_f16x2((u & 0x000f000fu) | 0x64006400u, kLow);
+    e[3] = (u & 0x00f000f0u) | 0x54005400u;
+    if constexpr (!RAW) {
+        e[1] = sub_f16x2(e[1], kHigh);
+        e[3] = sub_f16x2(e[3], kHigh);
     }
-    __syncthreads();
-    if (h < heads) {
-        for (int d = i; d < D; d += blockDim.x) q_out[((int64_t)b * heads + h) * D + d] = __float2bfloat16_rn(row[d]);
+}
+
+// A place in the line of units: group g of G of item (b, tile u, head h).
+template <int RT>
+struct Cursor {
+    int b, u, h, g, G;
+    int S, n, first, tiles;
+
+    __device__ __forceinline__ void load_request(const Attend &p) {
+        S = p.c.length(b);
+        first = b;
+        n = 1;
+        if (p.query_start) {
+            first = min(max(p.query_start[b], 0), p.tokens);
+            n = max(min(p.query_start[b + 1], p.tokens) - first, 0);
+        }
+        tiles = (n * p.rep + RT - 1) / RT;
+    }
+    // groups that the tile's last row sees; 1 where it sees none, so that someone writes its zeros
+    __device__ __forceinline__ int tile_groups(const Attend &p, int tile) const {
+        const int last = min(n - 1, (tile * RT + RT - 1) / p.rep);
+        return max(1, (S - n + last + 16) >> 4);
+    }
+    __device__ __forceinline__ long long request_units(const Attend &p) const {
+        long long units = 0;
+        for (int t = 0; t < tiles; ++t) units += tile_groups(p, t);
+        return units * p.c.kv_heads;
+    }
+    __device__ __forceinline__ void next_item(const Attend &p) {
+        if (++h < p.c.kv_heads) return;
+        h = 0;
+        if (++u >= tiles) {
+            u = 0;
+            do {
+                if (++b >= p.c.requests) {
+                    G = INT32_MAX;  // behind the last unit
+                    return;
+                }
+                load_request(p);
+            } while (tiles == 0);
+        }
+        G = tile_groups(p, u);
+    }
+    __device__ __forceinline__ void advance(const Attend &p, int by) {
+        g += by;
+        while (g >= G && b < p.c.requests) {
+            g -= G;
+            next_item(p);
+        }
+    }
+};
+
+// The rotary embedding of the lane's elements (32 b + 8 t .. + 7 of every block
+// b) of a row: halves rotated against each other, rounded once, to bf16.
+template <int D>
+__device__ __forceinline__ void rotate(const __nv_bfloat16 *rope, int t, float (&x)[D / 32][8]) {
+    constexpr int H = D / 64;
+#pragma unroll
+    for (int b = 0; b < H; ++b) {
+        float c[8], s[8];
+        load8<__nv_bfloat16>(rope + b * 32 + t * 8, c);
+        load8<__nv_bfloat16>(rope + D / 2 + b * 32 + t * 8, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x1 = x[b][i], x2 = x[b + H][i];
+            x[b][i] = round_bf16(x1 * c[i] - x2 * s[i]);
+            x[b + H][i] = round_bf16(x2 * c[i] + x1 * s[i]);
+        }
+    }
+}
+
+// One warp: the new token's key (rotated) and value of head h at position pos,
+// in 4 bits, into the group's copy in shared memory and into the cache.
+template <int D>
+__device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos, uint8_t *buf) {
+    using Q = KvQ4<D>;
+    constexpr int NB = Q::NB, H = D / 64;
+    const Attend &a = p.a;
+    if (pos >= p.rope_rows) {
+        record_device_error(a.c.err, DEV_ERR_BAD_PAGE);
         return;
     }
-    if (pos < 0 || pos >= rope_rows) return;
-    const int kvh = (h - heads) % c.kv_heads, is_v = h >= heads + c.kv_heads, key = pos & 15;
-    uint8_t *g = c.group<D>(b, kvh, pos >> 4);
-    if (!g || i >= 32) return;
-    float v[8];
-    const int block = (i >> 2) % Q::NB, t = i & 3;
+    const int lane = threadIdx.x & 31, t = lane & 3, block = (lane >> 2) % NB, is_v = (lane >> 2) / NB % 2;
+    const __nv_bfloat16 *row = p.qkv + ((int64_t)b * (a.heads + 2 * a.c.kv_heads) + a.heads + (is_v ? a.c.kv_heads : 0) + h) * D;
+    float x[8];
+    load8<__nv_bfloat16>(row + block * 32 + t * 8, x);
+    if (!is_v) {
+        const int first = block % H;
+        float y[8], c[8], s[8];
+        load8<__nv_bfloat16>(row + (block + H) % NB * 32 + t * 8, y);
+        load8<__nv_bfloat16>(p.rope + (int64_t)pos * D + first * 32 + t * 8, c);
+        load8<__nv_bfloat16>(p.rope + (int64_t)pos * D + D / 2 + first * 32 + t * 8, s);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = row[block * 32 + t * 8 + e];
-    const float d = __fdiv_rn(q4_0_extreme(v), -8.0f);
-    const float inv = (d != 0.0f) ? __fdiv_rn(1.0f, d) : 0.0f;
-    if (i >= 4 * Q::NB) return;
-    if (is_v) {
-        const uint32_t w = q4_0_v_halves(v, inv);
-        *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t, block)) = (unsigned short)w;
-        *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t + 1, block)) = (unsigned short)(w >> 16);
-    } else {
-        *reinterpret_cast<uint32_t *>(g + Q::k_word(key, t, block)) = q4_0_k_word(v, inv);
+        for (int i = 0; i < 8; ++i) x[i] = round_bf16(block < H ? x[i] * c[i] - y[i] * s[i] : x[i] * c[i] + y[i] * s[i]);
     }
-    if (t == 0)
-        *reinterpret_cast<__half *>(g + (is_v ? Q::v_scale(key, block) : Q::k_scale(key, block))) = __float2half_rn(d);
+    const float d = __fdiv_rn(q4_0_extreme(x), -8.0f);
+    const float inv = (d != 0.0f) ? __fdiv_rn(1.0f, d) : 0.0f;
+    uint8_t *group = a.c.group<D>(b, h, pos >> 4);
+    if (!group || lane >= 8 * NB) return;
+    const int key = pos & 15;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        uint8_t *g = k ? group : buf;
+        if (is_v) {
+            const uint32_t w = q4_0_v_halves(x, inv);
+            *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t, block)) = (unsigned short)w;
+            *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t + 1, block)) = (unsigned short)(w >> 16);
+        } else {
+            *reinterpret_cast<uint32_t *>(g + Q::k_word(key, t, block)) = q4_0_k_word(x, inv);
+        }
+        if (t == 0)
+            *reinterpret_cast<__half *>(g + (is_v ? Q::v_scale(key, block) : Q::k_scale(key, block))) = __float2half_rn(d);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(void *out, int64_t at, const float (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        T e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value)
+                e[i] = __float2half_rn(v[i]);
+            else
+                e[i] = __float2bfloat16_rn(v[i]);
+        }
+        uint2 w;
+        memcpy(&w, e, 8);
+        *reinterpret_cast<uint2 *>(static_cast<T *>(out) + at) = w;
+    }
+}
+
+// Four finished values of one row (d .. d + 3 of query head hq of packed token r).
+template <typename T, int D, bool STEP>
+__device__ __forceinline__ void finish4(const Split &p, int r, int hq, int d, const float (&v)[4]) {
+    const int64_t at = ((int64_t)r * p.a.heads + hq) * D + d;
+    store4<T>(p.a.out, at, v);
+    if constexpr (STEP) {
+        if (p.codes) {
+            // planar Q8_0 (k_quants.rs:676-706) of the bf16 output: 8 neighbouring lanes hold a block of 32
+            const unsigned gm = 0xffu << (threadIdx.x & 24);
+            float q[4], amax = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                q[e] = __bfloat162float(__float2bfloat16_rn(v[e]));
+                amax = fmaxf(amax, fabsf(q[e]));
+            }
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(gm, amax, off));
+            const float dq = __fdiv_rn(amax, 127.0f), id = (dq != 0.0f) ? __fdiv_rn(1.0f, dq) : 0.0f;
+            uint32_t word = 0;
+            int sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float t = roundf(__fmul_rn(q[e], id));
+                const int c = !(t == t) ? 0 : (t <= -128.0f ? -128 : (t >= 127.0f ? 127 : __float2int_rz(t)));
+                sum += c;
+                word |= (uint32_t)(c & 0xff) << (8 * e);
+            }
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) sum += __shfl_xor_sync(gm, sum, off);
+            *reinterpret_cast<uint32_t *>(p.codes + at) = word;
+            if ((threadIdx.x & 7) == 0) {
+                p.scales[at / 32] = __half2float(__float2half_rn(dq));
+                p.offsets[at / 32] = 12582912.0f + 8.0f * (float)sum;
+            }
+        }
+    }
+}
+
+template <typename T, int D, int NT, bool STEP>
+__global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_kernel(const Split p) {
+    using Q = KvQ4<D>;
+    using R = Ring<D>;
+    constexpr int NB = Q::NB, RT = 8 * NT, W = R::WARPS;
+    constexpr bool F32 = sizeof(T) == 4, BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int NQ = F32 ? 2 : 1;   // f16 terms of a query element
+    constexpr int NP = BF ? 1 : 2;    // f16 terms of a probability
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[W][R::STAGES];
+    __shared__ float ml_sm[W][8][2];
+    __shared__ int is_last;
+    float *merge = reinterpret_cast<float *>(smem + R::BYTES);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lg = lane >> 2, lt = lane & 3;
+    uint8_t *ring = smem + warp * R::STAGES * Q::GROUP_BYTES;
+    if (lane == 0) {
+        for (int s = 0; s < R::STAGES; ++s) mbar_init(&bars[warp][s], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // ---- this CTA's units
+    const Attend &a = p.a;
+    Cursor<RT> at;
+    long long total = 0;
+    for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
+        long long w = 0;
+        at.b = b0 + lane;
+        if (at.b < a.c.requests) {
+            at.load_request(a);
+            w = at.request_units(a);
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) w += __shfl_xor_sync(0xffffffffu, w, off);
+        total += w;
+    }
+    if (total == 0) return;
+    const int grid = (int)min((long long)gridDim.x, max(1ll, total / p.min_units));
+    const int cta = blockIdx.x;
+    if (cta >= grid) return;
+    const long long lo = cta * total / grid, hi = (cta + 1) * total / grid;
+    long long item0 = 0;  // line position of the current item's first unit
+    {
+        long long before = 0;
+        for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
+            long long w = 0;
+            at.b = b0 + lane;
+            if (at.b < a.c.requests) {
+                at.load_request(a);
+                w = at.request_units(a);
+            }
+            long long upto = w;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, upto, off);
+                if (lane >= off) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > lo);
+            if (past) {
+                const int l0 = __ffs(past) - 1;
+                item0 = before + __shfl_sync(0xffffffffu, upto - w, l0);
+                at.b = b0 + l0;
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        at.load_request(a);
+        at.u = at.h = 0;
+        for (;; ++at.u) {  // the tile, then the head
+            at.G = at.tile_groups(a, at.u);
+            const long long units = (long long)at.G * a.c.kv_heads;
+            if (item0 + units > lo) break;
+            item0 += units;
+        }
+        at.h = (int)((lo - item0) / at.G);
+        item0 += (long long)at.h * at.G;
+        at.g = (int)(lo - item0);
+    }
+
+    // ---- the ring: unit i of this CTA (i = warp, warp + W, ...) goes to stage (i / W) % STAGES
+    const int units = (int)(hi - lo);
+    Cursor<RT> ahead = at;
+    ahead.advance(a, warp);
+    int ahead_i = warp, ahead_k = 0, issued = 0;  // the next unit to bring, its place in the ring; units brought
+    bool broken = false;
+    uint32_t bad = 0;  // stages whose unit has no page
+    auto issue = [&]() {
+        if (ahead_i < units && !broken) {
+            ++issued;
+            const int s = ahead_k % R::STAGES;
+            const uint8_t *src = nullptr;
+            if (ahead.g * kKvGroup < ahead.S) src = a.c.group<D>(ahead.b, ahead.h, ahead.g);
+            bad = src ? bad & ~(1u << s) : bad | (1u << s);
+            if (src && lane == 0) {
+                mbar_arrive_expect_tx(&bars[warp][s], Q::GROUP_BYTES);
+                bulk_g2s(ring + s * Q::GROUP_BYTES, src, Q::GROUP_BYTES, &bars[warp][s]);
+            } else if (!src && lane == 0) {
+                mbar_arrive(&bars[warp][s]);
+            }
+        }
+        ahead.advance(a, W);
+        ahead_i += W;
+        ++ahead_k;
+    };
+    for (int s = 0; s < R::STAGES - 1; ++s) issue();
+
+    int done_i = 0, my_i = warp, my_k = 0;  // units of finished items; this warp's next unit
+    int broken_k = 0;
+    while (done_i < units) {
+        // ---- one item, or this CTA's part of it: groups [at.g, at.g + count)
+        const int count = min(at.G - at.g, units - done_i);
+        const int g0 = at.g - done_i;  // unit i is group g0 + i
+        const int rows = min(RT, at.n * a.rep - at.u * RT);
+        const int row0 = at.u * RT;
+
+        // ---- queries as the first product's B fragments: lane (g, t) holds row g, elements 32 b + 8 t .. + 7
+        uint32_t qf[NT][NB][NQ][4];
+        float start[NT][NB][2];  // what a score's accumulator starts from, for the columns 2t, 2t + 1
+        float to_log2[NT][2];
+        int limit[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int row = nt * 8 + lg;
+            float x[NB][8];
+            const bool live = row < rows;
+            const int tok = (row0 + row) / a.rep, hq = at.h * a.rep + (row0 + row) % a.rep;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
+            if (live) {
+                const T *src;
+                if constexpr (STEP)
+                    src = reinterpret_cast<const T *>(p.qkv) + ((int64_t)at.b * (a.heads + 2 * a.c.kv_heads) + hq) * D;
+                else
+                    src = static_cast<const T *>(a.q) + (at.first + tok) * a.q_token + hq * a.q_head;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) load8<T>(src + b * 32 + lt * 8, x[b]);
+            }
+            if constexpr (STEP) {
+                const int64_t pos = max((int64_t)0, min((int64_t)at.S - 1, p.rope_rows - 1));
+                rotate<D>(p.rope + pos * D, lt, x);
+            }
+            // the row's largest magnitude goes to [2^13, 2^14): no element overflows f16, and one that loses bits there
+            // lies 2^27 below it
+            float scale = 1.0f, back = 1.0f;
+            if constexpr (!std::is_same<T, __half>::value) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[b][i]));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                if (amax > 0.0f && amax < INFINITY) {
+                    const int e = min(max(267 - (int)(__float_as_uint(amax) >> 23), 1), 253);
+                    scale = __uint_as_float((uint32_t)e << 23);
+                    back = __uint_as_float((uint32_t)(254 - e) << 23);
+                }
+            }
+            float sums[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                sums[b] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x0 = x[b][2 * j] * scale, x1 = x[b][2 * j + 1] * scale;
+                    qf[nt][b][0][j] = pack_f16(x0, x1);
+                    const float2 f = unpack_f16(qf[nt][b][0][j]);
+                    if constexpr (NQ == 2) qf[nt][b][1][j] = pack_f16(x0 - f.x, x1 - f.y);
+                    if (j & 1) sums[b] += f.x + f.y;
+                }
+                sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 1);
+                sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 2);
+            }
+            const int seen = live ? at.S - at.n + tok + 1 : 0;  // keys that row g sees
+            const float c = a.scale * 1.4426950408889634f * back;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int from = (2 * lt + j) * 4;
+                to_log2[nt][j] = __shfl_sync(0xffffffffu, c, from);
+                limit[nt][j] = __shfl_sync(0xffffffffu, seen, from);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    start[nt][b][j] = F32 ? 0.0f : -72.0f * __shfl_sync(0xffffffffu, sums[b], from);
+            }
+        }
+        // the fewest keys that a row of the tile sees: groups below need no mask
+        const int all_see = rows == RT ? at.S - at.n + row0 / a.rep + 1 : 0;
+
+        float o[NT][NB][2][4], l[NT][2], off[NT][2];
+        float high[NT][2];  // the row's reference + kSlack: scores above move it
+        // Value scales up to vlim = 2^voff need no lower reference. A bf16 result's probabilities are f16 themselves
+        // and must stay in range; in two terms their products with the scales only.
+        float vlim = NP == 1 ? 1.0f : 0.0f, voff = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) l[nt][j] = 0.0f, high[nt][j] = -INFINITY, off[nt][j] = kBias;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[nt][b][k][i] = 0.0f;
+        }
+
+        for (; my_i < done_i + count; my_i += W, ++my_k) {
+            const int stage = my_k % R::STAGES;
+            const int group = g0 + my_i;
+            issue();
+            if (!broken && !mbar_wait(&bars[warp][stage], (my_k / R::STAGES) & 1)) {
+                record_device_error(a.c.err, DEV_ERR_WAIT_FULL);
+                broken = true;
+            }
+            if (__any_sync(0xffffffffu, broken)) {
+                if (!broken_k) broken_k = my_k + 1;
+                broken = true;
+            }
+            if (broken || (bad >> stage & 1)) {
+                __syncwarp();
+                continue;
+            }
+            uint8_t *buf = ring + stage * Q::GROUP_BYTES;
+            if constexpr (STEP) {
+                // the group of the new token: its row goes into this copy and into the cache
+                if (group == (at.S - 1) >> 4) {
+                    append_new<D>(p, at.b, at.h, at.S - 1, buf);
+                    __syncwarp();
+                }
+            }
+            const bool masked = (group + 1) * kKvGroup > all_see;
+
+            // ---- scores
+            uint32_t kw[2][NB];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint8_t *src = buf + Q::K_CODES + (lg + 8 * k) * (D / 2) + lt * NB * 4;
+                if constexpr (NB == 4)
+                    *reinterpret_cast<uint4 *>(kw[k]) = *reinterpret_cast<const uint4 *>(src);
+                else
+                    *reinterpret_cast<uint2 *>(kw[k]) = *reinterpret_cast<const uint2 *>(src);
+            }
+            uint32_t ks[2][NB / 2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint8_t *src = buf + Q::K_SCALES + (lg + 8 * k) * NB * 2;
+                if constexpr (NB == 4)
+                    *reinterpret_cast<uint2 *>(ks[k]) = *reinterpret_cast<const uint2 *>(src);
+                else
+                    ks[k][0] = *reinterpret_cast<const uint32_t *>(src);
+            }
+            float s[NT][4];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t e0[4], e1[4];
+                unpack_codes<!F32>(kw[0][b], e0);
+                unpack_codes<!F32>(kw[1][b], e1);
+                const float2 f0 = unpack_f16(ks[0][b / 2]), f1 = unpack_f16(ks[1][b / 2]);
+                const float d0 = b & 1 ? f0.y : f0.x, d1 = b & 1 ? f1.y : f1.x;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float c0[4] = {start[nt][b][0], start[nt][b][1], start[nt][b][0], start[nt][b][1]};
+                    float acc[4];
+                    mma16816(acc, e0[0], e1[0], e0[1], e1[1], qf[nt][b][0][0], qf[nt][b][0][1], c0);
+                    mma16816(acc, e0[2], e1[2], e0[3], e1[3], qf[nt][b][0][2], qf[nt][b][0][3], acc);
+                    if constexpr (NQ == 2) {
+                        mma16816(acc, e0[0], e1[0], e0[1], e1[1], qf[nt][b][1][0], qf[nt][b][1][1], acc);
+                        mma16816(acc, e0[2], e1[2], e0[3], e1[3], qf[nt][b][1][2], qf[nt][b][1][3], acc);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float d = i < 2 ? d0 : d1;
+                        s[nt][i] = b == 0 ? acc[i] * d : fmaf(acc[i], d, s[nt][i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[nt][i] *= to_log2[nt][i & 1];
+                    if (masked && group * kKvGroup + lg + 8 * (i >> 1) >= limit[nt][i & 1]) s[nt][i] = -INFINITY;
+                }
+
+            // ---- references that are too low for a score, or for a value scale
+            const uint32_t vs_word = lane < 8 * NB ? *reinterpret_cast<const uint32_t *>(buf + Q::V_SCALES + lane * 4) : 0u;
+            const float2 vsf = unpack_f16(vs_word & 0x7fff7fffu);
+            float vmax = fmaxf(vsf.x, vsf.y);
+            if (masked && group * kKvGroup + lane / (NB / 2) >= at.S) vmax = 0.0f;
+            bool low = vmax > vlim && vmax < INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) low |= s[nt][i] > high[nt][i & 1];
+            if (__any_sync(0xffffffffu, low)) {
+                if (!(vmax < INFINITY)) vmax = 65504.0f;
+#pragma unroll
+                for (int o2 = 16; o2; o2 >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o2));
+                if (vmax > vlim) {  // the power of two above it
+                    const uint32_t e = (__float_as_uint(vmax) >> 23) + 1;
+                    vlim = __uint_as_float(e << 23);
+                    voff = (float)((int)e - 127);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float m = fmaxf(s[nt][j], s[nt][j + 2]);
+#pragma unroll
+                        for (int o2 = 4; o2 < 32; o2 <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
+                        m = fmaxf(m, high[nt][j] - kSlack);
+                        if (m == -INFINITY) continue;
+                        const float noff = kBias - voff - m;
+                        const float alpha = high[nt][j] == -INFINITY ? 1.0f : exp2_approx(noff - off[nt][j]);
+                        high[nt][j] = m + kSlack;
+                        off[nt][j] = noff;
+                        l[nt][j] *= alpha;
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                o[nt][b][k][j] *= alpha;
+                                o[nt][b][k][j + 2] *= alpha;
+                            }
+                    }
+            }
+
+            // ---- probabilities, times the values' scales, as the second product's B fragments
+            uint32_t pf[NT][NB][NP][2];
+            if constexpr (BF) {
+                uint32_t vs[2][NB];  // (token 2t, token 2t + 1) of each block, and 2t + 8, 2t + 9
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint8_t *src = buf + Q::V_SCALES + (2 * lt + 8 * k) * NB * 2;
+                    if constexpr (NB == 4) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(src);
+                        vs[k][0] = __byte_perm(w.x, w.z, 0x5410);
+                        vs[k][1] = __byte_perm(w.x, w.z, 0x7632);
+                        vs[k][2] = __byte_perm(w.y, w.w, 0x5410);
+                        vs[k][3] = __byte_perm(w.y, w.w, 0x7632);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(src);
+                        vs[k][0] = __byte_perm(w.x, w.y, 0x5410);
+                        vs[k][1] = __byte_perm(w.x, w.y, 0x7632);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e[i] = exp2_approx(s[nt][i] + off[nt][i & 1]);
+                        l[nt][i & 1] += e[i];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t pt = transpose8x8(pack_f16(e[2 * k], e[2 * k + 1]));  // (2t, 2t + 1) of row g
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            uint32_t v = mul_f16x2(pt, vs[k][b]);
+                            if (masked) {  // what a row does not see may hold anything
+                                if (!(pt & 0x0000ffffu)) v &= 0xffff0000u;
+                                if (!(pt & 0xffff0000u)) v &= 0x0000ffffu;
+                            }
+                            pf[nt][b][0][k] = v;
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float dv[NB];
+                    const uint8_t *src = buf + Q::V_SCALES + (lg + 8 * k) * NB * 2;
+#pragma unroll
+                    for (int b = 0; b < NB; b += 2) {
+                        const float2 f = unpack_f16(*reinterpret_cast<const uint32_t *>(src + b * 2));
+                        dv[b] = f.x, dv[b + 1] = f.y;
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float e[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            e[j] = exp2_approx(s[nt][2 * k + j] + off[nt][j]);
+                            l[nt][j] += e[j];
+                        }
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const float x0 = masked && s[nt][2 * k] == -INFINITY ? 0.0f : e[0] * dv[b];
+                            const float x1 = masked && s[nt][2 * k + 1] == -INFINITY ? 0.0f : e[1] * dv[b];
+                            const uint32_t h = pack_f16(x0, x1);
+                            const float2 f = unpack_f16(h);
+                            pf[nt][b][0][k] = transpose8x8(h);
+                            pf[nt][b][NP - 1][k] = transpose8x8(pack_f16(x0 - f.x, x1 - f.y));
+                        }
+                    }
+                }
+            }
+
+            // ---- values
+            uint32_t vw[2][NB];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint8_t *src = buf + Q::V_CODES + k * 4 * D + lane * NB * 4;
+                if constexpr (NB == 4)
+                    *reinterpret_cast<uint4 *>(vw[k]) = *reinterpret_cast<const uint4 *>(src);
+                else
+                    *reinterpret_cast<uint2 *>(vw[k]) = *reinterpret_cast<const uint2 *>(src);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t e0[4], e1[4];
+                unpack_codes<false>(vw[0][b], e0);
+                unpack_codes<false>(vw[1][b], e1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) {
+                        mma16816(o[nt][b][0], e0[0], e0[1], e1[0], e1[1], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][0]);
+                        mma16816(o[nt][b][1], e0[2], e0[3], e1[2], e1[3], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][1]);
+                    }
+            }
+            __syncwarp();  // every lane has read the stage before a copy comes into it
+        }
+
+        // ---- the warps' results of the item, or of this CTA's part of it
+        const bool whole = at.g == 0 && count == at.G;
+        float *po = p.part_o + ((int64_t)cta * 2 + (at.g == 0)) * RT * D;
+        float *pml = p.part_ml + ((int64_t)cta * 2 + (at.g == 0)) * RT * 2;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (nt) __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float sum = l[nt][j];
+#pragma unroll
+                for (int o2 = 4; o2 < 32; o2 <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+                if (lg == 0) {
+                    // a row that met no key weighs nothing (NaN scores count: they set no reference, but their sum is NaN)
+                    ml_sm[warp][2 * lt + j][0] = high[nt][j] == -INFINITY && sum == 0.0f ? INFINITY : off[nt][j];
+                    ml_sm[warp][2 * lt + j][1] = sum;
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    *reinterpret_cast<float4 *>(merge + (warp * 8 + 2 * lt + j) * R::ROW + b * 32 + lg * 4) =
+                        make_float4(o[nt][b][0][j], o[nt][b][0][j + 2], o[nt][b][1][j], o[nt][b][1][j + 2]);
+            }
+            __syncthreads();
+            // thread: row tid / (D/4) .. of the 8, four dimensions
+            for (int idx = tid; idx < 8 * (D / 4); idx += kSplitThreads) {
+                const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+                float least = INFINITY;
+#pragma unroll
+                for (int w = 0; w < W; ++w) least = fminf(least, ml_sm[w][row][0]);
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+                if (least < INFINITY) {
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        if (ml_sm[w][row][0] == INFINITY) continue;
+                        const float f = exp2_approx(least - ml_sm[w][row][0]);
+                        const float4 x = *reinterpret_cast<const float4 *>(merge + (w * 8 + row) * R::ROW + d);
+                        v[0] = fmaf(f, x.x, v[0]);
+                        v[1] = fmaf(f, x.y, v[1]);
+                        v[2] = fmaf(f, x.z, v[2]);
+                        v[3] = fmaf(f, x.w, v[3]);
+                        sum = fmaf(f, ml_sm[w][row][1], sum);
+                    }
+                }
+                const int rr = nt * 8 + row;
+                if (!whole) {
+                    __stcg(reinterpret_cast<float4 *>(po + rr * D + d), make_float4(v[0], v[1], v[2], v[3]));
+                    if (d == 0) __stcg(reinterpret_cast<float2 *>(pml + rr * 2), make_float2(least, sum));
+                } else if (rr < rows) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] *= inv;
+                    const int r = at.first + (row0 + rr) / a.rep, hq = at.h * a.rep + (row0 + rr) % a.rep;
+                    finish4<T, D, STEP>(p, r, hq, d, v);
+                    if (d == 0 && a.lse)
+                        a.lse[(int64_t)r * a.heads + hq] = sum == 0.0f ? 0.0f : (log2f(sum) - least) * 0.6931471805599453f;
+                }
+            }
+        }
+        __syncthreads();
+        if (!whole) {
+            // The item lies in CTAs c0 .. c1. Each sets its flag behind its part and then looks at the others': the
+            // fences put one CTA's look behind everyone's flag, and that one (now and then two, with the same result)
+            // joins the parts in order. A flag is this launch's number, so that what lay in the workspace does not
+            // matter, and goes back to 0, so that a replay of the launch finds none set.
+            const int c0 = (int)(((item0 + 1) * grid - 1) / total), c1 = (int)(((item0 + at.G) * grid - 1) / total);
+            auto slot = [&](int c) { return (int64_t)c * 2 + (c == c0); };
+            if (warp == 0) {
+                if (lane == 0) {
+                    __threadfence();
+                    *reinterpret_cast<volatile unsigned long long *>(p.flags + slot(cta)) = p.nonce;
+                }
+                __syncwarp();
+                __threadfence();
+                bool all = true;
+                for (int c = c0 + lane; c <= c1; c += 32)
+                    all &= *reinterpret_cast<const volatile unsigned long long *>(p.flags + slot(c)) == p.nonce;
+                all = __all_sync(0xffffffffu, all);
+                __threadfence();
+                if (lane == 0) is_last = all;
+            }
+            __syncthreads();
+            if (is_last) {
+                for (int idx = tid; idx < RT * (D / 4); idx += kSplitThreads) {
+                    const int rr = idx / (D / 4), d = idx % (D / 4) * 4;
+                    float least = INFINITY;
+                    for (int c = c0; c <= c1; ++c) least = fminf(least, __ldcg(p.part_ml + (slot(c) * RT + rr) * 2));
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+                    if (least < INFINITY) {
+#pragma unroll 4
+                        for (int c = c0; c <= c1; ++c) {
+                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + (slot(c) * RT + rr) * 2));
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (slot(c) * RT + rr) * D + d));
+                            const float f = ml.x == INFINITY ? 0.0f : exp2_approx(least - ml.x);
+                            if (ml.x == INFINITY) continue;
+                            v[0] = fmaf(f, x.x, v[0]);
+                            v[1] = fmaf(f, x.y, v[1]);
+                            v[2] = fmaf(f, x.z, v[2]);
+                            v[3] = fmaf(f, x.w, v[3]);
+                            sum = fmaf(f, ml.y, sum);
+                        }
+                    }
+                    if (rr < rows) {
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] *= inv;
+                        const int r = at.first + (row0 + rr) / a.rep, hq = at.h * a.rep + (row0 + rr) % a.rep;
+                        finish4<T, D, STEP>(p, r, hq, d, v);
+                        if (d == 0 && a.lse)
+                            a.lse[(int64_t)r * a.heads + hq] =
+                                sum == 0.0f ? 0.0f : (log2f(sum) - least) * 0.6931471805599453f;
+                    }
+                }
+                __syncthreads();
+                for (int c = c0 + tid; c <= c1; c += kSplitThreads) p.flags[slot(c)] = 0;
+            }
+        }
+        done_i += count;
+        if (done_i < units) {
+            item0 += at.G;
+            at.g = 0;
+            at.next_item(a);
+        }
+    }
+    if (broken) {  // copies still on their way (each wait bounded) before the shared memory goes
+        for (int k = broken_k - 1; k < issued; ++k) mbar_wait(&bars[warp][k % R::STAGES], (k / R::STAGES) & 1);
+    }
+}
+
+constexpr int kMaxGrid = 296;  // CTAs whose parts a workspace holds
+
+// The rows of a tile: 8 hold every head that shares a KV head in decode (up to 8); more rows a request make
+// tiles of 16, which read the cache half as often.
+int tile_rows(int64_t max_query, int64_t rep) { return max_query * rep <= 8 ? 8 : 16; }
+
+int64_t workspace_bytes(int rows, int64_t dim) { return (int64_t)kMaxGrid * 2 * (rows * (dim + 2) * 4 + 8); }
+
+unsigned long long next_nonce() {
+    static std::atomic<unsigned long long> count{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+    unsigned long long z = count.fetch_add(0x9e3779b97f4a7c15ull) + 0x9e3779b97f4a7c15ull;
+    z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+    z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+    z ^= z >> 31;
+    return z ? z : 1;
+}
+
+template <typename T, int D, int NT, bool STEP>
+int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op) {
+    DeviceFacts f{};
+    int st = device_facts(&f);
+    if (st) return st;
+    constexpr int rows = 8 * NT;
+    const int grid = std::min(f.sm_count * (NT == 1 ? 2 : 1), kMaxGrid);
+    p.part_o = static_cast<float *>(workspace);
+    p.part_ml = p.part_o + (int64_t)kMaxGrid * 2 * rows * D;
+    p.flags = reinterpret_cast<unsigned long long *>(p.part_ml + (int64_t)kMaxGrid * 2 * rows * 2);
+    p.nonce = next_nonce();
+    auto kernel = sdpa_q4_split_kernel<T, D, NT, STEP>;
+    st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D>::SMEM), op,
+                    "cudaFuncSetAttribute");
+    if (st) return st;
+    return launch_pdl(kernel, dim3((unsigned)grid), dim3(kSplitThreads), Ring<D>::SMEM, stream, op, p);
+}
+
+template <typename T, int D>
+int launch_attend(Split &p, int64_t max_query, void *workspace, cudaStream_t stream) {
+    return tile_rows(max_query, p.a.rep) == 8 ? launch_split<T, D, 1, false>(p, workspace, stream, "tn_sdpa_q4_cache")
+                                              : launch_split<T, D, 2, false>(p, workspace, stream, "tn_sdpa_q4_cache");
 }
 
 int check_cache(const char *op, const KvPool &c, int64_t requests, int64_t max_pages, int64_t table_stride,
@@ -197,8 +918,8 @@ int check_cache(const char *op, const KvPool &c, int64_t requests, int64_t max_p
 
 extern "C" int64_t tn_sdpa_q4_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                               int64_t max_query) {
-    (void)kv_heads, (void)max_query;
-    return tokens * heads * head_dim * 2 + 256;
+    if (kv_heads < 1 || heads < 1) return 0;
+    return tn::workspace_bytes(tn::tile_rows(std::max<int64_t>(1, std::min(max_query, tokens)), heads / kv_heads), head_dim);
 }
 
 extern "C" int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strides, int64_t tokens, int64_t heads,
@@ -224,21 +945,25 @@ extern "C" int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strid
     const int64_t size = (int64_t)tn_dtype_size(dtype);
     if ((uintptr_t)q % 16 || q_strides[0] * size % 16 || q_strides[1] * size % 16 || (uintptr_t)out % 16)
         return tn::set_error(TN_ERR_INVALID, std::string(op) + ": query rows must be 16-byte aligned with a unit inner stride");
-    (void)max_query;
+    max_query = std::max<int64_t>(1, std::min(query_start ? max_query : 1, tokens));
     if (!workspace || workspace_bytes < tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, head_dim, max_query))
         return tn::set_error(TN_ERR_SHAPE, std::string(op) + ": the workspace is smaller than tn_sdpa_q4_workspace_bytes");
     const float sc = scale > 0.0 ? (float)scale : 1.0f / sqrtf((float)head_dim);
-    tn::Attend p{q, q_strides[0], q_strides[1], c, query_start, out, lse, (int)tokens, (int)heads, (int)(heads / kv_heads), sc};
+    if ((uintptr_t)workspace % 16)
+        return tn::set_error(TN_ERR_INVALID, std::string(op) + ": the workspace must be 16-byte aligned");
+    tn::Split p{};
+    p.a = {q, q_strides[0], q_strides[1], c, query_start, out, lse, (int)tokens, (int)heads, (int)(heads / kv_heads), sc};
+    p.min_units = 8;
     __atomic_fetch_add(&tn::counters().sdpa_calls, 1ull, __ATOMIC_RELAXED);
     __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     cudaStream_t s = tn::stream_of(stream);
     if (head_dim == 128)
-        return dtype == TN_F32   ? tn::launch_attend<float, 128>(p, s)
-               : dtype == TN_F16 ? tn::launch_attend<__half, 128>(p, s)
-                                 : tn::launch_attend<__nv_bfloat16, 128>(p, s);
-    return dtype == TN_F32   ? tn::launch_attend<float, 64>(p, s)
-           : dtype == TN_F16 ? tn::launch_attend<__half, 64>(p, s)
-                             : tn::launch_attend<__nv_bfloat16, 64>(p, s);
+        return dtype == TN_F32   ? tn::launch_attend<float, 128>(p, max_query, workspace, s)
+               : dtype == TN_F16 ? tn::launch_attend<__half, 128>(p, max_query, workspace, s)
+                                 : tn::launch_attend<__nv_bfloat16, 128>(p, max_query, workspace, s);
+    return dtype == TN_F32   ? tn::launch_attend<float, 64>(p, max_query, workspace, s)
+           : dtype == TN_F16 ? tn::launch_attend<__half, 64>(p, max_query, workspace, s)
+                             : tn::launch_attend<__nv_bfloat16, 64>(p, max_query, workspace, s);
 }
 
 extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t rope_rows, void *pool, int64_t num_pages,
@@ -267,17 +992,19 @@ extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t
     cudaStream_t s = tn::stream_of(stream);
     if (!workspace || workspace_bytes < tn_sdpa_q4_workspace_bytes(requests, heads, kv_heads, head_dim, 1))
         return tn::set_error(TN_ERR_SHAPE, std::string(op) + ": the workspace is smaller than tn_sdpa_q4_workspace_bytes");
-    void *q = workspace;
+    if ((uintptr_t)workspace % 16)
+        return tn::set_error(TN_ERR_INVALID, std::string(op) + ": the workspace must be 16-byte aligned");
     __atomic_fetch_add(&tn::counters().sdpa_calls, 1ull, __ATOMIC_RELAXED);
     __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
-    tn::Attend p{q, heads * head_dim, head_dim, c, nullptr, out, lse, (int)requests, (int)heads, (int)(heads / kv_heads), sc};
-    const dim3 grid((unsigned)(heads + 2 * kv_heads), (unsigned)requests);
-    auto kernel = head_dim == 128 ? tn::rope_append_q4_kernel<128> : tn::rope_append_q4_kernel<64>;
-    st = tn::launch_pdl(kernel, grid, dim3(64), 0, s, op, (const __nv_bfloat16 *)qkv, (const __nv_bfloat16 *)rope, rope_rows,
-                        c, (int)heads, (__nv_bfloat16 *)q);
-    if (st) return st;
-    st = head_dim == 128 ? tn::launch_attend<__nv_bfloat16, 128>(p, s) : tn::launch_attend<__nv_bfloat16, 64>(p, s);
-    if (st || !codes) return st;
-    return tn_q8_0_quantize_planar(out, TN_BF16, heads * head_dim, codes, heads * head_dim, scales, offsets, requests,
-                                   heads * head_dim, stream);
+    tn::Split p{};
+    p.a = {nullptr, 0, 0, c, nullptr, out, lse, (int)requests, (int)heads, (int)(heads / kv_heads), sc};
+    p.min_units = 8;
+    p.qkv = (const __nv_bfloat16 *)qkv;
+    p.rope = (const __nv_bfloat16 *)rope;
+    p.rope_rows = rope_rows;
+    p.codes = codes;
+    p.scales = scales;
+    p.offsets = offsets;
+    return head_dim == 128 ? tn::launch_split<__nv_bfloat16, 128, 1, true>(p, workspace, s, op)
+                           : tn::launch_split<__nv_bfloat16, 64, 1, true>(p, workspace, s, op);
 }
