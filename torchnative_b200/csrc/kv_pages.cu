@@ -24,7 +24,8 @@ int check_kv_pool(const char *op, const void *pool, int64_t num_pages, int64_t k
     if (head_dim != 64 && head_dim != 128)
         return set_error(TN_ERR_NOT_IMPLEMENTED, name + ": the 4-bit KV cache takes head dimensions 64 and 128, got " +
                                                      std::to_string(head_dim));
-    if (num_pages < 0 || num_pages > INT32_MAX || kv_heads < 1 || kv_heads > 65535)
+    if (num_pages < 0 || kv_heads < 1 || kv_heads > 65535 ||
+        num_pages > INT32_MAX / (kv_heads * (page_size / kKvGroup)))
         return set_error(TN_ERR_SHAPE, name + ": bad page or head count");
     if ((!pool && num_pages > 0) || reinterpret_cast<uintptr_t>(pool) % 16 != 0)
         return set_error(TN_ERR_INVALID, name + ": the pool must be a 16-byte aligned device pointer");

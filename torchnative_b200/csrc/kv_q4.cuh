@@ -67,16 +67,19 @@ struct KvPool {
     }
     // The group of tokens [16 group, 16 group + 16) of request b, or NULL (and
     // the device error word set) where the table names no page of the pool.
+    // (A pool holds fewer than 2^31 groups: 4.9 TB.)
     template <int D>
     __device__ __forceinline__ uint8_t *group(int b, int kvh, int group) const {
-        const int page = table[b * table_stride + (group >> (page_shift - 4))];
+        return group_of_row<D>(table + b * table_stride, kvh, group);
+    }
+    template <int D>
+    __device__ __forceinline__ uint8_t *group_of_row(const int *row, int kvh, int group) const {
+        const int shift = page_shift - 4, page = row[group >> shift];
         if ((unsigned)page >= (unsigned)num_pages) {
             record_device_error(err, DEV_ERR_BAD_PAGE);
             return nullptr;
         }
-        const int64_t at = (((int64_t)page * kv_heads + kvh) << (page_shift - 4)) +
-                           (group & ((1 << (page_shift - 4)) - 1));
-        return pool + at * KvQ4<D>::GROUP_BYTES;
+        return pool + (int64_t)(((page * kv_heads + kvh) << shift) + (group & ((1 << shift) - 1))) * KvQ4<D>::GROUP_BYTES;
     }
 };
 

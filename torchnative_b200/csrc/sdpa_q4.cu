@@ -61,6 +61,8 @@ struct Ring {
 
 constexpr int kSplitThreads = 256;
 constexpr float kBias = 10.0f, kSlack = 5.0f;
+// What an item costs besides its groups (queries, the warps' results joined), in units.
+constexpr int kItemCost = 12;
 
 struct Split {
     Attend a;
@@ -132,10 +134,12 @@ __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&e)[4]) {
     }
 }
 
-// A place in the line of units: group g of G of item (b, tile u, head h).
+// A place in the line of units: group g of item (b, tile u, head h), whose
+// groups this CTA has from `from` to `upto`. `rel` is the place of the item's
+// group 0 against the first of the CTA's `len` places.
 template <int RT>
 struct Cursor {
-    int b, u, h, g, G;
+    int b, u, h, G, rel;
     int S, n, first, tiles;
 
     __device__ __forceinline__ void load_request(const Attend &p) {
@@ -153,32 +157,30 @@ struct Cursor {
         const int last = min(n - 1, (tile * RT + RT - 1) / p.rep);
         return max(1, (S - n + last + 16) >> 4);
     }
-    __device__ __forceinline__ long long request_units(const Attend &p) const {
-        long long units = 0;
-        for (int t = 0; t < tiles; ++t) units += tile_groups(p, t);
-        return units * p.c.kv_heads;
+    __device__ __forceinline__ long long request_places(const Attend &p) const {
+        long long places = 0;
+        for (int t = 0; t < tiles; ++t) places += tile_groups(p, t) + kItemCost;
+        return places * p.c.kv_heads;
     }
+    __device__ __forceinline__ int from() const { return max(0, -rel); }
+    __device__ __forceinline__ int upto(int len) const { return min(G, len - rel); }
+    // The next item; past the last one rel is beyond every len.
     __device__ __forceinline__ void next_item(const Attend &p) {
+        rel += G + kItemCost;
         if (++h < p.c.kv_heads) return;
         h = 0;
         if (++u >= tiles) {
             u = 0;
             do {
                 if (++b >= p.c.requests) {
-                    G = INT32_MAX;  // behind the last unit
+                    rel = INT32_MAX / 2;
+                    G = 1;
                     return;
                 }
                 load_request(p);
             } while (tiles == 0);
         }
         G = tile_groups(p, u);
-    }
-    __device__ __forceinline__ void advance(const Attend &p, int by) {
-        g += by;
-        while (g >= G && b < p.c.requests) {
-            g -= G;
-            next_item(p);
-        }
     }
 };
 
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- this CTA's units
+    // ---- this CTA's places in the line
     const Attend &a = p.a;
     Cursor<RT> at;
     long long total = 0;
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
         at.b = b0 + lane;
         if (at.b < a.c.requests) {
             at.load_request(a);
-            w = at.request_units(a);
+            w = at.request_places(a);
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) w += __shfl_xor_sync(0xffffffffu, w, off);
@@ -345,16 +347,16 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
     const int grid = (int)min((long long)gridDim.x, max(1ll, total / p.min_units));
     const int cta = blockIdx.x;
     if (cta >= grid) return;
-    const long long lo = cta * total / grid, hi = (cta + 1) * total / grid;
-    long long item0 = 0;  // line position of the current item's first unit
+    const long long lo = cta * total / grid;
+    const int len = (int)((cta + 1) * total / grid - lo);
+    long long place = 0;  // of the current request, then tile
     {
-        long long before = 0;
         for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
             long long w = 0;
             at.b = b0 + lane;
             if (at.b < a.c.requests) {
                 at.load_request(a);
-                w = at.request_units(a);
+                w = at.request_places(a);
             }
             long long upto = w;
 #pragma unroll
@@ -362,61 +364,66 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                 const long long v = __shfl_up_sync(0xffffffffu, upto, off);
                 if (lane >= off) upto += v;
             }
-            const unsigned past = __ballot_sync(0xffffffffu, before + upto > lo);
+            const unsigned past = __ballot_sync(0xffffffffu, place + upto > lo);
             if (past) {
                 const int l0 = __ffs(past) - 1;
-                item0 = before + __shfl_sync(0xffffffffu, upto - w, l0);
+                place += __shfl_sync(0xffffffffu, upto - w, l0);
                 at.b = b0 + l0;
                 break;
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            place += __shfl_sync(0xffffffffu, upto, 31);
         }
         at.load_request(a);
-        at.u = at.h = 0;
-        for (;; ++at.u) {  // the tile, then the head
+        for (at.u = 0;; ++at.u) {
             at.G = at.tile_groups(a, at.u);
-            const long long units = (long long)at.G * a.c.kv_heads;
-            if (item0 + units > lo) break;
-            item0 += units;
+            const long long places = (long long)(at.G + kItemCost) * a.c.kv_heads;
+            if (place + places > lo) break;
+            place += places;
         }
-        at.h = (int)((lo - item0) / at.G);
-        item0 += (long long)at.h * at.G;
-        at.g = (int)(lo - item0);
+        at.h = (int)((lo - place) / (at.G + kItemCost));
+        at.rel = (int)(place + (long long)at.h * (at.G + kItemCost) + kItemCost - lo);
     }
 
-    // ---- the ring: unit i of this CTA (i = warp, warp + W, ...) goes to stage (i / W) % STAGES
-    const int units = (int)(hi - lo);
+    // ---- the ring: this warp's k-th group goes to stage k % STAGES; the CTA's groups go round its warps
     Cursor<RT> ahead = at;
-    ahead.advance(a, warp);
-    int ahead_i = warp, ahead_k = 0, issued = 0;  // the next unit to bring, its place in the ring; units brought
+    const int *ahead_row = a.c.table + ahead.b * a.c.table_stride;
+    int ahead_g = ahead.from() + warp, ahead_k = 0;
+    uint32_t bad = 0;  // stages whose group has no page
     bool broken = false;
-    uint32_t bad = 0;  // stages whose unit has no page
     auto issue = [&]() {
-        if (ahead_i < units && !broken) {
-            ++issued;
-            const int s = ahead_k % R::STAGES;
-            const uint8_t *src = nullptr;
-            if (ahead.g * kKvGroup < ahead.S) src = a.c.group<D>(ahead.b, ahead.h, ahead.g);
-            bad = src ? bad & ~(1u << s) : bad | (1u << s);
-            if (src && lane == 0) {
+        if (ahead_g >= ahead.upto(len)) {
+            do {
+                if (ahead.rel >= len) return;
+                ahead_g -= max(ahead.from(), ahead.upto(len));
+                ahead.next_item(a);
+                ahead_g += ahead.from();
+            } while (ahead_g >= ahead.upto(len));
+            ahead_row = a.c.table + ahead.b * a.c.table_stride;
+        }
+        if (broken) return;
+        const int s = ahead_k % R::STAGES;
+        const uint8_t *src = nullptr;
+        if (ahead_g * kKvGroup < ahead.S) src = a.c.group_of_row<D>(ahead_row, ahead.h, ahead_g);
+        bad = src ? bad & ~(1u << s) : bad | (1u << s);
+        if (lane == 0) {
+            if (src) {
                 mbar_arrive_expect_tx(&bars[warp][s], Q::GROUP_BYTES);
                 bulk_g2s(ring + s * Q::GROUP_BYTES, src, Q::GROUP_BYTES, &bars[warp][s]);
-            } else if (!src && lane == 0) {
+            } else {
                 mbar_arrive(&bars[warp][s]);
             }
         }
-        ahead.advance(a, W);
-        ahead_i += W;
+        ahead_g += W;
         ++ahead_k;
     };
     for (int s = 0; s < R::STAGES - 1; ++s) issue();
 
-    int done_i = 0, my_i = warp, my_k = 0;  // units of finished items; this warp's next unit
+    int turn = warp, my_k = 0;  // groups of the CTA until this warp's next one
     int broken_k = 0;
-    while (done_i < units) {
-        // ---- one item, or this CTA's part of it: groups [at.g, at.g + count)
-        const int count = min(at.G - at.g, units - done_i);
-        const int g0 = at.g - done_i;  // unit i is group g0 + i
+    for (; at.rel < len; at.next_item(a)) {
+        // ---- one item, or this CTA's part of it
+        const int g0 = at.from(), g1 = at.upto(len);
+        if (g0 >= g1) continue;
         const int rows = min(RT, at.n * a.rep - at.u * RT);
         const int row0 = at.u * RT;
 
@@ -512,31 +519,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                     for (int i = 0; i < 4; ++i) o[nt][b][k][i] = 0.0f;
         }
 
-        for (; my_i < done_i + count; my_i += W, ++my_k) {
-            const int stage = my_k % R::STAGES;
-            const int group = g0 + my_i;
-            issue();
-            if (!broken && !mbar_wait(&bars[warp][stage], (my_k / R::STAGES) & 1)) {
-                record_device_error(a.c.err, DEV_ERR_WAIT_FULL);
-                broken = true;
-            }
-            if (__any_sync(0xffffffffu, broken)) {
-                if (!broken_k) broken_k = my_k + 1;
-                broken = true;
-            }
-            if (broken || (bad >> stage & 1)) {
-                __syncwarp();
-                continue;
-            }
-            uint8_t *buf = ring + stage * Q::GROUP_BYTES;
-            if constexpr (STEP) {
-                // the group of the new token: its row goes into this copy and into the cache
-                if (group == (at.S - 1) >> 4) {
-                    append_new<D>(p, at.b, at.h, at.S - 1, buf);
-                    __syncwarp();
-                }
-            }
-            const bool masked = (group + 1) * kKvGroup > all_see;
+        // One group; `mask` where a row may not see all of its tokens.
+        auto take = [&](const uint8_t *buf, int group, auto mask) {
+            constexpr bool masked = decltype(mask)::value;
 
             // ---- scores
             uint32_t kw[2][NB];
@@ -728,13 +713,45 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                         mma16816(o[nt][b][1], e0[2], e0[3], e1[2], e1[3], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][1]);
                     }
             }
+        };
+
+        int group = g0 + turn;
+        for (; group < g1; group += W, ++my_k) {
+            const int stage = my_k % R::STAGES;
+            issue();
+            if (!broken && !mbar_wait(&bars[warp][stage], (my_k / R::STAGES) & 1)) {
+                record_device_error(a.c.err, DEV_ERR_WAIT_FULL);
+                broken = true;
+            }
+            if (__any_sync(0xffffffffu, broken)) {
+                if (!broken_k) broken_k = my_k + 1;
+                broken = true;
+            }
+            if (broken || (bad >> stage & 1)) {
+                __syncwarp();
+                continue;
+            }
+            uint8_t *buf = ring + stage * Q::GROUP_BYTES;
+            if constexpr (STEP) {
+                // the group of the new token: its row goes into this copy and into the cache
+                if (group == (at.S - 1) >> 4) {
+                    append_new<D>(p, at.b, at.h, at.S - 1, buf);
+                    __syncwarp();
+                }
+            }
+            if ((group + 1) * kKvGroup > all_see)
+                take(buf, group, std::true_type{});
+            else
+                take(buf, group, std::false_type{});
             __syncwarp();  // every lane has read the stage before a copy comes into it
         }
 
+        turn = group - g1;
+
         // ---- the warps' results of the item, or of this CTA's part of it
-        const bool whole = at.g == 0 && count == at.G;
-        float *po = p.part_o + ((int64_t)cta * 2 + (at.g == 0)) * RT * D;
-        float *pml = p.part_ml + ((int64_t)cta * 2 + (at.g == 0)) * RT * 2;
+        const bool whole = g0 == 0 && g1 == at.G;
+        float *po = p.part_o + ((int64_t)cta * 2 + (g0 == 0)) * RT * D;
+        float *pml = p.part_ml + ((int64_t)cta * 2 + (g0 == 0)) * RT * 2;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if (nt) __syncthreads();
@@ -795,7 +812,8 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
             // fences put one CTA's look behind everyone's flag, and that one (now and then two, with the same result)
             // joins the parts in order. A flag is this launch's number, so that what lay in the workspace does not
             // matter, and goes back to 0, so that a replay of the launch finds none set.
-            const int c0 = (int)(((item0 + 1) * grid - 1) / total), c1 = (int)(((item0 + at.G) * grid - 1) / total);
+            const long long first = lo + at.rel;
+            const int c0 = (int)(((first + 1) * grid - 1) / total), c1 = (int)(((first + at.G) * grid - 1) / total);
             auto slot = [&](int c) { return (int64_t)c * 2 + (c == c0); };
             if (warp == 0) {
                 if (lane == 0) {
@@ -847,15 +865,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                 for (int c = c0 + tid; c <= c1; c += kSplitThreads) p.flags[slot(c)] = 0;
             }
         }
-        done_i += count;
-        if (done_i < units) {
-            item0 += at.G;
-            at.g = 0;
-            at.next_item(a);
-        }
     }
     if (broken) {  // copies still on their way (each wait bounded) before the shared memory goes
-        for (int k = broken_k - 1; k < issued; ++k) mbar_wait(&bars[warp][k % R::STAGES], (k / R::STAGES) & 1);
+        for (int k = broken_k - 1; k < ahead_k; ++k) mbar_wait(&bars[warp][k % R::STAGES], (k / R::STAGES) & 1);
     }
 }
 
