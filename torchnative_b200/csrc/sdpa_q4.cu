@@ -25,52 +25,88 @@ struct Attend {
     float scale;
 };
 
-// ---- the split kernel: few query rows against a long cache
+// ---- the kernel
 //
-// One unit of work is one group of 16 tokens of one (request, row tile, KV
-// head); a row tile is 8 NT of the request's query rows (tokens times the heads
-// that share the KV head). All units of a call stand in one line, and CTA c of G
-// takes units [c W / G, (c + 1) W / G): every CTA gets the same number whatever
-// the lengths, which only the device knows. Inside a CTA the units go round the
-// warps; a warp brings its groups (18 D bytes, one bulk copy each) into a ring of
-// its own and needs no other warp until an item (request, tile, head) ends.
+// One unit of work is 32 tokens of one (request, row tile, KV head); a row tile
+// is 8 NT of the request's query rows (tokens times the heads that share the KV
+// head), and an item is all units of one of them. The items of a call stand in
+// one line, each as long as its units plus what an item costs besides, and CTA c
+// of G takes the c-th part of the line: every CTA gets as much whatever the
+// lengths, which only the device knows.
 //
-// Per group a warp computes, with m16n8k16 tensor instructions,
-//   S^T[16 keys, 8 rows] = sum over blocks b of d_k[key, b] * (codes_b . q_b)
-//   O^T[D, 8 rows] += sum over blocks: codes_b^T . (p[key, row] * d_v[key, b])
+// A CTA is W consumer warps and a producer warp, one CTA an SM. Unit i of a CTA
+// goes to warp i mod W. Lane w of the producer walks the line for warp w and
+// brings its units (36 D bytes, one bulk copy where a page holds 32 tokens) to
+// stage i / W of a ring; a stage is filled again when every warp is through with
+// it, so that the warps stay together: without that bound the SM's scheduler let
+// some run ahead, and the last ones ended alone (127 us of 82 at 2 x 100,000
+// tokens of 8 heads). The producer also prepares each item's queries.
+//
+// Per 16 tokens a warp computes, with m16n8k16 tensor instructions,
+//   S^T[16 tokens, 8 rows] = sum over blocks b of d_k[token, b] * (codes_b . q_b)
+//   O^T[D, 8 rows] += sum over blocks: codes_b^T . (p[token, row] * d_v[token, b])
 // so that the 4-bit codes enter the products as the small integers they are
 // (exact in f16), the tall side of both products is the cache's, and a tile of 8
-// rows wastes nothing. A code costs about 1.1 instructions to unpack: masks put
+// rows wastes nothing. A code costs about one instruction to unpack: masks put
 // the nibble below a float16 exponent (1024 + c, or 64 + c for a nibble at bit
 // 4), and 1032 or 72 goes off again, for a part of K in the accumulators' start.
 // The scores' fragment is turned into the second product's operand by a register
 // transpose (movmatrix).
 //
 // p is 2^(s - ref) times 2^10, f16, where ref follows the row's maximum by more
-// than 2^5 only (a vote per group; out = O / l holds for any ref), and goes down
+// than 2^5 only (a vote per unit; out = O / l holds for any ref), and goes down
 // when the value scales are above 1, so that p * d_v stays in f16's range.
+constexpr int kMaxGrid = 148;  // CTAs whose parts a workspace holds
+constexpr int kUnitGroups = 2, kUnit = kUnitGroups * kKvGroup;
+constexpr float kBias = 10.0f, kSlack = 5.0f;
+// What an item costs besides its units (queries, the warps' results joined), in units.
+constexpr int kItemCost = 12;
 
-template <int D>
-struct Ring {
-    static constexpr int WARPS = 8, STAGES = 4;
-    static constexpr int BYTES = WARPS * STAGES * KvQ4<D>::GROUP_BYTES;
-    static constexpr int ROW = D + 4;  // floats of a row of the merge buffer: rows 2t of a fragment differ in their banks
-    static constexpr int MERGE = WARPS * 8 * ROW * 4;
-    static constexpr int SMEM = BYTES + MERGE;
+// What the producer tells the consumers of an item.
+struct Item {
+    int end;             // no item: the work is done
+    int g0, g1;          // this CTA's units of it
+    int i0;              // the CTA's units before
+    int whole, c0, c1;   // all of its units; otherwise the CTAs that have some
+    int b, h, S;
+    int rows, row0;      // query rows of the tile, of the request before it
+    int first, all_see;  // the request's first packed token; keys that every row of the tile sees
 };
 
-constexpr int kSplitThreads = 256;
-constexpr float kBias = 10.0f, kSlack = 5.0f;
-// What an item costs besides its groups (queries, the warps' results joined), in units.
-constexpr int kItemCost = 12;
+template <typename T, int D, int NT>
+struct Shape {
+    static constexpr bool F32 = sizeof(T) == 4, BF = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int NQ = F32 ? 2 : 1;  // f16 terms of a query element
+    static constexpr int NP = BF ? 1 : 2;   // f16 terms of a probability
+    static constexpr int NB = D / 32;
+    // registers go to warps by fours: 12 warps of 168 a thread, 8 of 255 with two row tiles' accumulators
+    static constexpr int W = NT == 2 ? 7 : 11;
+    static constexpr int STAGES = D == 64 ? 4 : 3;
+    static constexpr int UNIT = kUnitGroups * KvQ4<D>::GROUP_BYTES;
+    static constexpr int RING = W * STAGES * UNIT;
+    static constexpr int ROW = D + 4;  // floats of a row of the merge buffer: rows 2t of a fragment differ in their banks
+    static constexpr int MERGE = W * 8 * ROW * 4;
+    // an item's queries, a lane's data as it takes them
+    struct Slot {
+        uint4 q[NT][NB][NQ][32];
+        float2 start[NT][NB][32];  // what a score's accumulator starts from, for the columns 2t, 2t + 1
+        float2 to_log2[NT][32];
+        int2 limit[NT][32];  // keys that the columns' rows see
+        Item item;
+    };
+    static constexpr int SMEM = RING + MERGE + 2 * (int)sizeof(Slot);
+    static_assert(kMaxGrid * 8 * 4 <= MERGE, "the weights of an item's parts fit");
+    static_assert(SMEM <= 226 * 1024, "shared memory of one SM");
+};
 
 struct Split {
     Attend a;
-    int min_units;        // units a CTA should have before another one is used
-    float *part_o;        // [grid][2][8 NT][D]
-    float *part_ml;       // [grid][2][8 NT][2]
-    unsigned long long *flags;  // [grid][2]
+    int min_places;       // of the line that a CTA should have before another one is used
+    float *part_o;        // [kMaxGrid][2][8 NT][D]
+    float *part_ml;       // [kMaxGrid][2][8 NT][2]
+    unsigned long long *flags;  // [kMaxGrid][2]
     unsigned long long nonce;
+    uint32_t f16_1024, f16_64;  // 1024 and 64 as half2: here so that the compiler keeps them in registers
     // decode step
     const __nv_bfloat16 *qkv, *rope;
     int64_t rope_rows;
@@ -118,16 +154,23 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
+// (a & mask) | bits as one instruction: `bits` in a register of its own, since an instruction takes one constant only.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+    return r;
+}
+
 // The nibbles n and n + 4 of a word as half2, n = 0 .. 3: codes minus 8, except
 // that with RAW the odd ones come as 64 + code.
 template <bool RAW>
-__device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&e)[4]) {
+__device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&e)[4], uint32_t low, uint32_t high) {
     constexpr uint32_t kLow = 0x64086408u, kHigh = 0x54805480u;  // 1032, 72
     const uint32_t u = w >> 8;
-    e[0] = sub_f16x2((w & 0x000f000fu) | 0x64006400u, kLow);
-    e[1] = (w & 0x00f000f0u) | 0x54005400u;
-    e[2] = sub_f16x2((u & 0x000f000fu) | 0x64006400u, kLow);
-    e[3] = (u & 0x00f000f0u) | 0x54005400u;
+    e[0] = sub_f16x2(and_or(w, 0x000f000fu, low), kLow);
+    e[1] = and_or(w, 0x00f000f0u, high);
+    e[2] = sub_f16x2(and_or(u, 0x000f000fu, low), kLow);
+    e[3] = and_or(u, 0x00f000f0u, high);
     if constexpr (!RAW) {
         e[1] = sub_f16x2(e[1], kHigh);
         e[3] = sub_f16x2(e[3], kHigh);
@@ -152,14 +195,14 @@ struct Cursor {
         }
         tiles = (n * p.rep + RT - 1) / RT;
     }
-    // groups that the tile's last row sees; 1 where it sees none, so that someone writes its zeros
-    __device__ __forceinline__ int tile_groups(const Attend &p, int tile) const {
+    // units that the tile's last row sees; 1 where it sees none, so that someone writes its zeros
+    __device__ __forceinline__ int tile_units(const Attend &p, int tile) const {
         const int last = min(n - 1, (tile * RT + RT - 1) / p.rep);
-        return max(1, (S - n + last + 16) >> 4);
+        return max(1, (S - n + last + kUnit) / kUnit);
     }
     __device__ __forceinline__ long long request_places(const Attend &p) const {
         long long places = 0;
-        for (int t = 0; t < tiles; ++t) places += tile_groups(p, t) + kItemCost;
+        for (int t = 0; t < tiles; ++t) places += tile_units(p, t) + kItemCost;
         return places * p.c.kv_heads;
     }
     __device__ __forceinline__ int from() const { return max(0, -rel); }
@@ -180,7 +223,7 @@ struct Cursor {
                 load_request(p);
             } while (tiles == 0);
         }
-        G = tile_groups(p, u);
+        G = tile_units(p, u);
     }
 };
 
@@ -304,203 +347,345 @@ __device__ __forceinline__ void finish4(const Split &p, int r, int hq, int d, co
     }
 }
 
+__device__ __forceinline__ void bar_consumers(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+
+// The producer's view of the line: the first place of CTA c.
+__device__ __forceinline__ long long line_start(int c, long long per, int rest) { return c * per + min(c, rest); }
+__device__ __forceinline__ int line_owner(long long place, long long total, int grid, long long per, int rest) {
+    int c = min(grid - 1, (int)((double)place / (double)total * grid));
+    while (c + 1 < grid && line_start(c + 1, per, rest) <= place) ++c;
+    while (line_start(c, per, rest) > place) --c;
+    return c;
+}
+
+// One warp: the item's queries as the first product's B fragments; lane (g, t)
+// holds row g, elements 32 b + 8 t .. + 7.
 template <typename T, int D, int NT, bool STEP>
-__global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_kernel(const Split p) {
+__device__ __forceinline__ void prepare_queries(const Split &p, const Cursor<8 * NT> &at, int rows, int row0,
+                                                typename Shape<T, D, NT>::Slot &slot) {
+    using H = Shape<T, D, NT>;
+    constexpr int NB = H::NB;
+    const Attend &a = p.a;
+    const int lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = nt * 8 + lg;
+        float x[NB][8];
+        const bool live = row < rows;
+        const int tok = (row0 + row) / a.rep, hq = at.h * a.rep + (row0 + row) % a.rep;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
+        if (live) {
+            const T *src;
+            if constexpr (STEP)
+                src = reinterpret_cast<const T *>(p.qkv) + ((int64_t)at.b * (a.heads + 2 * a.c.kv_heads) + hq) * D;
+            else
+                src = static_cast<const T *>(a.q) + (at.first + tok) * a.q_token + hq * a.q_head;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) load8<T>(src + b * 32 + lt * 8, x[b]);
+        }
+        if constexpr (STEP) {
+            const int64_t pos = max((int64_t)0, min((int64_t)at.S - 1, p.rope_rows - 1));
+            rotate<D>(p.rope + pos * D, lt, x);
+        }
+        // the row's largest magnitude goes to [2^13, 2^14): no element overflows f16, and one that loses bits there
+        // lies 2^27 below it
+        float scale = 1.0f, back = 1.0f;
+        if constexpr (!std::is_same<T, __half>::value) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[b][i]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            if (amax > 0.0f && amax < INFINITY) {
+                const int e = min(max(267 - (int)(__float_as_uint(amax) >> 23), 1), 253);
+                scale = __uint_as_float((uint32_t)e << 23);
+                back = __uint_as_float((uint32_t)(254 - e) << 23);
+            }
+        }
+        float sums[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t f16[H::NQ][4];
+            sums[b] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x0 = x[b][2 * j] * scale, x1 = x[b][2 * j + 1] * scale;
+                f16[0][j] = pack_f16(x0, x1);
+                const float2 f = unpack_f16(f16[0][j]);
+                if constexpr (H::NQ == 2) f16[1][j] = pack_f16(x0 - f.x, x1 - f.y);
+                if (j & 1) sums[b] += f.x + f.y;
+            }
+#pragma unroll
+            for (int k = 0; k < H::NQ; ++k) slot.q[nt][b][k][lane] = make_uint4(f16[k][0], f16[k][1], f16[k][2], f16[k][3]);
+            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 1);
+            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 2);
+        }
+        const int seen = live ? at.S - at.n + tok + 1 : 0;  // keys that row g sees
+        const float c = a.scale * 1.4426950408889634f * back;
+        const int from0 = 8 * lt, from1 = from0 + 4;  // lanes of rows 2t and 2t + 1
+        slot.to_log2[nt][lane] = make_float2(__shfl_sync(0xffffffffu, c, from0), __shfl_sync(0xffffffffu, c, from1));
+        slot.limit[nt][lane] = make_int2(__shfl_sync(0xffffffffu, seen, from0), __shfl_sync(0xffffffffu, seen, from1));
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float s0 = __shfl_sync(0xffffffffu, sums[b], from0), s1 = __shfl_sync(0xffffffffu, sums[b], from1);
+            slot.start[nt][b][lane] = H::F32 ? make_float2(0.0f, 0.0f) : make_float2(-72.0f * s0, -72.0f * s1);
+        }
+    }
+}
+
+template <typename T, int D, int NT, bool STEP>
+__global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kernel(const Split p) {
     using Q = KvQ4<D>;
-    using R = Ring<D>;
-    constexpr int NB = Q::NB, RT = 8 * NT, W = R::WARPS;
-    constexpr bool F32 = sizeof(T) == 4, BF = std::is_same<T, __nv_bfloat16>::value;
-    constexpr int NQ = F32 ? 2 : 1;   // f16 terms of a query element
-    constexpr int NP = BF ? 1 : 2;    // f16 terms of a probability
+    using H = Shape<T, D, NT>;
+    constexpr int NB = Q::NB, RT = 8 * NT, W = H::W, STAGES = H::STAGES, THREADS = 32 * W;
+    constexpr bool F32 = H::F32, BF = H::BF;
+    constexpr int NQ = H::NQ, NP = H::NP;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[W][R::STAGES];
-    __shared__ float ml_sm[W][8][2];
-    __shared__ int is_last;
-    float *merge = reinterpret_cast<float *>(smem + R::BYTES);
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full[2], q_empty[2];
+    __shared__ uint8_t gone_sm[STAGES][W];  // per unit, a bit for each group without a page
+    __shared__ float ml_sm[W][8][2], sum_sm[8][2];
+    __shared__ int is_last, stop;
+    uint8_t *ring = smem;
+    float *merge = reinterpret_cast<float *>(smem + H::RING);
+    typename H::Slot *slots = reinterpret_cast<typename H::Slot *>(smem + H::RING + H::MERGE);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lg = lane >> 2, lt = lane & 3;
-    uint8_t *ring = smem + warp * R::STAGES * Q::GROUP_BYTES;
-    if (lane == 0) {
-        for (int s = 0; s < R::STAGES; ++s) mbar_init(&bars[warp][s], 1);
+    const Attend &a = p.a;
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], W);
+            mbar_init(&empty[s], W);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&q_full[s], 1);
+            mbar_init(&q_empty[s], W);
+        }
+        stop = 0;
         fence_mbar_init();
     }
-    __syncwarp();
+    __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- this CTA's places in the line
-    const Attend &a = p.a;
-    Cursor<RT> at;
-    long long total = 0;
-    for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
-        long long w = 0;
-        at.b = b0 + lane;
-        if (at.b < a.c.requests) {
-            at.load_request(a);
-            w = at.request_places(a);
-        }
-#pragma unroll
-        for (int off = 16; off; off >>= 1) w += __shfl_xor_sync(0xffffffffu, w, off);
-        total += w;
-    }
-    if (total == 0) return;
-    const int grid = (int)min((long long)gridDim.x, max(1ll, total / p.min_units));
-    const int cta = blockIdx.x;
-    if (cta >= grid) return;
-    const long long lo = cta * total / grid;
-    const int len = (int)((cta + 1) * total / grid - lo);
-    long long place = 0;  // of the current request, then tile
-    {
+    if (warp == W) {
+        // ---- the producer: this CTA's part of the line
+        Cursor<RT> at;
+        long long total = 0, own = 0;
         for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
-            long long w = 0;
+            own = 0;
             at.b = b0 + lane;
             if (at.b < a.c.requests) {
                 at.load_request(a);
-                w = at.request_places(a);
+                own = at.request_places(a);
             }
-            long long upto = w;
+            long long w = own;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, upto, off);
-                if (lane >= off) upto += v;
+            for (int off = 16; off; off >>= 1) w += __shfl_xor_sync(0xffffffffu, w, off);
+            total += w;
+        }
+        const int grid = (int)min((long long)gridDim.x, max(1ll, total / p.min_places));
+        const int cta = blockIdx.x;
+        int len = 0;
+        const long long per = total / grid;
+        const int rest = (int)(total - per * grid);
+        const long long lo = line_start(cta, per, rest);
+        if (cta < grid && total > 0) {
+            len = (int)(line_start(cta + 1, per, rest) - lo);
+            long long place = 0;  // of the current request, then tile
+            for (int b0 = 0;; b0 += 32) {
+                if (a.c.requests > 32) {
+                    own = 0;
+                    at.b = b0 + lane;
+                    if (at.b < a.c.requests) {
+                        at.load_request(a);
+                        own = at.request_places(a);
+                    }
+                }
+                long long upto = own;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const long long v = __shfl_up_sync(0xffffffffu, upto, off);
+                    if (lane >= off) upto += v;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, place + upto > lo);
+                if (past) {
+                    const int l0 = __ffs(past) - 1;
+                    place += __shfl_sync(0xffffffffu, upto - own, l0);
+                    at.b = b0 + l0;
+                    break;
+                }
+                place += __shfl_sync(0xffffffffu, upto, 31);
             }
-            const unsigned past = __ballot_sync(0xffffffffu, place + upto > lo);
-            if (past) {
-                const int l0 = __ffs(past) - 1;
-                place += __shfl_sync(0xffffffffu, upto - w, l0);
-                at.b = b0 + l0;
+            at.load_request(a);
+            for (at.u = 0;; ++at.u) {
+                at.G = at.tile_units(a, at.u);
+                const long long places = (long long)(at.G + kItemCost) * a.c.kv_heads;
+                if (place + places > lo) break;
+                place += places;
+            }
+            at.h = 0;
+            while (place + at.G + kItemCost <= lo) place += at.G + kItemCost, ++at.h;
+            at.rel = (int)(place + kItemCost - lo);
+        } else {
+            at.rel = 0;  // len is 0: nothing to do
+        }
+
+        // lane w's next unit, of the units w, w + W, ..
+        Cursor<RT> mine = at;
+        const int *row = nullptr;
+        int g = 0;
+        bool have = lane < W && len > 0;
+        auto settle = [&]() {  // g may lie behind the item's units: go on to the item that has it
+            while (g >= mine.upto(len)) {
+                if (mine.rel >= len) {
+                    have = false;
+                    return;
+                }
+                g -= max(mine.from(), mine.upto(len));
+                mine.next_item(a);
+                g += mine.from();
+            }
+            row = a.c.table + mine.b * a.c.table_stride;
+        };
+        if (have) {
+            g = mine.from() + lane;
+            settle();
+        }
+        int i0 = 0, m = 0, k = 0;
+        bool broken = false;
+        for (; __any_sync(0xffffffffu, have) && !broken; ++k) {
+            const int s = k % STAGES;
+            if (k >= STAGES && !mbar_wait(&empty[s], (k / STAGES - 1) & 1)) broken = true;
+            if (__any_sync(0xffffffffu, broken)) {
+                broken = true;
                 break;
             }
-            place += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        at.load_request(a);
-        for (at.u = 0;; ++at.u) {
-            at.G = at.tile_groups(a, at.u);
-            const long long places = (long long)(at.G + kItemCost) * a.c.kv_heads;
-            if (place + places > lo) break;
-            place += places;
-        }
-        at.h = (int)((lo - place) / (at.G + kItemCost));
-        at.rel = (int)(place + (long long)at.h * (at.G + kItemCost) + kItemCost - lo);
-    }
-
-    // ---- the ring: this warp's k-th group goes to stage k % STAGES; the CTA's groups go round its warps
-    Cursor<RT> ahead = at;
-    const int *ahead_row = a.c.table + ahead.b * a.c.table_stride;
-    int ahead_g = ahead.from() + warp, ahead_k = 0;
-    uint32_t bad = 0;  // stages whose group has no page
-    bool broken = false;
-    auto issue = [&]() {
-        if (ahead_g >= ahead.upto(len)) {
-            do {
-                if (ahead.rel >= len) return;
-                ahead_g -= max(ahead.from(), ahead.upto(len));
-                ahead.next_item(a);
-                ahead_g += ahead.from();
-            } while (ahead_g >= ahead.upto(len));
-            ahead_row = a.c.table + ahead.b * a.c.table_stride;
-        }
-        if (broken) return;
-        const int s = ahead_k % R::STAGES;
-        const uint8_t *src = nullptr;
-        if (ahead_g * kKvGroup < ahead.S) src = a.c.group_of_row<D>(ahead_row, ahead.h, ahead_g);
-        bad = src ? bad & ~(1u << s) : bad | (1u << s);
-        if (lane == 0) {
-            if (src) {
-                mbar_arrive_expect_tx(&bars[warp][s], Q::GROUP_BYTES);
-                bulk_g2s(ring + s * Q::GROUP_BYTES, src, Q::GROUP_BYTES, &bars[warp][s]);
-            } else {
-                mbar_arrive(&bars[warp][s]);
+            if (lane < W) {
+                uint8_t *dst = ring + (s * W + lane) * H::UNIT;
+                uint32_t gone = 3;
+                if (have) {
+                    // a unit's two groups lie together, unless pages hold one group
+                    const int group = g * kUnitGroups;
+                    if (a.c.page_shift > 4) {
+                        const uint8_t *src = nullptr;
+                        if (group * kKvGroup < mine.S) src = a.c.group_of_row<D>(row, mine.h, group);
+                        if (src) {
+                            gone = 0;
+                            gone_sm[s][lane] = 0;
+                            mbar_arrive_expect_tx(&full[s], H::UNIT);
+                            bulk_g2s(dst, src, H::UNIT, &full[s]);
+                        }
+                    } else {
+                        const uint8_t *src[2] = {nullptr, nullptr};
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if ((group + j) * kKvGroup < mine.S) src[j] = a.c.group_of_row<D>(row, mine.h, group + j);
+                            if (src[j]) gone &= ~(1u << j);
+                        }
+                        if (gone != 3) {
+                            gone_sm[s][lane] = (uint8_t)gone;
+                            mbar_arrive_expect_tx(&full[s], gone ? Q::GROUP_BYTES : 2 * Q::GROUP_BYTES);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                if (src[j]) bulk_g2s(dst + j * Q::GROUP_BYTES, src[j], Q::GROUP_BYTES, &full[s]);
+                        }
+                    }
+                }
+                if (gone == 3) {
+                    gone_sm[s][lane] = 3;
+                    mbar_arrive(&full[s]);
+                }
+                if (have) {
+                    g += W;
+                    settle();
+                }
+            }
+            __syncwarp();
+            // the items that begin in this stage, once its copies are on their way: an item's slot comes free when the
+            // one before the last has begun, which may need this stage
+            while (at.rel < len && i0 < (k + 1) * W) {
+                const int g0 = at.from(), g1 = at.upto(len);
+                if (g0 < g1) {
+                    typename H::Slot &slot = slots[m & 1];
+                    if (m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
+                    if (__any_sync(0xffffffffu, broken)) {
+                        broken = true;
+                        break;
+                    }
+                    const int row0 = at.u * RT, rows = min(RT, at.n * a.rep - row0);
+                    prepare_queries<T, D, NT, STEP>(p, at, rows, row0, slot);
+                    if (lane == 0) {
+                        Item it;
+                        it.end = 0;
+                        it.g0 = g0, it.g1 = g1, it.i0 = i0;
+                        it.whole = g0 == 0 && g1 == at.G;
+                        it.c0 = it.c1 = cta;
+                        if (!it.whole) {
+                            it.c0 = line_owner(lo + at.rel, total, grid, per, rest);
+                            it.c1 = line_owner(lo + at.rel + at.G - 1, total, grid, per, rest);
+                        }
+                        it.b = at.b, it.h = at.h, it.S = at.S;
+                        it.rows = rows, it.row0 = row0, it.first = at.first;
+                        it.all_see = at.S - at.n + row0 / a.rep + 1;
+                        slot.item = it;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&q_full[m & 1]);
+                    i0 += g1 - g0;
+                    ++m;
+                }
+                at.next_item(a);
             }
         }
-        ahead_g += W;
-        ++ahead_k;
-    };
-    for (int s = 0; s < R::STAGES - 1; ++s) issue();
+        if (!broken && m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
+        broken = __any_sync(0xffffffffu, broken);
+        if (broken) {
+            // copies still on their way (each wait bounded) before the shared memory goes
+            if (lane == 0) record_device_error(a.c.err, DEV_ERR_WAIT_EMPTY);
+            for (int j = max(0, k - STAGES); j < k; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1);
+        } else if (lane == 0) {
+            slots[m & 1].item.end = 1;
+            mbar_arrive(&q_full[m & 1]);
+        }
+        return;
+    }
 
-    int turn = warp, my_k = 0;  // groups of the CTA until this warp's next one
-    int broken_k = 0;
-    for (; at.rel < len; at.next_item(a)) {
-        // ---- one item, or this CTA's part of it
-        const int g0 = at.from(), g1 = at.upto(len);
-        if (g0 >= g1) continue;
-        const int rows = min(RT, at.n * a.rep - at.u * RT);
-        const int row0 = at.u * RT;
-
-        // ---- queries as the first product's B fragments: lane (g, t) holds row g, elements 32 b + 8 t .. + 7
+    // ---- a consumer
+    const uint32_t f16_1024 = p.f16_1024, f16_64 = p.f16_64;
+    int my_i = warp, my_k = 0;
+    bool broken = false;
+    for (int m = 0;; ++m) {
+        typename H::Slot &slot = slots[m & 1];
+        if (warp == 0 && !mbar_wait(&q_full[m & 1], (m / 2) & 1)) {
+            record_device_error(a.c.err, DEV_ERR_WAIT_FULL);
+            stop = 1;
+        }
+        bar_consumers(THREADS);  // and the merge buffer is free again
+        if (*(volatile int *)&stop) return;
+        const Item it = slot.item;
+        if (it.end) return;
         uint32_t qf[NT][NB][NQ][4];
-        float start[NT][NB][2];  // what a score's accumulator starts from, for the columns 2t, 2t + 1
+        float start[NT][NB][2];
         float to_log2[NT][2];
         int limit[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int row = nt * 8 + lg;
-            float x[NB][8];
-            const bool live = row < rows;
-            const int tok = (row0 + row) / a.rep, hq = at.h * a.rep + (row0 + row) % a.rep;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
-            if (live) {
-                const T *src;
-                if constexpr (STEP)
-                    src = reinterpret_cast<const T *>(p.qkv) + ((int64_t)at.b * (a.heads + 2 * a.c.kv_heads) + hq) * D;
-                else
-                    src = static_cast<const T *>(a.q) + (at.first + tok) * a.q_token + hq * a.q_head;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) load8<T>(src + b * 32 + lt * 8, x[b]);
-            }
-            if constexpr (STEP) {
-                const int64_t pos = max((int64_t)0, min((int64_t)at.S - 1, p.rope_rows - 1));
-                rotate<D>(p.rope + pos * D, lt, x);
-            }
-            // the row's largest magnitude goes to [2^13, 2^14): no element overflows f16, and one that loses bits there
-            // lies 2^27 below it
-            float scale = 1.0f, back = 1.0f;
-            if constexpr (!std::is_same<T, __half>::value) {
-                float amax = 0.0f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[b][i]));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                if (amax > 0.0f && amax < INFINITY) {
-                    const int e = min(max(267 - (int)(__float_as_uint(amax) >> 23), 1), 253);
-                    scale = __uint_as_float((uint32_t)e << 23);
-                    back = __uint_as_float((uint32_t)(254 - e) << 23);
-                }
-            }
-            float sums[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                sums[b] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float x0 = x[b][2 * j] * scale, x1 = x[b][2 * j + 1] * scale;
-                    qf[nt][b][0][j] = pack_f16(x0, x1);
-                    const float2 f = unpack_f16(qf[nt][b][0][j]);
-                    if constexpr (NQ == 2) qf[nt][b][1][j] = pack_f16(x0 - f.x, x1 - f.y);
-                    if (j & 1) sums[b] += f.x + f.y;
-                }
-                sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 1);
-                sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 2);
+                for (int q = 0; q < NQ; ++q) *reinterpret_cast<uint4 *>(qf[nt][b][q]) = slot.q[nt][b][q][lane];
+                *reinterpret_cast<float2 *>(start[nt][b]) = slot.start[nt][b][lane];
             }
-            const int seen = live ? at.S - at.n + tok + 1 : 0;  // keys that row g sees
-            const float c = a.scale * 1.4426950408889634f * back;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int from = (2 * lt + j) * 4;
-                to_log2[nt][j] = __shfl_sync(0xffffffffu, c, from);
-                limit[nt][j] = __shfl_sync(0xffffffffu, seen, from);
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    start[nt][b][j] = F32 ? 0.0f : -72.0f * __shfl_sync(0xffffffffu, sums[b], from);
-            }
+            *reinterpret_cast<float2 *>(to_log2[nt]) = slot.to_log2[nt][lane];
+            *reinterpret_cast<int2 *>(limit[nt]) = slot.limit[nt][lane];
         }
-        // the fewest keys that a row of the tile sees: groups below need no mask
-        const int all_see = rows == RT ? at.S - at.n + row0 / a.rep + 1 : 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[m & 1]);
 
         float o[NT][NB][2][4], l[NT][2], off[NT][2];
         float high[NT][2];  // the row's reference + kSlack: scores above move it
@@ -519,76 +704,83 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                     for (int i = 0; i < 4; ++i) o[nt][b][k][i] = 0.0f;
         }
 
-        // One group; `mask` where a row may not see all of its tokens.
-        auto take = [&](const uint8_t *buf, int group, auto mask) {
+        // One unit, tokens token0 .. + 31; `mask` where a row may not see all of them, or a group is gone.
+        auto take = [&](const uint8_t *unit_buf, int token0, uint32_t gone, auto mask) {
             constexpr bool masked = decltype(mask)::value;
-
-            // ---- scores
-            uint32_t kw[2][NB];
+            float s[kUnitGroups][NT][4];
+            bool low = false;
+            float vmax = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint8_t *src = buf + Q::K_CODES + (lg + 8 * k) * (D / 2) + lt * NB * 4;
-                if constexpr (NB == 4)
-                    *reinterpret_cast<uint4 *>(kw[k]) = *reinterpret_cast<const uint4 *>(src);
-                else
-                    *reinterpret_cast<uint2 *>(kw[k]) = *reinterpret_cast<const uint2 *>(src);
-            }
-            uint32_t ks[2][NB / 2];
+            for (int u = 0; u < kUnitGroups; ++u) {
+                const uint8_t *buf = unit_buf + u * Q::GROUP_BYTES;
+                // ---- scores
+                uint32_t kw[2][NB];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint8_t *src = buf + Q::K_SCALES + (lg + 8 * k) * NB * 2;
-                if constexpr (NB == 4)
-                    *reinterpret_cast<uint2 *>(ks[k]) = *reinterpret_cast<const uint2 *>(src);
-                else
-                    ks[k][0] = *reinterpret_cast<const uint32_t *>(src);
-            }
-            float s[NT][4];
+                for (int k = 0; k < 2; ++k) {
+                    const uint8_t *src = buf + Q::K_CODES + (lg + 8 * k) * (D / 2) + lt * NB * 4;
+                    if constexpr (NB == 4)
+                        *reinterpret_cast<uint4 *>(kw[k]) = *reinterpret_cast<const uint4 *>(src);
+                    else
+                        *reinterpret_cast<uint2 *>(kw[k]) = *reinterpret_cast<const uint2 *>(src);
+                }
+                uint32_t ks[2][NB / 2];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                uint32_t e0[4], e1[4];
-                unpack_codes<!F32>(kw[0][b], e0);
-                unpack_codes<!F32>(kw[1][b], e1);
-                const float2 f0 = unpack_f16(ks[0][b / 2]), f1 = unpack_f16(ks[1][b / 2]);
-                const float d0 = b & 1 ? f0.y : f0.x, d1 = b & 1 ? f1.y : f1.x;
+                for (int k = 0; k < 2; ++k) {
+                    const uint8_t *src = buf + Q::K_SCALES + (lg + 8 * k) * NB * 2;
+                    if constexpr (NB == 4)
+                        *reinterpret_cast<uint2 *>(ks[k]) = *reinterpret_cast<const uint2 *>(src);
+                    else
+                        ks[k][0] = *reinterpret_cast<const uint32_t *>(src);
+                }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float c0[4] = {start[nt][b][0], start[nt][b][1], start[nt][b][0], start[nt][b][1]};
-                    float acc[4];
-                    mma16816(acc, e0[0], e1[0], e0[1], e1[1], qf[nt][b][0][0], qf[nt][b][0][1], c0);
-                    mma16816(acc, e0[2], e1[2], e0[3], e1[3], qf[nt][b][0][2], qf[nt][b][0][3], acc);
-                    if constexpr (NQ == 2) {
-                        mma16816(acc, e0[0], e1[0], e0[1], e1[1], qf[nt][b][1][0], qf[nt][b][1][1], acc);
-                        mma16816(acc, e0[2], e1[2], e0[3], e1[3], qf[nt][b][1][2], qf[nt][b][1][3], acc);
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t e0[4], e1[4];
+                    unpack_codes<!F32>(kw[0][b], e0, f16_1024, f16_64);
+                    unpack_codes<!F32>(kw[1][b], e1, f16_1024, f16_64);
+                    const float2 f0 = unpack_f16(ks[0][b / 2]), f1 = unpack_f16(ks[1][b / 2]);
+                    const float d0 = b & 1 ? f0.y : f0.x, d1 = b & 1 ? f1.y : f1.x;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float c0[4] = {start[nt][b][0], start[nt][b][1], start[nt][b][0], start[nt][b][1]};
+                        float acc[4];
+                        mma16816(acc, e0[0], e1[0], e0[1], e1[1], qf[nt][b][0][0], qf[nt][b][0][1], c0);
+                        mma16816(acc, e0[2], e1[2], e0[3], e1[3], qf[nt][b][0][2], qf[nt][b][0][3], acc);
+                        if constexpr (NQ == 2) {
+                            mma16816(acc, e0[0], e1[0], e0[1], e1[1], qf[nt][b][1][0], qf[nt][b][1][1], acc);
+                            mma16816(acc, e0[2], e1[2], e0[3], e1[3], qf[nt][b][1][2], qf[nt][b][1][3], acc);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float d = i < 2 ? d0 : d1;
+                            s[u][nt][i] = b == 0 ? acc[i] * d : fmaf(acc[i], d, s[u][nt][i]);
+                        }
                     }
+                }
+                // ---- references that are too low for a score, or for a value scale
+                const uint32_t vs_word =
+                    lane < 8 * NB ? *reinterpret_cast<const uint32_t *>(buf + Q::V_SCALES + lane * 4) : 0u;
+                const float2 vsf = unpack_f16(vs_word & 0x7fff7fffu);
+                float v = fmaxf(vsf.x, vsf.y);
+                if constexpr (masked) {
+                    if (token0 + u * kKvGroup + lane / (NB / 2) >= it.S || (gone >> u & 1)) v = 0.0f;
+                }
+                vmax = fmaxf(vmax, v);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float d = i < 2 ? d0 : d1;
-                        s[nt][i] = b == 0 ? acc[i] * d : fmaf(acc[i], d, s[nt][i]);
+                        s[u][nt][i] *= to_log2[nt][i & 1];
+                        if constexpr (masked) {
+                            if (token0 + u * kKvGroup + lg + 8 * (i >> 1) >= limit[nt][i & 1] || (gone >> u & 1))
+                                s[u][nt][i] = -INFINITY;
+                        }
+                        low |= s[u][nt][i] > high[nt][i & 1];
                     }
-                }
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[nt][i] *= to_log2[nt][i & 1];
-                    if (masked && group * kKvGroup + lg + 8 * (i >> 1) >= limit[nt][i & 1]) s[nt][i] = -INFINITY;
-                }
-
-            // ---- references that are too low for a score, or for a value scale
-            const uint32_t vs_word = lane < 8 * NB ? *reinterpret_cast<const uint32_t *>(buf + Q::V_SCALES + lane * 4) : 0u;
-            const float2 vsf = unpack_f16(vs_word & 0x7fff7fffu);
-            float vmax = fmaxf(vsf.x, vsf.y);
-            if (masked && group * kKvGroup + lane / (NB / 2) >= at.S) vmax = 0.0f;
-            bool low = vmax > vlim && vmax < INFINITY;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) low |= s[nt][i] > high[nt][i & 1];
-            if (__any_sync(0xffffffffu, low)) {
-                if (!(vmax < INFINITY)) vmax = 65504.0f;
+            if (__any_sync(0xffffffffu, low || vmax > vlim)) {
 #pragma unroll
                 for (int o2 = 16; o2; o2 >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o2));
+                vmax = fminf(vmax, 65504.0f);
                 if (vmax > vlim) {  // the power of two above it
                     const uint32_t e = (__float_as_uint(vmax) >> 23) + 1;
                     vlim = __uint_as_float(e << 23);
@@ -598,7 +790,9 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float m = fmaxf(s[nt][j], s[nt][j + 2]);
+                        float m = fmaxf(s[0][nt][j], s[0][nt][j + 2]);
+#pragma unroll
+                        for (int u = 1; u < kUnitGroups; ++u) m = fmaxf(m, fmaxf(s[u][nt][j], s[u][nt][j + 2]));
 #pragma unroll
                         for (int o2 = 4; o2 < 32; o2 <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
                         m = fmaxf(m, high[nt][j] - kSlack);
@@ -618,143 +812,141 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                     }
             }
 
-            // ---- probabilities, times the values' scales, as the second product's B fragments
-            uint32_t pf[NT][NB][NP][2];
-            if constexpr (BF) {
-                uint32_t vs[2][NB];  // (token 2t, token 2t + 1) of each block, and 2t + 8, 2t + 9
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint8_t *src = buf + Q::V_SCALES + (2 * lt + 8 * k) * NB * 2;
-                    if constexpr (NB == 4) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(src);
-                        vs[k][0] = __byte_perm(w.x, w.z, 0x5410);
-                        vs[k][1] = __byte_perm(w.x, w.z, 0x7632);
-                        vs[k][2] = __byte_perm(w.y, w.w, 0x5410);
-                        vs[k][3] = __byte_perm(w.y, w.w, 0x7632);
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2 *>(src);
-                        vs[k][0] = __byte_perm(w.x, w.y, 0x5410);
-                        vs[k][1] = __byte_perm(w.x, w.y, 0x7632);
-                    }
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        e[i] = exp2_approx(s[nt][i] + off[nt][i & 1]);
-                        l[nt][i & 1] += e[i];
-                    }
+            for (int u = 0; u < kUnitGroups; ++u) {
+                const uint8_t *buf = unit_buf + u * Q::GROUP_BYTES;
+                // ---- probabilities, times the values' scales, as the second product's B fragments
+                uint32_t pf[NT][NB][NP][2];
+                if constexpr (BF) {
+                    uint32_t vs[2][NB];  // (token 2t, token 2t + 1) of each block, and 2t + 8, 2t + 9
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const uint32_t pt = transpose8x8(pack_f16(e[2 * k], e[2 * k + 1]));  // (2t, 2t + 1) of row g
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            uint32_t v = mul_f16x2(pt, vs[k][b]);
-                            if (masked) {  // what a row does not see may hold anything
-                                if (!(pt & 0x0000ffffu)) v &= 0xffff0000u;
-                                if (!(pt & 0xffff0000u)) v &= 0x0000ffffu;
-                            }
-                            pf[nt][b][0][k] = v;
+                        const uint8_t *src = buf + Q::V_SCALES + (2 * lt + 8 * k) * NB * 2;
+                        if constexpr (NB == 4) {
+                            const uint4 w = *reinterpret_cast<const uint4 *>(src);
+                            vs[k][0] = __byte_perm(w.x, w.z, 0x5410);
+                            vs[k][1] = __byte_perm(w.x, w.z, 0x7632);
+                            vs[k][2] = __byte_perm(w.y, w.w, 0x5410);
+                            vs[k][3] = __byte_perm(w.y, w.w, 0x7632);
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(src);
+                            vs[k][0] = __byte_perm(w.x, w.y, 0x5410);
+                            vs[k][1] = __byte_perm(w.x, w.y, 0x7632);
                         }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float dv[NB];
-                    const uint8_t *src = buf + Q::V_SCALES + (lg + 8 * k) * NB * 2;
-#pragma unroll
-                    for (int b = 0; b < NB; b += 2) {
-                        const float2 f = unpack_f16(*reinterpret_cast<const uint32_t *>(src + b * 2));
-                        dv[b] = f.x, dv[b + 1] = f.y;
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float e[2];
+                        float e[4];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            e[j] = exp2_approx(s[nt][2 * k + j] + off[nt][j]);
-                            l[nt][j] += e[j];
+                        for (int i = 0; i < 4; ++i) {
+                            e[i] = exp2_approx(s[u][nt][i] + off[nt][i & 1]);
+                            l[nt][i & 1] += e[i];
                         }
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const float x0 = masked && s[nt][2 * k] == -INFINITY ? 0.0f : e[0] * dv[b];
-                            const float x1 = masked && s[nt][2 * k + 1] == -INFINITY ? 0.0f : e[1] * dv[b];
-                            const uint32_t h = pack_f16(x0, x1);
-                            const float2 f = unpack_f16(h);
-                            pf[nt][b][0][k] = transpose8x8(h);
-                            pf[nt][b][NP - 1][k] = transpose8x8(pack_f16(x0 - f.x, x1 - f.y));
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t pt = transpose8x8(pack_f16(e[2 * k], e[2 * k + 1]));  // (2t, 2t + 1) of row g
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) {
+                                uint32_t v = mul_f16x2(pt, vs[k][b]);
+                                if (masked) {  // what a row does not see may hold anything
+                                    if (!(pt & 0x0000ffffu)) v &= 0xffff0000u;
+                                    if (!(pt & 0xffff0000u)) v &= 0x0000ffffu;
+                                }
+                                pf[nt][b][0][k] = v;
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float dv[NB];
+                        const uint8_t *src = buf + Q::V_SCALES + (lg + 8 * k) * NB * 2;
+#pragma unroll
+                        for (int b = 0; b < NB; b += 2) {
+                            const float2 f = unpack_f16(*reinterpret_cast<const uint32_t *>(src + b * 2));
+                            dv[b] = f.x, dv[b + 1] = f.y;
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float e[2];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                e[j] = exp2_approx(s[u][nt][2 * k + j] + off[nt][j]);
+                                l[nt][j] += e[j];
+                            }
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) {
+                                const float x0 = masked && s[u][nt][2 * k] == -INFINITY ? 0.0f : e[0] * dv[b];
+                                const float x1 = masked && s[u][nt][2 * k + 1] == -INFINITY ? 0.0f : e[1] * dv[b];
+                                const uint32_t h = pack_f16(x0, x1);
+                                const float2 f = unpack_f16(h);
+                                pf[nt][b][0][k] = transpose8x8(h);
+                                pf[nt][b][NP - 1][k] = transpose8x8(pack_f16(x0 - f.x, x1 - f.y));
+                            }
                         }
                     }
                 }
-            }
 
-            // ---- values
-            uint32_t vw[2][NB];
+                // ---- values
+                uint32_t vw[2][NB];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint8_t *src = buf + Q::V_CODES + k * 4 * D + lane * NB * 4;
-                if constexpr (NB == 4)
-                    *reinterpret_cast<uint4 *>(vw[k]) = *reinterpret_cast<const uint4 *>(src);
-                else
-                    *reinterpret_cast<uint2 *>(vw[k]) = *reinterpret_cast<const uint2 *>(src);
-            }
+                for (int k = 0; k < 2; ++k) {
+                    const uint8_t *src = buf + Q::V_CODES + k * 4 * D + lane * NB * 4;
+                    if constexpr (NB == 4)
+                        *reinterpret_cast<uint4 *>(vw[k]) = *reinterpret_cast<const uint4 *>(src);
+                    else
+                        *reinterpret_cast<uint2 *>(vw[k]) = *reinterpret_cast<const uint2 *>(src);
+                }
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                uint32_t e0[4], e1[4];
-                unpack_codes<false>(vw[0][b], e0);
-                unpack_codes<false>(vw[1][b], e1);
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t e0[4], e1[4];
+                    unpack_codes<false>(vw[0][b], e0, f16_1024, f16_64);
+                    unpack_codes<false>(vw[1][b], e1, f16_1024, f16_64);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int q = 0; q < NP; ++q) {
-                        mma16816(o[nt][b][0], e0[0], e0[1], e1[0], e1[1], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][0]);
-                        mma16816(o[nt][b][1], e0[2], e0[3], e1[2], e1[3], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][1]);
-                    }
+                        for (int q = 0; q < NP; ++q) {
+                            mma16816(o[nt][b][0], e0[0], e0[1], e1[0], e1[1], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][0]);
+                            mma16816(o[nt][b][1], e0[2], e0[3], e1[2], e1[3], pf[nt][b][q][0], pf[nt][b][q][1], o[nt][b][1]);
+                        }
+                }
             }
         };
 
-        int group = g0 + turn;
-        for (; group < g1; group += W, ++my_k) {
-            const int stage = my_k % R::STAGES;
-            issue();
-            if (!broken && !mbar_wait(&bars[warp][stage], (my_k / R::STAGES) & 1)) {
+        for (; my_i < it.i0 + it.g1 - it.g0; my_i += W, ++my_k) {
+            const int stage = my_k % STAGES, unit = it.g0 + my_i - it.i0;
+            if (!broken && !mbar_wait(&full[stage], (my_k / STAGES) & 1)) {
                 record_device_error(a.c.err, DEV_ERR_WAIT_FULL);
                 broken = true;
             }
-            if (__any_sync(0xffffffffu, broken)) {
-                if (!broken_k) broken_k = my_k + 1;
-                broken = true;
-            }
-            if (broken || (bad >> stage & 1)) {
-                __syncwarp();
-                continue;
-            }
-            uint8_t *buf = ring + stage * Q::GROUP_BYTES;
-            if constexpr (STEP) {
-                // the group of the new token: its row goes into this copy and into the cache
-                if (group == (at.S - 1) >> 4) {
-                    append_new<D>(p, at.b, at.h, at.S - 1, buf);
-                    __syncwarp();
+            broken = __any_sync(0xffffffffu, broken);
+            const uint32_t gone = gone_sm[stage][warp];
+            if (!broken && gone != 3) {
+                uint8_t *buf = ring + (stage * W + warp) * H::UNIT;
+                if constexpr (STEP) {
+                    // the unit of the new token: its row goes into this copy and into the cache
+                    const int group = (it.S - 1) >> 4;
+                    if (group / kUnitGroups == unit && !(gone >> (group & 1) & 1)) {
+                        append_new<D>(p, it.b, it.h, it.S - 1, buf + (group & 1) * Q::GROUP_BYTES);
+                        __syncwarp();
+                    }
                 }
+                if ((unit + 1) * kUnit > it.all_see || gone)
+                    take(buf, unit * kUnit, gone, std::true_type{});
+                else
+                    take(buf, unit * kUnit, 0u, std::false_type{});
             }
-            if ((group + 1) * kKvGroup > all_see)
-                take(buf, group, std::true_type{});
-            else
-                take(buf, group, std::false_type{});
             __syncwarp();  // every lane has read the stage before a copy comes into it
+            if (lane == 0) mbar_arrive(&empty[stage]);
         }
 
-        turn = group - g1;
-
         // ---- the warps' results of the item, or of this CTA's part of it
-        const bool whole = g0 == 0 && g1 == at.G;
-        float *po = p.part_o + ((int64_t)cta * 2 + (g0 == 0)) * RT * D;
-        float *pml = p.part_ml + ((int64_t)cta * 2 + (g0 == 0)) * RT * 2;
+        const int64_t own_slot = (int64_t)blockIdx.x * 2 + (it.g0 == 0);
+        float *po = p.part_o + own_slot * RT * D;
+        float *pml = p.part_ml + own_slot * RT * 2;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if (nt) __syncthreads();
+            if (nt) bar_consumers(THREADS);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float sum = l[nt][j];
@@ -767,12 +959,11 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
-                    *reinterpret_cast<float4 *>(merge + (warp * 8 + 2 * lt + j) * R::ROW + b * 32 + lg * 4) =
+                    *reinterpret_cast<float4 *>(merge + (warp * 8 + 2 * lt + j) * H::ROW + b * 32 + lg * 4) =
                         make_float4(o[nt][b][0][j], o[nt][b][0][j + 2], o[nt][b][1][j], o[nt][b][1][j + 2]);
             }
-            __syncthreads();
-            // thread: row tid / (D/4) .. of the 8, four dimensions
-            for (int idx = tid; idx < 8 * (D / 4); idx += kSplitThreads) {
+            bar_consumers(THREADS);
+            for (int idx = tid; idx < 8 * (D / 4); idx += THREADS) {
                 const int row = idx / (D / 4), d = idx % (D / 4) * 4;
                 float least = INFINITY;
 #pragma unroll
@@ -783,7 +974,7 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                     for (int w = 0; w < W; ++w) {
                         if (ml_sm[w][row][0] == INFINITY) continue;
                         const float f = exp2_approx(least - ml_sm[w][row][0]);
-                        const float4 x = *reinterpret_cast<const float4 *>(merge + (w * 8 + row) * R::ROW + d);
+                        const float4 x = *reinterpret_cast<const float4 *>(merge + (w * 8 + row) * H::ROW + d);
                         v[0] = fmaf(f, x.x, v[0]);
                         v[1] = fmaf(f, x.y, v[1]);
                         v[2] = fmaf(f, x.z, v[2]);
@@ -792,86 +983,102 @@ __global__ void __launch_bounds__(kSplitThreads, NT == 1 ? 2 : 1) sdpa_q4_split_
                     }
                 }
                 const int rr = nt * 8 + row;
-                if (!whole) {
+                if (!it.whole) {
                     __stcg(reinterpret_cast<float4 *>(po + rr * D + d), make_float4(v[0], v[1], v[2], v[3]));
                     if (d == 0) __stcg(reinterpret_cast<float2 *>(pml + rr * 2), make_float2(least, sum));
-                } else if (rr < rows) {
+                } else if (rr < it.rows) {
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] *= inv;
-                    const int r = at.first + (row0 + rr) / a.rep, hq = at.h * a.rep + (row0 + rr) % a.rep;
+                    const int r = it.first + (it.row0 + rr) / a.rep, hq = it.h * a.rep + (it.row0 + rr) % a.rep;
                     finish4<T, D, STEP>(p, r, hq, d, v);
                     if (d == 0 && a.lse)
                         a.lse[(int64_t)r * a.heads + hq] = sum == 0.0f ? 0.0f : (log2f(sum) - least) * 0.6931471805599453f;
                 }
             }
         }
-        __syncthreads();
-        if (!whole) {
-            // The item lies in CTAs c0 .. c1. Each sets its flag behind its part and then looks at the others': the
-            // fences put one CTA's look behind everyone's flag, and that one (now and then two, with the same result)
-            // joins the parts in order. A flag is this launch's number, so that what lay in the workspace does not
-            // matter, and goes back to 0, so that a replay of the launch finds none set.
-            const long long first = lo + at.rel;
-            const int c0 = (int)(((first + 1) * grid - 1) / total), c1 = (int)(((first + at.G) * grid - 1) / total);
-            auto slot = [&](int c) { return (int64_t)c * 2 + (c == c0); };
-            if (warp == 0) {
-                if (lane == 0) {
-                    __threadfence();
-                    *reinterpret_cast<volatile unsigned long long *>(p.flags + slot(cta)) = p.nonce;
-                }
-                __syncwarp();
+        if (it.whole) continue;
+
+        // The item lies in CTAs c0 .. c1. Each sets its flag behind its part and then looks at the others': the fences
+        // put one CTA's look behind everyone's flag, and that one (now and then two, with the same result) joins the
+        // parts in order. A flag is this launch's number, so that what lay in the workspace does not matter, and goes
+        // back to 0, so that a replay of the launch finds none set.
+        const int c0 = it.c0, c1 = it.c1;
+        auto part = [&](int c) { return (int64_t)c * 2 + (c == c0); };
+        bar_consumers(THREADS);
+        if (warp == 0) {
+            if (lane == 0) {
                 __threadfence();
-                bool all = true;
-                for (int c = c0 + lane; c <= c1; c += 32)
-                    all &= *reinterpret_cast<const volatile unsigned long long *>(p.flags + slot(c)) == p.nonce;
-                all = __all_sync(0xffffffffu, all);
-                __threadfence();
-                if (lane == 0) is_last = all;
+                *reinterpret_cast<volatile unsigned long long *>(p.flags + own_slot) = p.nonce;
             }
-            __syncthreads();
-            if (is_last) {
-                for (int idx = tid; idx < RT * (D / 4); idx += kSplitThreads) {
-                    const int rr = idx / (D / 4), d = idx % (D / 4) * 4;
-                    float least = INFINITY;
-                    for (int c = c0; c <= c1; ++c) least = fminf(least, __ldcg(p.part_ml + (slot(c) * RT + rr) * 2));
-                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-                    if (least < INFINITY) {
-#pragma unroll 4
-                        for (int c = c0; c <= c1; ++c) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + (slot(c) * RT + rr) * 2));
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (slot(c) * RT + rr) * D + d));
-                            const float f = ml.x == INFINITY ? 0.0f : exp2_approx(least - ml.x);
-                            if (ml.x == INFINITY) continue;
-                            v[0] = fmaf(f, x.x, v[0]);
-                            v[1] = fmaf(f, x.y, v[1]);
-                            v[2] = fmaf(f, x.z, v[2]);
-                            v[3] = fmaf(f, x.w, v[3]);
-                            sum = fmaf(f, ml.y, sum);
-                        }
-                    }
-                    if (rr < rows) {
-                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] *= inv;
-                        const int r = at.first + (row0 + rr) / a.rep, hq = at.h * a.rep + (row0 + rr) % a.rep;
-                        finish4<T, D, STEP>(p, r, hq, d, v);
-                        if (d == 0 && a.lse)
-                            a.lse[(int64_t)r * a.heads + hq] =
-                                sum == 0.0f ? 0.0f : (log2f(sum) - least) * 0.6931471805599453f;
-                    }
-                }
-                __syncthreads();
-                for (int c = c0 + tid; c <= c1; c += kSplitThreads) p.flags[slot(c)] = 0;
-            }
+            __syncwarp();
+            __threadfence();
+            bool all = true;
+            for (int c = c0 + lane; c <= c1; c += 32)
+                all &= *reinterpret_cast<const volatile unsigned long long *>(p.flags + part(c)) == p.nonce;
+            all = __all_sync(0xffffffffu, all);
+            __threadfence();
+            if (lane == 0) is_last = all;
         }
-    }
-    if (broken) {  // copies still on their way (each wait bounded) before the shared memory goes
-        for (int k = broken_k - 1; k < ahead_k; ++k) mbar_wait(&bars[warp][k % R::STAGES], (k / R::STAGES) & 1);
+        bar_consumers(THREADS);
+        if (!is_last) continue;
+        // eight rows at a time: 16 lanes a row find the parts' common reference and weights, then a thread adds up four
+        // dimensions of a row, eight parts in flight
+        const int parts = c1 - c0 + 1;
+#pragma unroll 1
+        for (int nt = 0; nt < NT; ++nt) {
+            const int wr = tid >> 4, wl = tid & 15;
+            if (wr < 8) {
+                float least = INFINITY, sum = 0.0f;
+#pragma unroll 4
+                for (int c = c0 + wl; c <= c1; c += 16)
+                    least = fminf(least, __ldcg(p.part_ml + (part(c) * RT + nt * 8 + wr) * 2));
+#pragma unroll
+                for (int o2 = 8; o2; o2 >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o2));
+#pragma unroll 4
+                for (int c = c0 + wl; c <= c1; c += 16) {
+                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + (part(c) * RT + nt * 8 + wr) * 2));
+                    const float f = ml.x == INFINITY ? 0.0f : exp2_approx(least - ml.x);
+                    merge[wr * parts + c - c0] = f;
+                    sum = fmaf(f, ml.y, sum);
+                }
+#pragma unroll
+                for (int o2 = 8; o2; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+                if (wl == 0) {
+                    sum_sm[wr][0] = least;
+                    sum_sm[wr][1] = sum;
+                }
+            }
+            bar_consumers(THREADS);
+            for (int idx = tid; idx < 8 * (D / 4); idx += THREADS) {
+                const int row = idx / (D / 4), d = idx % (D / 4) * 4, rr = nt * 8 + row;
+                if (rr >= it.rows) continue;
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float *w = merge + row * parts;
+                const float *src = p.part_o + rr * D + d;
+#pragma unroll 8
+                for (int c = 0; c < parts; ++c) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + part(c0 + c) * (RT * D)));
+                    const float f = w[c];
+                    v[0] = fmaf(f, x.x, v[0]);
+                    v[1] = fmaf(f, x.y, v[1]);
+                    v[2] = fmaf(f, x.z, v[2]);
+                    v[3] = fmaf(f, x.w, v[3]);
+                }
+                const float all_l = sum_sm[row][1], inv = all_l == 0.0f ? 0.0f : 1.0f / all_l;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= inv;
+                const int r = it.first + (it.row0 + rr) / a.rep, hq = it.h * a.rep + (it.row0 + rr) % a.rep;
+                finish4<T, D, STEP>(p, r, hq, d, v);
+                if (d == 0 && a.lse)
+                    a.lse[(int64_t)r * a.heads + hq] =
+                        all_l == 0.0f ? 0.0f : (log2f(all_l) - sum_sm[row][0]) * 0.6931471805599453f;
+            }
+            bar_consumers(THREADS);
+        }
+        for (int c = c0 + tid; c <= c1; c += THREADS) p.flags[part(c)] = 0;
     }
 }
-
-constexpr int kMaxGrid = 296;  // CTAs whose parts a workspace holds
 
 // The rows of a tile: 8 hold every head that shares a KV head in decode (up to 8); more rows a request make
 // tiles of 16, which read the cache half as often.
@@ -894,16 +1101,18 @@ int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op)
     int st = device_facts(&f);
     if (st) return st;
     constexpr int rows = 8 * NT;
-    const int grid = std::min(f.sm_count * (NT == 1 ? 2 : 1), kMaxGrid);
+    const int grid = std::min(f.sm_count, kMaxGrid);
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = p.part_o + (int64_t)kMaxGrid * 2 * rows * D;
     p.flags = reinterpret_cast<unsigned long long *>(p.part_ml + (int64_t)kMaxGrid * 2 * rows * 2);
     p.nonce = next_nonce();
-    auto kernel = sdpa_q4_split_kernel<T, D, NT, STEP>;
-    st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<D>::SMEM), op,
+    p.f16_1024 = 0x64006400u;
+    p.f16_64 = 0x54005400u;
+    auto kernel = sdpa_q4_kernel<T, D, NT, STEP>;
+    st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D, NT>::SMEM), op,
                     "cudaFuncSetAttribute");
     if (st) return st;
-    return launch_pdl(kernel, dim3((unsigned)grid), dim3(kSplitThreads), Ring<D>::SMEM, stream, op, p);
+    return launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * (Shape<T, D, NT>::W + 1)), Shape<T, D, NT>::SMEM, stream, op, p);
 }
 
 template <typename T, int D>
@@ -965,7 +1174,7 @@ extern "C" int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strid
         return tn::set_error(TN_ERR_INVALID, std::string(op) + ": the workspace must be 16-byte aligned");
     tn::Split p{};
     p.a = {q, q_strides[0], q_strides[1], c, query_start, out, lse, (int)tokens, (int)heads, (int)(heads / kv_heads), sc};
-    p.min_units = 8;
+    p.min_places = 24;
     __atomic_fetch_add(&tn::counters().sdpa_calls, 1ull, __ATOMIC_RELAXED);
     __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     cudaStream_t s = tn::stream_of(stream);
@@ -1010,7 +1219,7 @@ extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t
     __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     tn::Split p{};
     p.a = {nullptr, 0, 0, c, nullptr, out, lse, (int)requests, (int)heads, (int)(heads / kv_heads), sc};
-    p.min_units = 8;
+    p.min_places = 24;
     p.qkv = (const __nv_bfloat16 *)qkv;
     p.rope = (const __nv_bfloat16 *)rope;
     p.rope_rows = rope_rows;
