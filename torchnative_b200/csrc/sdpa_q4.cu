@@ -35,9 +35,8 @@ struct Attend {
 // lengths, which only the device knows.
 //
 // A CTA is W consumer warps and a producer warp, one CTA an SM. Unit i of a CTA
-// goes to warp i mod W. Lane w of the producer walks the line for warp w and
-// brings its units (36 D bytes, one bulk copy where a page holds 32 tokens) to
-// stage i / W of a ring; a stage is filled again when every warp is through with
+// goes to warp i mod W, through stage i / W of a ring that the producer's bulk
+// copies fill; a stage is filled again when every warp is through with
 // it, so that the warps stay together: without that bound the SM's scheduler let
 // some run ahead, and the last ones ended alone (127 us of 82 at 2 x 100,000
 // tokens of 8 heads). The producer also prepares each item's queries.
@@ -68,9 +67,19 @@ struct Item {
     int g0, g1;          // this CTA's units of it
     int i0;              // the CTA's units before
     int whole, c0, c1;   // all of its units; otherwise the CTAs that have some
-    int b, h, S;
+    int h, S;
+    int new_unit;        // decode step: the unit of the new token, -1 where this CTA has it not
     int rows, row0;      // query rows of the tile, of the request before it
     int first, all_see;  // the request's first packed token; keys that every row of the tile sees
+};
+
+// A token's bytes in its group: K words, V pieces by element, scales.
+template <int D>
+struct NewToken {
+    uint32_t k[D / 8];
+    uint16_t v[D / 4];
+    __half ks[D / 32], vs[D / 32];
+    int key;  // its place in the group, -1: none
 };
 
 template <typename T, int D, int NT>
@@ -79,8 +88,11 @@ struct Shape {
     static constexpr int NQ = F32 ? 2 : 1;  // f16 terms of a query element
     static constexpr int NP = BF ? 1 : 2;   // f16 terms of a probability
     static constexpr int NB = D / 32;
-    // registers go to warps by fours: 12 warps of 168 a thread, 8 of 255 with two row tiles' accumulators
-    static constexpr int W = NT == 2 ? 7 : 11;
+    // Consumer warps, and the registers of a thread: what the four producer warps do not need goes to them (one CTA has
+    // the 65,536 of its SM).
+    static constexpr int W = NT == 2 ? 8 : 12;
+    static constexpr int CONSUMER_REGS = NT == 2 ? 208 : 152, PRODUCER_REGS = NT == 2 ? 88 : 56;
+    static_assert(W * 32 * CONSUMER_REGS + 128 * PRODUCER_REGS <= (NT == 2 ? 384 * 168 : 512 * 128), "what the CTA is launched with");
     static constexpr int STAGES = D == 64 ? 4 : 3;
     static constexpr int UNIT = kUnitGroups * KvQ4<D>::GROUP_BYTES;
     static constexpr int RING = W * STAGES * UNIT;
@@ -93,6 +105,7 @@ struct Shape {
         float2 to_log2[NT][32];
         int2 limit[NT][32];  // keys that the columns' rows see
         Item item;
+        NewToken<D> added;  // decode step: the token that the item's last unit gets
     };
     static constexpr int SMEM = RING + MERGE + 2 * (int)sizeof(Slot);
     static_assert(kMaxGrid * 8 * 4 <= MERGE, "the weights of an item's parts fit");
@@ -202,6 +215,7 @@ struct Cursor {
     }
     __device__ __forceinline__ long long request_places(const Attend &p) const {
         long long places = 0;
+#pragma unroll 1
         for (int t = 0; t < tiles; ++t) places += tile_units(p, t) + kItemCost;
         return places * p.c.kv_heads;
     }
@@ -214,6 +228,7 @@ struct Cursor {
         h = 0;
         if (++u >= tiles) {
             u = 0;
+#pragma unroll 1
             do {
                 if (++b >= p.c.requests) {
                     rel = INT32_MAX / 2;
@@ -247,17 +262,21 @@ __device__ __forceinline__ void rotate(const __nv_bfloat16 *rope, int t, float (
 }
 
 // One warp: the new token's key (rotated) and value of head h at position pos,
-// in 4 bits, into the group's copy in shared memory and into the cache.
+// in 4 bits, into the cache and into `added`, from where the warp that has its
+// unit puts it into its copy.
 template <int D>
-__device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos, uint8_t *buf) {
+__device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos, NewToken<D> &added) {
     using Q = KvQ4<D>;
     constexpr int NB = Q::NB, H = D / 64;
     const Attend &a = p.a;
-    if (pos >= p.rope_rows) {
-        record_device_error(a.c.err, DEV_ERR_BAD_PAGE);
-        return;
-    }
     const int lane = threadIdx.x & 31, t = lane & 3, block = (lane >> 2) % NB, is_v = (lane >> 2) / NB % 2;
+    uint8_t *group = nullptr;
+    if (pos >= p.rope_rows)
+        record_device_error(a.c.err, DEV_ERR_BAD_PAGE);
+    else if (pos >= 0)
+        group = a.c.group<D>(b, h, pos >> 4);
+    if (lane == 0) added.key = group ? pos & 15 : -1;
+    if (!group) return;
     const __nv_bfloat16 *row = p.qkv + ((int64_t)b * (a.heads + 2 * a.c.kv_heads) + a.heads + (is_v ? a.c.kv_heads : 0) + h) * D;
     float x[8];
     load8<__nv_bfloat16>(row + block * 32 + t * 8, x);
@@ -272,22 +291,32 @@ __device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos
     }
     const float d = __fdiv_rn(q4_0_extreme(x), -8.0f);
     const float inv = (d != 0.0f) ? __fdiv_rn(1.0f, d) : 0.0f;
-    uint8_t *group = a.c.group<D>(b, h, pos >> 4);
-    if (!group || lane >= 8 * NB) return;
+    if (lane >= 8 * NB) return;
     const int key = pos & 15;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        uint8_t *g = k ? group : buf;
-        if (is_v) {
-            const uint32_t w = q4_0_v_halves(x, inv);
-            *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t, block)) = (unsigned short)w;
-            *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t + 1, block)) = (unsigned short)(w >> 16);
-        } else {
-            *reinterpret_cast<uint32_t *>(g + Q::k_word(key, t, block)) = q4_0_k_word(x, inv);
-        }
-        if (t == 0)
-            *reinterpret_cast<__half *>(g + (is_v ? Q::v_scale(key, block) : Q::k_scale(key, block))) = __float2half_rn(d);
+    const __half d16 = __float2half_rn(d);
+    if (is_v) {
+        const uint32_t w = q4_0_v_halves(x, inv);
+        *reinterpret_cast<uint16_t *>(group + Q::v_half(key, 2 * t, block)) = added.v[block * 8 + 2 * t] = (uint16_t)w;
+        *reinterpret_cast<uint16_t *>(group + Q::v_half(key, 2 * t + 1, block)) = added.v[block * 8 + 2 * t + 1] = (uint16_t)(w >> 16);
+        if (t == 0) *reinterpret_cast<__half *>(group + Q::v_scale(key, block)) = added.vs[block] = d16;
+    } else {
+        *reinterpret_cast<uint32_t *>(group + Q::k_word(key, t, block)) = added.k[t * NB + block] = q4_0_k_word(x, inv);
+        if (t == 0) *reinterpret_cast<__half *>(group + Q::k_scale(key, block)) = added.ks[block] = d16;
     }
+}
+
+// One warp: the new token into its group's copy in shared memory.
+template <int D>
+__device__ __forceinline__ void patch_new(const NewToken<D> &added, uint8_t *buf) {
+    using Q = KvQ4<D>;
+    const int lane = threadIdx.x & 31, key = added.key;
+    if (lane < D / 8) *reinterpret_cast<uint32_t *>(buf + Q::K_CODES + key * (D / 2) + lane * 4) = added.k[lane];
+    if (lane < D / 4) *reinterpret_cast<uint16_t *>(buf + Q::v_half(key, lane & 7, lane >> 3)) = added.v[lane];
+    if (lane < D / 32) {
+        *reinterpret_cast<__half *>(buf + Q::k_scale(key, lane)) = added.ks[lane];
+        *reinterpret_cast<__half *>(buf + Q::v_scale(key, lane)) = added.vs[lane];
+    }
+    __syncwarp();
 }
 
 template <typename T>
@@ -351,11 +380,24 @@ __device__ __forceinline__ void bar_consumers(int threads) { asm volatile("bar.s
 
 // The producer's view of the line: the first place of CTA c.
 __device__ __forceinline__ long long line_start(int c, long long per, int rest) { return c * per + min(c, rest); }
-__device__ __forceinline__ int line_owner(long long place, long long total, int grid, long long per, int rest) {
-    int c = min(grid - 1, (int)((double)place / (double)total * grid));
-    while (c + 1 < grid && line_start(c + 1, per, rest) <= place) ++c;
-    while (line_start(c, per, rest) > place) --c;
-    return c;
+// The CTA that has `place`; a whole warp asks.
+__device__ __forceinline__ int line_owner(long long place, int grid, long long per, int rest) {
+    int before = 0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < grid; c0 += 32) {
+        const int c = c0 + (threadIdx.x & 31);
+        before += __popc(__ballot_sync(0xffffffffu, c < grid && line_start(c, per, rest) <= place));
+    }
+    return before - 1;
+}
+
+template <int REGS>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 // One warp: the item's queries as the first product's B fragments; lane (g, t)
@@ -439,7 +481,7 @@ __device__ __forceinline__ void prepare_queries(const Split &p, const Cursor<8 *
 }
 
 template <typename T, int D, int NT, bool STEP>
-__global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kernel(const Split p) {
+__global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kernel(const Split p) {
     using Q = KvQ4<D>;
     using H = Shape<T, D, NT>;
     constexpr int NB = Q::NB, RT = 8 * NT, W = H::W, STAGES = H::STAGES, THREADS = 32 * W;
@@ -458,7 +500,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
     const Attend &a = p.a;
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], W);
+            mbar_init(&full[s], 1);
             mbar_init(&empty[s], W);
         }
         for (int s = 0; s < 2; ++s) {
@@ -472,10 +514,12 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
     pdl_launch_dependents();
     pdl_wait();
 
-    if (warp == W) {
-        // ---- the producer: this CTA's part of the line
+    if (warp >= W) {
+        fewer_registers<H::PRODUCER_REGS>();
+        // ---- a producer: this CTA's part of the line
         Cursor<RT> at;
         long long total = 0, own = 0;
+#pragma unroll 1
         for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
             own = 0;
             at.b = b0 + lane;
@@ -497,6 +541,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
         if (cta < grid && total > 0) {
             len = (int)(line_start(cta + 1, per, rest) - lo);
             long long place = 0;  // of the current request, then tile
+#pragma unroll 1
             for (int b0 = 0;; b0 += 32) {
                 if (a.c.requests > 32) {
                     own = 0;
@@ -522,6 +567,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
                 place += __shfl_sync(0xffffffffu, upto, 31);
             }
             at.load_request(a);
+#pragma unroll 1
             for (at.u = 0;; ++at.u) {
                 at.G = at.tile_units(a, at.u);
                 const long long places = (long long)(at.G + kItemCost) * a.c.kv_heads;
@@ -529,136 +575,126 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
                 place += places;
             }
             at.h = 0;
+#pragma unroll 1
             while (place + at.G + kItemCost <= lo) place += at.G + kItemCost, ++at.h;
             at.rel = (int)(place + kItemCost - lo);
         } else {
             at.rel = 0;  // len is 0: nothing to do
         }
 
-        // lane w's next unit, of the units w, w + W, ..
-        Cursor<RT> mine = at;
-        const int *row = nullptr;
-        int g = 0;
-        bool have = lane < W && len > 0;
-        auto settle = [&]() {  // g may lie behind the item's units: go on to the item that has it
-            while (g >= mine.upto(len)) {
-                if (mine.rel >= len) {
-                    have = false;
-                    return;
-                }
-                g -= max(mine.from(), mine.upto(len));
-                mine.next_item(a);
-                g += mine.from();
-            }
-            row = a.c.table + mine.b * a.c.table_stride;
-        };
-        if (have) {
-            g = mine.from() + lane;
-            settle();
-        }
-        int i0 = 0, m = 0, k = 0;
-        bool broken = false;
-        for (; __any_sync(0xffffffffu, have) && !broken; ++k) {
-            const int s = k % STAGES;
-            if (k >= STAGES && !mbar_wait(&empty[s], (k / STAGES - 1) & 1)) broken = true;
-            if (__any_sync(0xffffffffu, broken)) {
-                broken = true;
-                break;
-            }
-            if (lane < W) {
-                uint8_t *dst = ring + (s * W + lane) * H::UNIT;
-                uint32_t gone = 3;
-                if (have) {
-                    // a unit's two groups lie together, unless pages hold one group
-                    const int group = g * kUnitGroups;
-                    if (a.c.page_shift > 4) {
-                        const uint8_t *src = nullptr;
-                        if (group * kKvGroup < mine.S) src = a.c.group_of_row<D>(row, mine.h, group);
-                        if (src) {
-                            gone = 0;
-                            gone_sm[s][lane] = 0;
-                            mbar_arrive_expect_tx(&full[s], H::UNIT);
-                            bulk_g2s(dst, src, H::UNIT, &full[s]);
-                        }
+        if (warp > W) {
+            // ---- copies, a third of the stages for each of three warps: lanes 2w and 2w + 1 find the two groups of warp w's units, every W-th of the CTA's; groups that
+            // lie together (a page's) come in one copy. (A copy's addresses are a warp's, not a lane's.)
+            static_assert(2 * W <= 32, "a lane for each group");
+            constexpr int WARPS = 3;
+            int k = warp - W - 1, g = at.from() + (lane >> 1) + k * W;
+            bool have = lane < 2 * W && len > 0, broken = false;
+#pragma unroll 1
+            for (;; k += WARPS) {
+#pragma unroll 1
+                while (have && g >= at.upto(len)) {  // g lies behind the item's units: on to the item that has it
+                    if (at.rel >= len) {
+                        have = false;
                     } else {
-                        const uint8_t *src[2] = {nullptr, nullptr};
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            if ((group + j) * kKvGroup < mine.S) src[j] = a.c.group_of_row<D>(row, mine.h, group + j);
-                            if (src[j]) gone &= ~(1u << j);
-                        }
-                        if (gone != 3) {
-                            gone_sm[s][lane] = (uint8_t)gone;
-                            mbar_arrive_expect_tx(&full[s], gone ? Q::GROUP_BYTES : 2 * Q::GROUP_BYTES);
-#pragma unroll
-                            for (int j = 0; j < 2; ++j)
-                                if (src[j]) bulk_g2s(dst + j * Q::GROUP_BYTES, src[j], Q::GROUP_BYTES, &full[s]);
-                        }
+                        g -= max(at.from(), at.upto(len));
+                        at.next_item(a);
+                        g += at.from();
                     }
                 }
-                if (gone == 3) {
-                    gone_sm[s][lane] = 3;
-                    mbar_arrive(&full[s]);
-                }
+                __syncwarp();
+                if (!__any_sync(0xffffffffu, have)) break;
+                const uint8_t *src = nullptr;
                 if (have) {
-                    g += W;
-                    settle();
+                    const int group = g * kUnitGroups + (lane & 1);
+                    if (group * kKvGroup < at.S) src = a.c.group_of_row<D>(a.c.table + at.b * a.c.table_stride, at.h, group);
+                    g += WARPS * W;
                 }
+                __syncwarp();
+                const unsigned there = __ballot_sync(0xffffffffu, src != nullptr);
+                const unsigned long long addr = reinterpret_cast<unsigned long long>(src);
+                const unsigned long long prev = __shfl_up_sync(0xffffffffu, addr, 1);
+                const bool follows = lane > 0 && src && (there >> (lane - 1) & 1) && prev + Q::GROUP_BYTES == addr;
+                const unsigned stops = __ballot_sync(0xffffffffu, !follows);
+                unsigned heads = there & stops;
+                const int run = __ffs((stops >> lane >> 1) | (1u << (31 - lane)));  // groups from here to the next stop
+                const int s = k % STAGES;
+                if (k >= STAGES && !mbar_wait(&empty[s], (k / STAGES - 1) & 1)) broken = true;
+                if (__any_sync(0xffffffffu, broken)) break;
+                if (lane < W) gone_sm[s][lane] = (uint8_t)(~there >> (2 * lane) & 3);
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(there) * Q::GROUP_BYTES);
+                uint8_t *dst = ring + s * W * H::UNIT;
+#pragma unroll 1
+                while (heads) {
+                    const int j = __ffs(heads) - 1;
+                    heads &= heads - 1;
+                    const uint8_t *from = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, addr, j));
+                    const int n = __shfl_sync(0xffffffffu, run, j);
+                    if (lane == 0) bulk_g2s(dst + j * Q::GROUP_BYTES, from, (uint32_t)(n * Q::GROUP_BYTES), &full[s]);
+                }
+            }
+            if (__any_sync(0xffffffffu, broken)) {
+                // this warp's last copies (a bounded wait) before the shared memory goes
+                if (lane == 0) record_device_error(a.c.err, DEV_ERR_WAIT_EMPTY);
+                if (k >= WARPS) mbar_wait(&full[(k - WARPS) % STAGES], ((k - WARPS) / STAGES) & 1);
+            }
+            return;
+        }
+
+        // ---- items: their queries, one item ahead of the consumers
+        int i0 = 0;
+        bool broken = false;
+#pragma unroll 1
+        for (int m = 0;; ++m) {
+#pragma unroll 1
+            while (at.rel < len && at.from() >= at.upto(len)) at.next_item(a);
+            typename H::Slot &slot = slots[m & 1];
+            if (m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
+            if (__any_sync(0xffffffffu, broken)) {
+                if (lane == 0) record_device_error(a.c.err, DEV_ERR_WAIT_EMPTY);
+                return;
+            }
+            const bool end = at.rel >= len;
+            if (!end) {
+                const int g0 = at.from(), g1 = at.upto(len), row0 = at.u * RT, rows = min(RT, at.n * a.rep - row0);
+                prepare_queries<T, D, NT, STEP>(p, at, rows, row0, slot);
+                Item it;
+                it.end = 0;
+                it.g0 = g0, it.g1 = g1, it.i0 = i0;
+                it.whole = g0 == 0 && g1 == at.G;
+                it.c0 = it.c1 = cta;
+                if (!it.whole) {
+                    it.c0 = line_owner(lo + at.rel, grid, per, rest);
+                    it.c1 = line_owner(lo + at.rel + at.G - 1, grid, per, rest);
+                }
+                it.h = at.h, it.S = at.S;
+                it.new_unit = -1;
+                if constexpr (STEP) {
+                    if (g1 == at.G) {
+                        append_new<D>(p, at.b, at.h, at.S - 1, slot.added);
+                        it.new_unit = at.G - 1;
+                    }
+                }
+                it.rows = rows, it.row0 = row0, it.first = at.first;
+                it.all_see = at.S - at.n + row0 / a.rep + 1;
+                if (lane == 0) slot.item = it;
+                i0 += g1 - g0;
+            } else if (lane == 0) {
+                slot.item.end = 1;
             }
             __syncwarp();
-            // the items that begin in this stage, once its copies are on their way: an item's slot comes free when the
-            // one before the last has begun, which may need this stage
-            while (at.rel < len && i0 < (k + 1) * W) {
-                const int g0 = at.from(), g1 = at.upto(len);
-                if (g0 < g1) {
-                    typename H::Slot &slot = slots[m & 1];
-                    if (m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
-                    if (__any_sync(0xffffffffu, broken)) {
-                        broken = true;
-                        break;
-                    }
-                    const int row0 = at.u * RT, rows = min(RT, at.n * a.rep - row0);
-                    prepare_queries<T, D, NT, STEP>(p, at, rows, row0, slot);
-                    if (lane == 0) {
-                        Item it;
-                        it.end = 0;
-                        it.g0 = g0, it.g1 = g1, it.i0 = i0;
-                        it.whole = g0 == 0 && g1 == at.G;
-                        it.c0 = it.c1 = cta;
-                        if (!it.whole) {
-                            it.c0 = line_owner(lo + at.rel, total, grid, per, rest);
-                            it.c1 = line_owner(lo + at.rel + at.G - 1, total, grid, per, rest);
-                        }
-                        it.b = at.b, it.h = at.h, it.S = at.S;
-                        it.rows = rows, it.row0 = row0, it.first = at.first;
-                        it.all_see = at.S - at.n + row0 / a.rep + 1;
-                        slot.item = it;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&q_full[m & 1]);
-                    i0 += g1 - g0;
-                    ++m;
-                }
-                at.next_item(a);
-            }
+            if (lane == 0) mbar_arrive(&q_full[m & 1]);
+            if (end) return;
+            at.next_item(a);
         }
-        if (!broken && m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
-        broken = __any_sync(0xffffffffu, broken);
-        if (broken) {
-            // copies still on their way (each wait bounded) before the shared memory goes
-            if (lane == 0) record_device_error(a.c.err, DEV_ERR_WAIT_EMPTY);
-            for (int j = max(0, k - STAGES); j < k; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1);
-        } else if (lane == 0) {
-            slots[m & 1].item.end = 1;
-            mbar_arrive(&q_full[m & 1]);
-        }
-        return;
     }
 
     // ---- a consumer
+    more_registers<H::CONSUMER_REGS>();
     const uint32_t f16_1024 = p.f16_1024, f16_64 = p.f16_64;
     int my_i = warp, my_k = 0;
     bool broken = false;
+#pragma unroll 1
     for (int m = 0;; ++m) {
         typename H::Slot &slot = slots[m & 1];
         if (warp == 0 && !mbar_wait(&q_full[m & 1], (m / 2) & 1)) {
@@ -684,8 +720,6 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
             *reinterpret_cast<float2 *>(to_log2[nt]) = slot.to_log2[nt][lane];
             *reinterpret_cast<int2 *>(limit[nt]) = slot.limit[nt][lane];
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_empty[m & 1]);
 
         float o[NT][NB][2][4], l[NT][2], off[NT][2];
         float high[NT][2];  // the row's reference + kSlack: scores above move it
@@ -704,7 +738,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
                     for (int i = 0; i < 4; ++i) o[nt][b][k][i] = 0.0f;
         }
 
-        // One unit, tokens token0 .. + 31; `mask` where a row may not see all of them, or a group is gone.
+        // One unit, tokens token0 .. + 31; `masked` where a row may not see all of them, or a group is gone.
         auto take = [&](const uint8_t *unit_buf, int token0, uint32_t gone, auto mask) {
             constexpr bool masked = decltype(mask)::value;
             float s[kUnitGroups][NT][4];
@@ -848,7 +882,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
 #pragma unroll
                             for (int b = 0; b < NB; ++b) {
                                 uint32_t v = mul_f16x2(pt, vs[k][b]);
-                                if (masked) {  // what a row does not see may hold anything
+                                if constexpr (masked) {  // what a row does not see may hold anything
                                     if (!(pt & 0x0000ffffu)) v &= 0xffff0000u;
                                     if (!(pt & 0xffff0000u)) v &= 0x0000ffffu;
                                 }
@@ -913,6 +947,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
             }
         };
 
+#pragma unroll 1
         for (; my_i < it.i0 + it.g1 - it.g0; my_i += W, ++my_k) {
             const int stage = my_k % STAGES, unit = it.g0 + my_i - it.i0;
             if (!broken && !mbar_wait(&full[stage], (my_k / STAGES) & 1)) {
@@ -924,12 +959,8 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
             if (!broken && gone != 3) {
                 uint8_t *buf = ring + (stage * W + warp) * H::UNIT;
                 if constexpr (STEP) {
-                    // the unit of the new token: its row goes into this copy and into the cache
-                    const int group = (it.S - 1) >> 4;
-                    if (group / kUnitGroups == unit && !(gone >> (group & 1) & 1)) {
-                        append_new<D>(p, it.b, it.h, it.S - 1, buf + (group & 1) * Q::GROUP_BYTES);
-                        __syncwarp();
-                    }
+                    if (unit == it.new_unit && slot.added.key >= 0)
+                        patch_new<D>(slot.added, buf + ((it.S - 1) >> 4 & 1) * Q::GROUP_BYTES);
                 }
                 if ((unit + 1) * kUnit > it.all_see || gone)
                     take(buf, unit * kUnit, gone, std::true_type{});
@@ -939,6 +970,9 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
             __syncwarp();  // every lane has read the stage before a copy comes into it
             if (lane == 0) mbar_arrive(&empty[stage]);
         }
+
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[m & 1]);
 
         // ---- the warps' results of the item, or of this CTA's part of it
         const int64_t own_slot = (int64_t)blockIdx.x * 2 + (it.g0 == 0);
@@ -963,24 +997,24 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
                         make_float4(o[nt][b][0][j], o[nt][b][0][j + 2], o[nt][b][1][j], o[nt][b][1][j + 2]);
             }
             bar_consumers(THREADS);
+#pragma unroll 1
             for (int idx = tid; idx < 8 * (D / 4); idx += THREADS) {
                 const int row = idx / (D / 4), d = idx % (D / 4) * 4;
                 float least = INFINITY;
 #pragma unroll
                 for (int w = 0; w < W; ++w) least = fminf(least, ml_sm[w][row][0]);
                 float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-                if (least < INFINITY) {
+                // (a warp without keys has off = inf: weight 0)
+                const float base = least < INFINITY ? least : 0.0f;
 #pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        if (ml_sm[w][row][0] == INFINITY) continue;
-                        const float f = exp2_approx(least - ml_sm[w][row][0]);
-                        const float4 x = *reinterpret_cast<const float4 *>(merge + (w * 8 + row) * H::ROW + d);
-                        v[0] = fmaf(f, x.x, v[0]);
-                        v[1] = fmaf(f, x.y, v[1]);
-                        v[2] = fmaf(f, x.z, v[2]);
-                        v[3] = fmaf(f, x.w, v[3]);
-                        sum = fmaf(f, ml_sm[w][row][1], sum);
-                    }
+                for (int w = 0; w < W; ++w) {
+                    const float f = exp2_approx(base - ml_sm[w][row][0]);
+                    const float4 x = *reinterpret_cast<const float4 *>(merge + (w * 8 + row) * H::ROW + d);
+                    v[0] = fmaf(f, x.x, v[0]);
+                    v[1] = fmaf(f, x.y, v[1]);
+                    v[2] = fmaf(f, x.z, v[2]);
+                    v[3] = fmaf(f, x.w, v[3]);
+                    sum = fmaf(f, ml_sm[w][row][1], sum);
                 }
                 const int rr = nt * 8 + row;
                 if (!it.whole) {
@@ -1014,6 +1048,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
             __syncwarp();
             __threadfence();
             bool all = true;
+#pragma unroll 1
             for (int c = c0 + lane; c <= c1; c += 32)
                 all &= *reinterpret_cast<const volatile unsigned long long *>(p.flags + part(c)) == p.nonce;
             all = __all_sync(0xffffffffu, all);
@@ -1050,6 +1085,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
                 }
             }
             bar_consumers(THREADS);
+#pragma unroll 1
             for (int idx = tid; idx < 8 * (D / 4); idx += THREADS) {
                 const int row = idx / (D / 4), d = idx % (D / 4) * 4, rr = nt * 8 + row;
                 if (rr >= it.rows) continue;
@@ -1076,6 +1112,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 1), 1) sdpa_q4_kern
             }
             bar_consumers(THREADS);
         }
+#pragma unroll 1
         for (int c = c0 + tid; c <= c1; c += THREADS) p.flags[part(c)] = 0;
     }
 }
@@ -1112,7 +1149,7 @@ int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op)
     st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D, NT>::SMEM), op,
                     "cudaFuncSetAttribute");
     if (st) return st;
-    return launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * (Shape<T, D, NT>::W + 1)), Shape<T, D, NT>::SMEM, stream, op, p);
+    return launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * (Shape<T, D, NT>::W + 4)), Shape<T, D, NT>::SMEM, stream, op, p);
 }
 
 template <typename T, int D>
