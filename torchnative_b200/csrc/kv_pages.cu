@@ -36,6 +36,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kMaxRequests = 8192;
+// Up to here the one CTA that keeps the pages writes the slots too; above, a second launch over the whole GPU does.
+constexpr int kSlotsInOne = 4096;
 
 enum : int { BAD_NONE = 0, BAD_POOL = 1, BAD_LENGTH = 2, BAD_TOKENS = 3, BAD_STACK = 4 };
 
@@ -52,6 +54,7 @@ struct Resize {
     int *positions;
     int max_tokens;
     int *query_start, *status;
+    int aligned;  // slots and positions may be written in 16-byte vectors
 };
 
 __device__ __forceinline__ int pages_of(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
@@ -67,6 +70,11 @@ __device__ __forceinline__ int find(const int *starts, int n, int x) {
             hi = mid;
     }
     return lo;
+}
+
+__device__ __forceinline__ int64_t slot_of(const Resize &p, int b, int position) {
+    const int page = p.table[b * p.table_stride + (position >> p.page_shift)];
+    return ((int64_t)page << p.page_shift) + (position & ((1 << p.page_shift) - 1));
 }
 
 // Latency bounds it: one launch, and inside it a chain of dependent loads
@@ -137,9 +145,11 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
     if (bad) {  // nothing changes; no token has a slot
         if (tid == 0 && *p.status == 0) *p.status = bad;
         for (int b = tid; b <= B; b += kThreads) p.query_start[b] = 0;
-        for (int r = tid; r < p.max_tokens; r += kThreads) {
-            p.slots[r] = -1;
-            p.positions[r] = -1;
+        if (p.max_tokens <= kSlotsInOne) {
+            for (int r = tid; r < p.max_tokens; r += kThreads) {
+                p.slots[r] = -1;
+                p.positions[r] = -1;
+            }
         }
         return;
     }
@@ -173,18 +183,55 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
         const int b = find(take_at, B, i);
         p.table[b * p.table_stride + pages_of(old_len[b], p.page_shift) + (i - take_at[b])] = p.free_pages[top - 1 - i];
     }
+    if (p.max_tokens > kSlotsInOne) return;
+    __syncthreads();
     for (int r = tid; r < p.max_tokens; r += kThreads) {
         int64_t slot = -1;
         int position = -1;
         if (r < (int)tokens) {
             const int b = find(tok_at, B, r);
             position = old_len[b] + r - tok_at[b];
-            const int j = position >> p.page_shift, have = pages_of(old_len[b], p.page_shift);
-            const int page = j < have ? p.table[b * p.table_stride + j] : p.free_pages[top - 1 - (take_at[b] + j - have)];
-            slot = ((int64_t)page << p.page_shift) + (position & ((1 << p.page_shift) - 1));
+            slot = slot_of(p, b, position);
         }
         p.slots[r] = slot;
         p.positions[r] = position;
+    }
+}
+
+// The slots and positions of many new tokens, from the tables and lengths that
+// the launch before left; four neighbouring tokens a thread.
+__global__ void __launch_bounds__(256) kv_pages_slots_kernel(const Resize p) {
+    extern __shared__ int sm[];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int B = p.requests;
+    for (int b = threadIdx.x; b <= B; b += 256) sm[b] = p.query_start[b];
+    __syncthreads();
+    const int r0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (r0 >= p.max_tokens) return;
+    const int tokens = sm[B];
+    int b = r0 < tokens ? find(sm, B, r0) : 0;
+    int64_t slots[4];
+    int positions[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        slots[i] = -1;
+        positions[i] = -1;
+        if (r0 + i < tokens) {
+            while (sm[b + 1] <= r0 + i) ++b;
+            positions[i] = p.lengths[b] - (sm[b + 1] - (r0 + i));
+            slots[i] = slot_of(p, b, positions[i]);
+        }
+    }
+    if (r0 + 4 <= p.max_tokens && p.aligned) {
+        *reinterpret_cast<longlong2 *>(p.slots + r0) = make_longlong2(slots[0], slots[1]);
+        *reinterpret_cast<longlong2 *>(p.slots + r0 + 2) = make_longlong2(slots[2], slots[3]);
+        *reinterpret_cast<int4 *>(p.positions + r0) = make_int4(positions[0], positions[1], positions[2], positions[3]);
+    } else {
+        for (int i = 0; i < 4 && r0 + i < p.max_tokens; ++i) {
+            p.slots[r0 + i] = slots[i];
+            p.positions[r0 + i] = positions[i];
+        }
     }
 }
 
@@ -219,7 +266,8 @@ extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t
     if (new_lengths && new_lengths == lengths)
         return tn::set_error(TN_ERR_INVALID, op + ": new_lengths must not be lengths");
     tn::Resize p{page_table, table_stride, (int)max_pages, lengths, new_lengths, (int)grow, (int)requests, free_pages,
-                 free_count, (int)num_pages, shift, slots, positions, (int)max_tokens, query_start, status};
+                 free_count, (int)num_pages, shift, slots, positions, (int)max_tokens, query_start, status,
+                 ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0};
     const int smem = (int)(5 * requests * sizeof(int));
     if (smem > 48 * 1024 - 1024) {
         int st = tn::check_cuda(
@@ -227,6 +275,9 @@ extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t
             "tn_kv_pages_resize", "cudaFuncSetAttribute");
         if (st) return st;
     }
-    return tn::launch_pdl(tn::kv_pages_resize_kernel, dim3(1), dim3(tn::kThreads), smem, tn::stream_of(stream),
-                          "tn_kv_pages_resize", p);
+    cudaStream_t s = tn::stream_of(stream);
+    int st = tn::launch_pdl(tn::kv_pages_resize_kernel, dim3(1), dim3(tn::kThreads), smem, s, "tn_kv_pages_resize", p);
+    if (st || max_tokens <= tn::kSlotsInOne) return st;
+    return tn::launch_pdl(tn::kv_pages_slots_kernel, dim3((unsigned)((max_tokens + 1023) / 1024)), dim3(256),
+                          (int)((requests + 1) * sizeof(int)), s, "tn_kv_pages_resize", p);
 }

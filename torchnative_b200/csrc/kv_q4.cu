@@ -22,54 +22,62 @@ struct Append {
     int *err;
 };
 
-// Work item: one block of one row, four lanes. Items run over blocks, then K
-// and V, then heads, then tokens.
+// One warp: 256 / D neighbouring tokens of one head, keys and values; a lane has
+// eight elements of a row. HBM bounds it: 2 D elements read and 9 D / 8 bytes
+// written a token and head.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv_q4_append_kernel(const Append p) {
     using Q = KvQ4<D>;
+    constexpr int ROW_LANES = D / 8, TOKENS = 32 / ROW_LANES;
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t item = (blockIdx.x * (int64_t)kThreads + threadIdx.x) >> 2;
-    const int t = threadIdx.x & 3;
-    const int block = (int)(item % Q::NB);
-    const int is_v = (int)(item / Q::NB % 2);
-    const int64_t row = item / (2 * Q::NB);
-    const int head = (int)(row % p.kv_heads);
-    const int64_t token = row / p.kv_heads;
+    const int lane = threadIdx.x & 31, t = lane & 3, block = lane % ROW_LANES >> 2, head = blockIdx.y;
+    const int64_t token = (blockIdx.x * (int64_t)(kThreads / 32) + (threadIdx.x >> 5)) * TOKENS + lane / ROW_LANES;
     const bool live = token < p.tokens;
-    int64_t slot = live ? p.slots[token] : -1;
+    float k[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.0f;
+    int64_t slot = -1;
+    if (live) {
+        slot = p.slots[token];
+        const int64_t e = block * 32 + t * 8;
+        load8<T>(static_cast<const T *>(p.k) + token * p.k_token + head * p.k_head + e, k);
+        load8<T>(static_cast<const T *>(p.v) + token * p.v_token + head * p.v_head + e, v);
+    }
+    const float kd = __fdiv_rn(q4_0_extreme(k), -8.0f), vd = __fdiv_rn(q4_0_extreme(v), -8.0f);
+    const uint32_t kw = q4_0_k_word(k, kd != 0.0f ? __fdiv_rn(1.0f, kd) : 0.0f);
+    const uint32_t vw = q4_0_v_halves(v, vd != 0.0f ? __fdiv_rn(1.0f, vd) : 0.0f);
+    // an even token whose odd neighbour's row is in the other half of the lanes: their 16-bit pieces as words
+    const uint32_t vw2 = __shfl_xor_sync(0xffffffffu, vw, ROW_LANES);
+    const int64_t slot2 = __shfl_xor_sync(0xffffffffu, slot, ROW_LANES);
     if (slot >= p.num_slots) {  // never followed
         record_device_error(p.err, DEV_ERR_BAD_PAGE);
-        slot = -1;
+        return;
     }
-    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (slot >= 0) {
-        const T *src = is_v ? static_cast<const T *>(p.v) + token * p.v_token + head * p.v_head
-                            : static_cast<const T *>(p.k) + token * p.k_token + head * p.k_head;
-        load8<T>(src + block * 32 + t * 8, x);
-    }
-    const float d = __fdiv_rn(q4_0_extreme(x), -8.0f);
-    const float inv = (d != 0.0f) ? __fdiv_rn(1.0f, d) : 0.0f;
     if (slot < 0) return;
     const int64_t page = slot >> p.page_shift;
     const int in_page = (int)(slot & ((1 << p.page_shift) - 1)), key = in_page & 15;
     uint8_t *g = p.pool + (((page * p.kv_heads + head) << (p.page_shift - 4)) + (in_page >> 4)) * Q::GROUP_BYTES;
-    if (is_v) {
-        const uint32_t w = q4_0_v_halves(x, inv);
-        *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t, block)) = (unsigned short)w;
-        *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t + 1, block)) = (unsigned short)(w >> 16);
+    *reinterpret_cast<uint32_t *>(g + Q::k_word(key, t, block)) = kw;
+    if ((slot ^ 1) == slot2) {
+        const int odd = key & 1;
+        const uint32_t word = odd ? (vw2 >> 16) | (vw & 0xffff0000u) : (vw & 0xffffu) | (vw2 << 16);
+        *reinterpret_cast<uint32_t *>(g + Q::v_half(key & ~1, 2 * t + odd, block)) = word;
     } else {
-        *reinterpret_cast<uint32_t *>(g + Q::k_word(key, t, block)) = q4_0_k_word(x, inv);
+        *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t, block)) = (unsigned short)vw;
+        *reinterpret_cast<unsigned short *>(g + Q::v_half(key, 2 * t + 1, block)) = (unsigned short)(vw >> 16);
     }
-    if (t == 0)
-        *reinterpret_cast<__half *>(g + (is_v ? Q::v_scale(key, block) : Q::k_scale(key, block))) = __float2half_rn(d);
+    if (t == 0) {
+        *reinterpret_cast<__half *>(g + Q::k_scale(key, block)) = __float2half_rn(kd);
+        *reinterpret_cast<__half *>(g + Q::v_scale(key, block)) = __float2half_rn(vd);
+    }
 }
 
 template <typename T, int D>
 int launch_append(const Append &p, cudaStream_t stream) {
-    const int64_t threads = p.tokens * p.kv_heads * 2 * KvQ4<D>::NB * 4;
-    return launch_pdl(kv_q4_append_kernel<T, D>, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads),
-                      0, stream, "tn_kv_q4_append", p);
+    constexpr int tokens = kThreads / 32 * (256 / D);  // of a CTA
+    return launch_pdl(kv_q4_append_kernel<T, D>, dim3((unsigned)((p.tokens + tokens - 1) / tokens), (unsigned)p.kv_heads),
+                      dim3(kThreads), 0, stream, "tn_kv_q4_append", p);
 }
 
 bool aligned(const void *p, int64_t token, int64_t head, int64_t size) {

@@ -60,6 +60,8 @@ constexpr int kUnitGroups = 2, kUnit = kUnitGroups * kKvGroup;
 constexpr float kBias = 10.0f, kSlack = 5.0f;
 // What an item costs besides its units (queries, the warps' results joined), in units.
 constexpr int kItemCost = 12;
+// A CTA has 2^kMinPlaces places of the line before another one is used.
+constexpr int kMinPlaces = 4;
 
 // What the producer tells the consumers of an item.
 struct Item {
@@ -69,6 +71,7 @@ struct Item {
     int whole, c0, c1;   // all of its units; otherwise the CTAs that have some
     int h, S;
     int new_unit;        // decode step: the unit of the new token, -1 where this CTA has it not
+    int single;          // the request has one query token
     int rows, row0;      // query rows of the tile, of the request before it
     int first, all_see;  // the request's first packed token; keys that every row of the tile sees
 };
@@ -108,13 +111,12 @@ struct Shape {
         NewToken<D> added;  // decode step: the token that the item's last unit gets
     };
     static constexpr int SMEM = RING + MERGE + 2 * (int)sizeof(Slot);
-    static_assert(kMaxGrid * 8 * 4 <= MERGE, "the weights of an item's parts fit");
+    static_assert(kMaxGrid * 8 * 8 <= MERGE, "the weights of an item's parts fit");
     static_assert(SMEM <= 226 * 1024, "shared memory of one SM");
 };
 
 struct Split {
     Attend a;
-    int min_places;       // of the line that a CTA should have before another one is used
     float *part_o;        // [kMaxGrid][2][8 NT][D]
     float *part_ml;       // [kMaxGrid][2][8 NT][2]
     unsigned long long *flags;  // [kMaxGrid][2]
@@ -210,7 +212,7 @@ struct Cursor {
     }
     // units that the tile's last row sees; 1 where it sees none, so that someone writes its zeros
     __device__ __forceinline__ int tile_units(const Attend &p, int tile) const {
-        const int last = min(n - 1, (tile * RT + RT - 1) / p.rep);
+        const int last = n == 1 ? 0 : min(n - 1, (tile * RT + RT - 1) / p.rep);
         return max(1, (S - n + last + kUnit) / kUnit);
     }
     __device__ __forceinline__ long long request_places(const Attend &p) const {
@@ -400,38 +402,50 @@ __device__ __forceinline__ void fewer_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
-// One warp: the item's queries as the first product's B fragments; lane (g, t)
-// holds row g, elements 32 b + 8 t .. + 7.
+// One warp: the item's queries; lane (g, t) holds row g, elements 32 b + 8 t ..
+// + 7 of each block.
 template <typename T, int D, int NT, bool STEP>
-__device__ __forceinline__ void prepare_queries(const Split &p, const Cursor<8 * NT> &at, int rows, int row0,
-                                                typename Shape<T, D, NT>::Slot &slot) {
-    using H = Shape<T, D, NT>;
-    constexpr int NB = H::NB;
+__device__ __forceinline__ void load_queries(const Split &p, const Cursor<8 * NT> &at, float (&x)[NT][D / 32][8]) {
     const Attend &a = p.a;
-    const int lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
+    const int lane = threadIdx.x & 31, lt = lane & 3, row0 = at.u * 8 * NT;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int row = nt * 8 + lg;
-        float x[NB][8];
-        const bool live = row < rows;
-        const int tok = (row0 + row) / a.rep, hq = at.h * a.rep + (row0 + row) % a.rep;
+        const int row = row0 + nt * 8 + (lane >> 2);
+        const int tok = at.n == 1 ? 0 : row / a.rep, hq = at.h * a.rep + row - tok * a.rep;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
-        if (live) {
+            for (int i = 0; i < 8; ++i) x[nt][b][i] = 0.0f;
+        if (row < at.n * a.rep) {
             const T *src;
             if constexpr (STEP)
                 src = reinterpret_cast<const T *>(p.qkv) + ((int64_t)at.b * (a.heads + 2 * a.c.kv_heads) + hq) * D;
             else
                 src = static_cast<const T *>(a.q) + (at.first + tok) * a.q_token + hq * a.q_head;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) load8<T>(src + b * 32 + lt * 8, x[b]);
+            for (int b = 0; b < D / 32; ++b) load8<T>(src + b * 32 + lt * 8, x[nt][b]);
         }
         if constexpr (STEP) {
             const int64_t pos = max((int64_t)0, min((int64_t)at.S - 1, p.rope_rows - 1));
-            rotate<D>(p.rope + pos * D, lt, x);
+            rotate<D>(p.rope + pos * D, lt, x[nt]);
         }
+    }
+}
+
+// The same warp: into the slot, as the first product's B fragments.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void put_queries(const Split &p, const Cursor<8 * NT> &at, const float (&q)[NT][D / 32][8],
+                                            typename Shape<T, D, NT>::Slot &slot) {
+    using H = Shape<T, D, NT>;
+    constexpr int NB = H::NB;
+    const Attend &a = p.a;
+    const int lane = threadIdx.x & 31, lt = lane & 3, row0 = at.u * 8 * NT;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = row0 + nt * 8 + (lane >> 2);
+        const bool live = row < at.n * a.rep;
+        const int tok = at.n == 1 ? 0 : row / a.rep;
+        const float(&x)[NB][8] = q[nt];
         // the row's largest magnitude goes to [2^13, 2^14): no element overflows f16, and one that loses bits there
         // lies 2^27 below it
         float scale = 1.0f, back = 1.0f;
@@ -487,8 +501,9 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
     constexpr int NB = Q::NB, RT = 8 * NT, W = H::W, STAGES = H::STAGES, THREADS = 32 * W;
     constexpr bool F32 = H::F32, BF = H::BF;
     constexpr int NQ = H::NQ, NP = H::NP;
+    constexpr int COPY_WARPS = STEP ? 2 : 3;  // a decode step has a warp for the new tokens
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full[2], q_empty[2];
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full[2], q_empty[2], new_full[2];
     __shared__ uint8_t gone_sm[STAGES][W];  // per unit, a bit for each group without a page
     __shared__ float ml_sm[W][8][2], sum_sm[8][2];
     __shared__ int is_last, stop;
@@ -505,6 +520,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&q_full[s], 1);
+            mbar_init(&new_full[s], 1);
             mbar_init(&q_empty[s], W);
         }
         stop = 0;
@@ -532,10 +548,10 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
             for (int off = 16; off; off >>= 1) w += __shfl_xor_sync(0xffffffffu, w, off);
             total += w;
         }
-        const int grid = (int)min((long long)gridDim.x, max(1ll, total / p.min_places));
+        const int grid = (int)min((long long)gridDim.x, max(1ll, total >> kMinPlaces));
         const int cta = blockIdx.x;
         int len = 0;
-        const long long per = total / grid;
+        const long long per = total >> 31 ? total / grid : (unsigned)total / (unsigned)grid;
         const int rest = (int)(total - per * grid);
         const long long lo = line_start(cta, per, rest);
         if (cta < grid && total > 0) {
@@ -582,11 +598,29 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
             at.rel = 0;  // len is 0: nothing to do
         }
 
+        if (STEP && warp == W + 3) {
+            // ---- new tokens, one item ahead of the consumers like their queries
+#pragma unroll 1
+            for (int m = 0;; ++m) {
+#pragma unroll 1
+                while (at.rel < len && at.from() >= at.upto(len)) at.next_item(a);
+                if (at.rel >= len) return;
+                const bool ok = m < 2 || mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1);
+                if (__any_sync(0xffffffffu, !ok)) {
+                    if (lane == 0) record_device_error(a.c.err, DEV_ERR_WAIT_EMPTY);
+                    return;
+                }
+                if (at.upto(len) == at.G) append_new<D>(p, at.b, at.h, at.S - 1, slots[m & 1].added);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&new_full[m & 1]);
+                at.next_item(a);
+            }
+        }
         if (warp > W) {
-            // ---- copies, a third of the stages for each of three warps: lanes 2w and 2w + 1 find the two groups of warp w's units, every W-th of the CTA's; groups that
+            // ---- copies, the stages in turn to two or three warps: lanes 2w and 2w + 1 find the two groups of warp w's units, every W-th of the CTA's; groups that
             // lie together (a page's) come in one copy. (A copy's addresses are a warp's, not a lane's.)
             static_assert(2 * W <= 32, "a lane for each group");
-            constexpr int WARPS = 3;
+            constexpr int WARPS = COPY_WARPS;
             int k = warp - W - 1, g = at.from() + (lane >> 1) + k * W;
             bool have = lane < 2 * W && len > 0, broken = false;
 #pragma unroll 1
@@ -649,15 +683,17 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
 #pragma unroll 1
             while (at.rel < len && at.from() >= at.upto(len)) at.next_item(a);
             typename H::Slot &slot = slots[m & 1];
+            const bool end = at.rel >= len;
             if (m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
             if (__any_sync(0xffffffffu, broken)) {
                 if (lane == 0) record_device_error(a.c.err, DEV_ERR_WAIT_EMPTY);
                 return;
             }
-            const bool end = at.rel >= len;
             if (!end) {
                 const int g0 = at.from(), g1 = at.upto(len), row0 = at.u * RT, rows = min(RT, at.n * a.rep - row0);
-                prepare_queries<T, D, NT, STEP>(p, at, rows, row0, slot);
+                float q[NT][NB][8];
+                load_queries<T, D, NT, STEP>(p, at, q);
+                put_queries<T, D, NT>(p, at, q, slot);
                 Item it;
                 it.end = 0;
                 it.g0 = g0, it.g1 = g1, it.i0 = i0;
@@ -668,15 +704,10 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                     it.c1 = line_owner(lo + at.rel + at.G - 1, grid, per, rest);
                 }
                 it.h = at.h, it.S = at.S;
-                it.new_unit = -1;
-                if constexpr (STEP) {
-                    if (g1 == at.G) {
-                        append_new<D>(p, at.b, at.h, at.S - 1, slot.added);
-                        it.new_unit = at.G - 1;
-                    }
-                }
+                it.single = at.n == 1;
+                it.new_unit = STEP && g1 == at.G ? at.G - 1 : -1;
                 it.rows = rows, it.row0 = row0, it.first = at.first;
-                it.all_see = at.S - at.n + row0 / a.rep + 1;
+                it.all_see = at.S - at.n + (at.n == 1 ? 0 : row0 / a.rep) + 1;
                 if (lane == 0) slot.item = it;
                 i0 += g1 - g0;
             } else if (lane == 0) {
@@ -959,8 +990,12 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
             if (!broken && gone != 3) {
                 uint8_t *buf = ring + (stage * W + warp) * H::UNIT;
                 if constexpr (STEP) {
-                    if (unit == it.new_unit && slot.added.key >= 0)
-                        patch_new<D>(slot.added, buf + ((it.S - 1) >> 4 & 1) * Q::GROUP_BYTES);
+                    if (unit == it.new_unit) {
+                        if (!mbar_wait(&new_full[m & 1], (m / 2) & 1))
+                            record_device_error(a.c.err, DEV_ERR_WAIT_FULL);
+                        else if (slot.added.key >= 0)
+                            patch_new<D>(slot.added, buf + ((it.S - 1) >> 4 & 1) * Q::GROUP_BYTES);
+                    }
                 }
                 if ((unit + 1) * kUnit > it.all_see || gone)
                     take(buf, unit * kUnit, gone, std::true_type{});
@@ -975,6 +1010,17 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
         if (lane == 0) mbar_arrive(&q_empty[m & 1]);
 
         // ---- the warps' results of the item, or of this CTA's part of it
+        // four finished sums of row rr, of weight `sum` against the reference `least`
+        auto finish = [&](int rr, int d, float (&v)[4], float sum, float least) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= inv;
+            const int tok = it.single ? 0 : (it.row0 + rr) / a.rep;
+            const int r = it.first + tok, hq = it.h * a.rep + it.row0 + rr - tok * a.rep;
+            finish4<T, D, STEP>(p, r, hq, d, v);
+            if (d == 0 && a.lse)
+                a.lse[(int64_t)r * a.heads + hq] = sum == 0.0f ? 0.0f : (log2f(sum) - least) * 0.6931471805599453f;
+        };
         const int64_t own_slot = (int64_t)blockIdx.x * 2 + (it.g0 == 0);
         float *po = p.part_o + own_slot * RT * D;
         float *pml = p.part_ml + own_slot * RT * 2;
@@ -1021,13 +1067,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                     __stcg(reinterpret_cast<float4 *>(po + rr * D + d), make_float4(v[0], v[1], v[2], v[3]));
                     if (d == 0) __stcg(reinterpret_cast<float2 *>(pml + rr * 2), make_float2(least, sum));
                 } else if (rr < it.rows) {
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= inv;
-                    const int r = it.first + (it.row0 + rr) / a.rep, hq = it.h * a.rep + (it.row0 + rr) % a.rep;
-                    finish4<T, D, STEP>(p, r, hq, d, v);
-                    if (d == 0 && a.lse)
-                        a.lse[(int64_t)r * a.heads + hq] = sum == 0.0f ? 0.0f : (log2f(sum) - least) * 0.6931471805599453f;
+                    finish(rr, d, v, sum, least);
                 }
             }
         }
@@ -1038,7 +1078,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
         // parts in order. A flag is this launch's number, so that what lay in the workspace does not matter, and goes
         // back to 0, so that a replay of the launch finds none set.
         const int c0 = it.c0, c1 = it.c1;
-        auto part = [&](int c) { return (int64_t)c * 2 + (c == c0); };
+        auto part = [&](int c) { return 2 * c + (c == c0); };
         bar_consumers(THREADS);
         if (warp == 0) {
             if (lane == 0) {
@@ -1058,30 +1098,34 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
         bar_consumers(THREADS);
         if (!is_last) continue;
         // eight rows at a time: 16 lanes a row find the parts' common reference and weights, then a thread adds up four
-        // dimensions of a row, eight parts in flight
+        // dimensions of a row, four parts in flight
         const int parts = c1 - c0 + 1;
 #pragma unroll 1
         for (int nt = 0; nt < NT; ++nt) {
-            const int wr = tid >> 4, wl = tid & 15;
-            if (wr < 8) {
+            const float *ml = p.part_ml + nt * 16, *po = p.part_o + nt * 8 * D;
+            if (tid < 128) {
+                const int row = tid >> 4;
                 float least = INFINITY, sum = 0.0f;
-#pragma unroll 4
-                for (int c = c0 + wl; c <= c1; c += 16)
-                    least = fminf(least, __ldcg(p.part_ml + (part(c) * RT + nt * 8 + wr) * 2));
+#pragma unroll 1
+                for (int c = tid & 15; c < parts; c += 16) {
+                    const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + (part(c0 + c) * RT + row) * 2));
+                    *reinterpret_cast<float2 *>(merge + (row * parts + c) * 2) = x;
+                    least = fminf(least, x.x);
+                }
 #pragma unroll
                 for (int o2 = 8; o2; o2 >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o2));
-#pragma unroll 4
-                for (int c = c0 + wl; c <= c1; c += 16) {
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + (part(c) * RT + nt * 8 + wr) * 2));
-                    const float f = ml.x == INFINITY ? 0.0f : exp2_approx(least - ml.x);
-                    merge[wr * parts + c - c0] = f;
-                    sum = fmaf(f, ml.y, sum);
+                const float base = least < INFINITY ? least : 0.0f;
+#pragma unroll 1
+                for (int c = tid & 15; c < parts; c += 16) {
+                    float *x = merge + (row * parts + c) * 2;
+                    x[0] = exp2_approx(base - x[0]);
+                    sum = fmaf(x[0], x[1], sum);
                 }
 #pragma unroll
                 for (int o2 = 8; o2; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
-                if (wl == 0) {
-                    sum_sm[wr][0] = least;
-                    sum_sm[wr][1] = sum;
+                if ((tid & 15) == 0) {
+                    sum_sm[row][0] = least;
+                    sum_sm[row][1] = sum;
                 }
             }
             bar_consumers(THREADS);
@@ -1090,25 +1134,17 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                 const int row = idx / (D / 4), d = idx % (D / 4) * 4, rr = nt * 8 + row;
                 if (rr >= it.rows) continue;
                 float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                const float *w = merge + row * parts;
-                const float *src = p.part_o + rr * D + d;
-#pragma unroll 8
+                const float *w = merge + row * parts * 2;
+#pragma unroll 4
                 for (int c = 0; c < parts; ++c) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + part(c0 + c) * (RT * D)));
-                    const float f = w[c];
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(po + (part(c0 + c) * RT + row) * D + d));
+                    const float f = w[2 * c];
                     v[0] = fmaf(f, x.x, v[0]);
                     v[1] = fmaf(f, x.y, v[1]);
                     v[2] = fmaf(f, x.z, v[2]);
                     v[3] = fmaf(f, x.w, v[3]);
                 }
-                const float all_l = sum_sm[row][1], inv = all_l == 0.0f ? 0.0f : 1.0f / all_l;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= inv;
-                const int r = it.first + (it.row0 + rr) / a.rep, hq = it.h * a.rep + (it.row0 + rr) % a.rep;
-                finish4<T, D, STEP>(p, r, hq, d, v);
-                if (d == 0 && a.lse)
-                    a.lse[(int64_t)r * a.heads + hq] =
-                        all_l == 0.0f ? 0.0f : (log2f(all_l) - sum_sm[row][0]) * 0.6931471805599453f;
+                finish(rr, d, v, sum_sm[row][1], sum_sm[row][0]);
             }
             bar_consumers(THREADS);
         }
@@ -1146,9 +1182,15 @@ int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op)
     p.f16_1024 = 0x64006400u;
     p.f16_64 = 0x54005400u;
     auto kernel = sdpa_q4_kernel<T, D, NT, STEP>;
-    st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D, NT>::SMEM), op,
-                    "cudaFuncSetAttribute");
-    if (st) return st;
+    static std::atomic<uint64_t> ready{0};  // a bit a device
+    int device = 0;
+    if ((st = check_cuda(cudaGetDevice(&device), op, "cudaGetDevice"))) return st;
+    if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
+        st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, D, NT>::SMEM), op,
+                        "cudaFuncSetAttribute");
+        if (st) return st;
+        ready.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * (Shape<T, D, NT>::W + 4)), Shape<T, D, NT>::SMEM, stream, op, p);
 }
 
@@ -1211,7 +1253,6 @@ extern "C" int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strid
         return tn::set_error(TN_ERR_INVALID, std::string(op) + ": the workspace must be 16-byte aligned");
     tn::Split p{};
     p.a = {q, q_strides[0], q_strides[1], c, query_start, out, lse, (int)tokens, (int)heads, (int)(heads / kv_heads), sc};
-    p.min_places = 24;
     __atomic_fetch_add(&tn::counters().sdpa_calls, 1ull, __ATOMIC_RELAXED);
     __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     cudaStream_t s = tn::stream_of(stream);
@@ -1256,7 +1297,6 @@ extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t
     __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     tn::Split p{};
     p.a = {nullptr, 0, 0, c, nullptr, out, lse, (int)requests, (int)heads, (int)(heads / kv_heads), sc};
-    p.min_places = 24;
     p.qkv = (const __nv_bfloat16 *)qkv;
     p.rope = (const __nv_bfloat16 *)rope;
     p.rope_rows = rope_rows;

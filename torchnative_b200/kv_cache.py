@@ -26,21 +26,23 @@ import torch
 from . import _native as N
 
 GROUP = 16  # tokens of one head that lie together
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_TwoStrides = ctypes.c_int64 * 2
 _CODE = {torch.float32: N.TN_F32, torch.bfloat16: N.TN_BF16, torch.float16: N.TN_F16}
 _STATUS = {1: "not enough free pages", 2: "a request's length is outside [0, max_pages * page_size]",
            3: "more new tokens than max_tokens", 4: "more free pages than the pool has"}
 
 
-def _require(op: str, device: torch.device, **tensors) -> None:
-    """Every (tensor, dtype) on `device`, contiguous, of its dtype."""
-    for name, (t, dtype) in tensors.items():
-        if t.dtype != dtype:
-            raise NotImplementedError(f"{op}: {name} must be {dtype}, got {t.dtype}")
-        if t.device != device:
-            raise RuntimeError(f"{op}: Expected all tensors to be on the same device, but found at least two devices, "
-                               f"{device} and {t.device} ({name})")
-        if not t.is_contiguous():
-            raise RuntimeError(f"{op}: {name} must be contiguous")
+def _require(op: str, device: torch.device, name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
+    """t on `device`, contiguous, of its dtype."""
+    if t.dtype is not dtype:
+        raise NotImplementedError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{op}: Expected all tensors to be on the same device, but found at least two devices, "
+                           f"{device} and {t.device} ({name})")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{op}: {name} must be contiguous")
 
 
 def _require_cuda(op: str, device: torch.device) -> None:
@@ -52,12 +54,31 @@ def _require_cuda(op: str, device: torch.device) -> None:
 def _call(device: torch.device, fn, *args) -> None:
     """One library call on the device's current stream; the library takes the
     current device, which may be another one."""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch._C._cuda_getDevice():
-        N.check(fn(*args, stream))
+    index = device.index
+    if index == _current_device():
+        status = fn(*args, _current_stream(index))
     else:
-        with torch.cuda.device(device):
-            N.check(fn(*args, stream))
+        with torch.cuda.device(index):
+            status = fn(*args, _current_stream(index))
+    if status:
+        N.check(status)
+
+
+_scratch: dict = {}
+
+
+def _workspace(device: torch.device, tokens: int, heads: int, kv_heads: int, dim: int, most: int) -> torch.Tensor:
+    """The attention calls' scratch: one a stream, since calls on a stream run
+    one after the other; a captured call gets memory of its graph's own, since
+    graphs captured on one stream may be replayed on several."""
+    key = (device.index, _current_stream(device.index), heads // kv_heads * most > 8, dim)
+    ws = _scratch.get(key)
+    if ws is None or torch._C._cuda_isCurrentStreamCapturing():
+        ws = torch.empty(N.lib().tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, dim, most), dtype=torch.uint8,
+                         device=device)
+        if not torch._C._cuda_isCurrentStreamCapturing():
+            _scratch[key] = ws
+    return ws
 
 
 def _table_shape(op: str, page_table: torch.Tensor, lengths: torch.Tensor):
@@ -98,8 +119,11 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     device = page_table.device
     i32 = torch.int32
     _require_cuda(op, device)
-    _require(op, device, page_table=(page_table, i32), lengths=(lengths, i32), free_pages=(free_pages, i32),
-             free_count=(free_count, i32), status=(status, i32))
+    _require(op, device, "page_table", page_table, i32)
+    _require(op, device, "lengths", lengths, i32)
+    _require(op, device, "free_pages", free_pages, i32)
+    _require(op, device, "free_count", free_count, i32)
+    _require(op, device, "status", status, i32)
     requests, max_pages = _table_shape(op, page_table, lengths)
     if free_pages.dim() != 1 or free_count.numel() != 1 or status.numel() != 1:
         raise RuntimeError(f"{op}: free_pages is [pages], free_count and status one number each")
@@ -109,13 +133,13 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     if new_lengths is not None:
         if grow:
             raise RuntimeError(f"{op}: new_lengths or grow, not both")
-        _require(op, device, new_lengths=(new_lengths, i32))
+        _require(op, device, "new_lengths", new_lengths, i32)
         if new_lengths.shape != lengths.shape:
             raise RuntimeError(f"{op}: new_lengths {list(new_lengths.shape)} do not fit lengths {list(lengths.shape)}")
         new = new_lengths.data_ptr()
     slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
     positions = torch.empty(max_tokens, dtype=i32, device=device)
-    query_start = torch.empty(requests + 1, dtype=i32, device=device)
+    query_start = lengths.new_empty(requests + 1)
     _call(device, N.lib().tn_kv_pages_resize, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
           int(grow), requests, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size,
           slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr())
@@ -124,16 +148,20 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t [tokens, heads, D] with the unit inner stride and 16-byte aligned rows the kernels read, copied if need be."""
-    es = t.element_size()
-    if (t.stride(2) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) * es % 16)
-            or (t.shape[1] > 1 and t.stride(1) * es % 16)):
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-    return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():  # whole rows of 64 or 128
+            return t
+        es = t.element_size()
+        if (t.stride(2) == 1 and (t.shape[0] == 1 or t.stride(0) * es % 16 == 0)
+                and (t.shape[1] == 1 or t.stride(1) * es % 16 == 0)):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _row_strides(t: torch.Tensor):
     """Element strides of token and head; a size-1 dimension is never stepped through."""
-    return (ctypes.c_int64 * 2)(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+    token, head, _ = t.stride()
+    return _TwoStrides(token if t.shape[0] > 1 else 0, head if t.shape[1] > 1 else 0)
 
 
 def kv_q4_append(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor, slots: torch.Tensor) -> None:
@@ -144,7 +172,8 @@ def kv_q4_append(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor, slo
     op = "kv_q4_append"
     device = pool.device
     _require_cuda(op, device)
-    _require(op, device, pool=(pool, torch.uint8), slots=(slots, torch.int64))
+    _require(op, device, "pool", pool, torch.uint8)
+    _require(op, device, "slots", slots, torch.int64)
     pages, heads, page_size, dim = _pool_shape(op, pool)
     if key.dtype not in _CODE or value.dtype != key.dtype:
         raise NotImplementedError(f"{op}: key and value must both be float32, float16 or bfloat16, got {key.dtype} and "
@@ -174,8 +203,9 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
     _require_cuda(op, device)
     if query.dtype not in _CODE:
         raise NotImplementedError(f"{op}: the query must be float32, float16 or bfloat16, got {query.dtype}")
-    _require(op, device, pool=(pool, torch.uint8), page_table=(page_table, torch.int32),
-             lengths=(lengths, torch.int32))
+    _require(op, device, "pool", pool, torch.uint8)
+    _require(op, device, "page_table", page_table, torch.int32)
+    _require(op, device, "lengths", lengths, torch.int32)
     pages, kv_heads, page_size, dim = _pool_shape(op, pool)
     requests, max_pages = _table_shape(op, page_table, lengths)
     if query.dim() != 3 or query.shape[2] != dim:
@@ -183,19 +213,19 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
     tokens, heads = query.shape[:2]
     start = None
     if query_start is not None:
-        _require(op, device, query_start=(query_start, torch.int32))
+        _require(op, device, "query_start", query_start, torch.int32)
         if query_start.numel() != requests + 1:
             raise RuntimeError(f"{op}: query_start must have requests + 1 = {requests + 1} entries, got "
                                f"{query_start.numel()}")
         start = query_start.data_ptr()
-    most = 1 if start is None else tokens if max_tokens is None else min(max_tokens, tokens)
+    if heads == 0 or heads % kv_heads:
+        raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
+    most = 1 if start is None else tokens if max_tokens is None else max(1, min(max_tokens, tokens))
     query = _rows(query)
-    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=device)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
-    lib = N.lib()
-    ws = torch.empty(lib.tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, dim, most), dtype=torch.uint8,
-                     device=device)
-    _call(device, lib.tn_sdpa_q4_cache, query.data_ptr(), _CODE[query.dtype], _row_strides(query), tokens, heads,
+    ws = _workspace(device, tokens, heads, kv_heads, dim, most)
+    _call(device, N.lib().tn_sdpa_q4_cache, query.data_ptr(), _CODE[query.dtype], _row_strides(query), tokens, heads,
           pool.data_ptr(), pages, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages,
           lengths.data_ptr(), requests, start, most, out.data_ptr(), lse.data_ptr(), 0.0 if scale is None else
           float(scale), ws.data_ptr(), ws.numel())
@@ -215,8 +245,11 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
     device = qkv.device
     _require_cuda(op, device)
     bf = torch.bfloat16
-    _require(op, device, qkv=(qkv, bf), rope=(rope, bf), pool=(pool, torch.uint8), page_table=(page_table, torch.int32),
-             lengths=(lengths, torch.int32))
+    _require(op, device, "qkv", qkv, bf)
+    _require(op, device, "rope", rope, bf)
+    _require(op, device, "pool", pool, torch.uint8)
+    _require(op, device, "page_table", page_table, torch.int32)
+    _require(op, device, "lengths", lengths, torch.int32)
     pages, kv_heads, page_size, dim = _pool_shape(op, pool)
     requests, max_pages = _table_shape(op, page_table, lengths)
     if tuple(qkv.shape) != (requests, (heads + 2 * kv_heads) * dim):
@@ -226,16 +259,18 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
     codes = scales = offsets = None
     if q8 is not None:
         codes, scales, offsets = q8
-        _require(op, device, codes=(codes, torch.int8), scales=(scales, torch.float32), offsets=(offsets, torch.float32))
+        _require(op, device, "codes", codes, torch.int8)
+        _require(op, device, "scales", scales, torch.float32)
+        _require(op, device, "offsets", offsets, torch.float32)
         if codes.numel() != requests * heads * dim or not scales.numel() == offsets.numel() == codes.numel() // 32:
             raise RuntimeError(f"{op}: q8 must be codes [{requests}, {heads * dim}], scales and offsets "
                                f"[{requests}, {heads * dim // 32}]")
         codes, scales, offsets = codes.data_ptr(), scales.data_ptr(), offsets.data_ptr()
+    if heads <= 0 or heads % kv_heads:
+        raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
     out = torch.empty((requests, heads, dim), dtype=bf, device=device)
-    lib = N.lib()
-    ws = torch.empty(lib.tn_sdpa_q4_workspace_bytes(requests, heads, kv_heads, dim, 1), dtype=torch.uint8,
-                     device=device)
-    _call(device, lib.tn_sdpa_q4_decode_step, qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
+    ws = _workspace(device, requests, heads, kv_heads, dim, 1)
+    _call(device, N.lib().tn_sdpa_q4_decode_step, qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
           heads, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
           out.data_ptr(), None, codes, scales, offsets, 0.0 if scale is None else float(scale), ws.data_ptr(),
           ws.numel())
