@@ -8,7 +8,9 @@ KV append -> SDPA against the cache -> o_proj -> residual -> RMSNorm ->
 gate/up (one fused Q4_0 linear) -> SiLU*up -> down_proj -> residual; then the
 final norm, lm_head and argmax. The KV cache is the reference's
 PreallocatedCache layout (torchnative/python/torchnative/kernels/kv_cache.py:
-51-185): one [B, Hkv, capacity, D] buffer per layer, read in place.
+51-185): one [B, Hkv, capacity, D] buffer per layer, read in place; or, with
+kv_cache="q4_0", pages of Q4_0 blocks (torchnative_b200.kv_cache), a quarter of
+the bytes, each request at a length of its own.
 
 Weights are random (synthetic, seeded): Q4_0 blobs built directly in the
 block layout (codes uniform in [-8, 7], scales f16(|N(0,1)| * 0.01)), bf16
@@ -67,6 +69,14 @@ def rope_inv_freq(head_dim: int, theta: float) -> torch.Tensor:
     return 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.int64).float() / head_dim))
 
 
+def rope_table(positions: int, head_dim: int, theta: float) -> torch.Tensor:
+    """bf16 [positions, D]: cosines, then sines, of every position's angles
+    (position times inv_freq, in 64 bits: far positions' angles are whole turns
+    off in 32)."""
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * rope_inv_freq(head_dim, theta).double()
+    return torch.cat((angle.cos(), angle.sin()), 1).to(torch.bfloat16)
+
+
 class Q4LlamaDecoder:
     """The decode step on one GPU, or on rank `tp.rank` of a tensor-parallel
     group (`tp` a torchnative_b200.tp.TPGroup): then q/k/v, gate/up and
@@ -78,7 +88,7 @@ class Q4LlamaDecoder:
 
     def __init__(self, shape: LlamaShape, batch: int, capacity: int, device, seed: int = 0,
                  layers: int | None = None, tp=None, exchange: str = "p2p", weights: dict | None = None,
-                 mega: bool | None = None, tp_plan: str = "rowwise"):
+                 mega: bool | None = None, tp_plan: str = "rowwise", kv_cache: str = "bf16", page_size: int = 64):
         """`weights` (from `from_gguf`): the full model's tensors on `device`
         -- per layer attn_norm, qkv, o, mlp_norm, gate_up, down as below, plus
         final_norm, lm_head, embed -- used instead of the seeded random ones.
@@ -89,11 +99,19 @@ class Q4LlamaDecoder:
         makes o_proj and down_proj row-parallel with their all-reduce fused
         into the GEMV (peer-memory exchange, batch <= 4; otherwise it falls
         back to "colwise"), "colwise" column-shards every linear with an
-        all-gather after each (the one-GPU token stream bit for bit)."""
+        all-gather after each (the one-GPU token stream bit for bit).
+        `kv_cache`: "bf16", one dense buffer a layer and one position for all
+        sequences, or "q4_0", Q4_0 blocks in pages of `page_size` tokens
+        (`self.paged`, a PagedQ4Cache): every sequence at its own length, one
+        of length 0 idle."""
         from . import tp as tpm
 
         self.s = shape
         self.B, self.cap = batch, capacity
+        if kv_cache not in ("bf16", "q4_0"):
+            raise ValueError(f"unknown kv_cache {kv_cache!r} (bf16 or q4_0)")
+        if kv_cache == "q4_0" and mega:
+            raise NotImplementedError("the persistent decode kernel reads a bf16 cache")
         self.dev = torch.device(device)
         self.n_layers = shape.layers if layers is None else layers
         self.tp = tp if tp is not None and tp.world > 1 else None
@@ -156,10 +174,26 @@ class Q4LlamaDecoder:
             self.embed = weights["embed"]
         else:
             self.embed = (0.02 * torch.randn((s.vocab, s.hidden), device=dev, generator=gen)).to(bf)
-        self.k_cache = [torch.zeros((batch, self.hkv, capacity, s.head_dim), device=dev, dtype=bf)
-                        for _ in range(self.n_layers)]
-        self.v_cache = [torch.zeros_like(self.k_cache[0]) for _ in range(self.n_layers)]
         self.inv_freq = rope_inv_freq(s.head_dim, s.rope_theta).to(dev)
+        self.paged = None
+        if kv_cache == "q4_0":
+            from .kv_cache import PagedQ4Cache
+
+            self.k_cache = self.v_cache = None
+            per_request = -(-capacity // page_size)
+            self.paged = PagedQ4Cache(self.n_layers, self.hkv, s.head_dim, batch * per_request, batch, per_request,
+                                      page_size, dev)
+            self.rope = rope_table(capacity, s.head_dim, s.rope_theta).to(dev)
+            # what a step's resize writes, and the attention's scratch: at fixed addresses, for the captured step
+            self._slots = torch.empty(batch, device=dev, dtype=torch.int64)
+            self._positions = torch.empty(batch, device=dev, dtype=torch.int32)
+            self._query_start = torch.empty(batch + 1, device=dev, dtype=torch.int32)
+            self._attn_ws = torch.empty(N.lib().tn_sdpa_q4_workspace_bytes(batch, self.hq, self.hkv, s.head_dim, 1),
+                                        device=dev, dtype=torch.uint8)
+        else:
+            self.k_cache = [torch.zeros((batch, self.hkv, capacity, s.head_dim), device=dev, dtype=bf)
+                            for _ in range(self.n_layers)]
+            self.v_cache = [torch.zeros_like(self.k_cache[0]) for _ in range(self.n_layers)]
         B, H, I = batch, s.hidden, s.inter
         kmax = max(H, I, s.heads * s.head_dim)
         self.h = torch.zeros((B, H), device=dev, dtype=bf)
@@ -208,7 +242,7 @@ class Q4LlamaDecoder:
         self.pos = torch.zeros(1, device=dev, dtype=torch.int32)
         st = lambda t: (ctypes.c_int64 * 4)(*[0 if t.shape[i] == 1 and i < 3 else t.stride(i) for i in range(4)])  # noqa: E731
         self._qstr = st(self.q_rot)
-        self._kstr = st(self.k_cache[0])
+        self._kstr = None if self.k_cache is None else st(self.k_cache[0])
         self._graph = None
         # Up to 4 rows, RMSNorm and the activation quantisation run inside the
         # Q4_0 GEMVs, SiLU*up in the gate/up GEMV's epilogue, and RoPE/append/
@@ -346,7 +380,8 @@ class Q4LlamaDecoder:
 
     def kv_bytes(self, length: int) -> int:
         s = self.s
-        return 2 * self.n_layers * self.B * self.hkv * length * s.head_dim * 2
+        tokens = self.n_layers * self.B * self.hkv * length
+        return tokens * 9 * s.head_dim // 8 if self.paged is not None else 2 * tokens * s.head_dim * 2
 
     @property
     def kernels_per_layer(self) -> int:
@@ -359,10 +394,12 @@ class Q4LlamaDecoder:
         if self._mega is not None:
             return 0  # the whole token is one launch (kernels_per_step)
         if self.rowwise:  # both reductions inside the GEMVs
-            return 5 if self.fused else 10
+            return 5 if self.fused else 8 if self.paged is not None else 10
         if self.fused:
             # one GPU: gate/up also writes the planar Q8_0 of act (no quantiser launch)
             return (5 if self.tp is None else 6) + extra
+        if self.paged is not None:  # rotary embedding, append and attention in one, on one GPU the quantiser too
+            return (8 if self.tp is None else 9) + extra
         return 11 + extra
 
     @property
@@ -373,11 +410,13 @@ class Q4LlamaDecoder:
             extra = 2  # the logits gather and the epoch step
         else:
             extra = 1 if (self.tp is not None and self.B > 1) else 0
+        if self.paged is not None:
+            extra += 1  # the step's pages
         return self.kernels_per_layer * self.n_layers + (2 if self.fused else 3) + extra
 
     @classmethod
     def from_gguf(cls, path, batch: int, capacity: int, device, layers: int | None = None, tp=None,
-                  exchange: str = "p2p") -> "Q4LlamaDecoder":
+                  exchange: str = "p2p", kv_cache: str = "bf16", page_size: int = 64) -> "Q4LlamaDecoder":
         """A decoder whose weights are a llama GGUF file's own tensors
         (transformers' GGUF tensor map for llama: blk.N.attn_q / attn_k /
         attn_v / attn_output / ffn_gate / ffn_up / ffn_down / attn_norm /
@@ -440,15 +479,36 @@ class Q4LlamaDecoder:
             lm = "output.weight" if "output.weight" in f.tensors else "token_embd.weight"
             weights = {"layers": lw_all, "final_norm": dense_bf16("output_norm.weight"), "lm_head": q4(lm),
                        "embed": dense_bf16("token_embd.weight")}
-        return cls(shape, batch, capacity, dev, layers=layers, tp=tp, exchange=exchange, weights=weights)
+        return cls(shape, batch, capacity, dev, layers=layers, tp=tp, exchange=exchange, weights=weights,
+                   kv_cache=kv_cache, page_size=page_size)
 
-    def fill_prompt_cache(self, length: int, seed: int = 1) -> None:
+    def fill_prompt_cache(self, length, seed: int = 1) -> None:
         """The prompt's K/V: synthetic N(0,1) values in slots [0, length), and
-        the position set to `length` (the decode loop continues from there)."""
+        the position set to `length` (the decode loop continues from there).
+        With a paged cache `length` may be a list, one for each sequence, 0 for
+        an idle one; a sequence's values then do not depend on the others'."""
         g = torch.Generator(device=self.dev)
         g.manual_seed(seed)
         s = self.s
         h0 = (self.tp.rank if self.tp else 0) * self.hkv  # this rank's KV heads of the full cache
+        if self.paged is not None:
+            lengths = [int(length)] * self.B if isinstance(length, int) else [int(n) for n in length]
+            if len(lengths) != self.B or min(lengths) < 0 or max(lengths) == 0 or max(lengths) > self.cap:
+                raise ValueError(f"{self.B} lengths of 0 to {self.cap} tokens are wanted, not all 0; got {lengths}")
+            new = torch.tensor(lengths, device=self.dev, dtype=torch.int32)
+            self.paged.resize(0, new_lengths=torch.zeros_like(new))
+            slots, _, _ = self.paged.resize(sum(lengths), new_lengths=new)
+            gens = [g] if isinstance(length, int) else [torch.Generator(device=self.dev).manual_seed(seed + b)
+                                                        for b in range(self.B)]
+            for li in range(self.n_layers):
+                kv = []
+                for _ in range(2):
+                    full = [torch.empty((self.B // len(gens), s.kv_heads, n, s.head_dim), device=self.dev,
+                                        dtype=torch.bfloat16).normal_(generator=gen)
+                            for n, gen in zip(lengths, gens)]
+                    kv.append(torch.cat([x[:, h0:h0 + self.hkv].transpose(1, 2).flatten(0, 1) for x in full]))
+                self.paged.append(li, kv[0], kv[1], slots)
+            return
         for kc, vc in zip(self.k_cache, self.v_cache):
             for c in (kc, vc):
                 full = torch.empty((self.B, s.kv_heads, length, s.head_dim), device=self.dev, dtype=c.dtype)
@@ -463,6 +523,34 @@ class Q4LlamaDecoder:
                                        P(self.h.data_ptr()), self._stream()))
 
     # ---- the step
+
+    def _pages(self, stream) -> None:
+        """Pages for the step's token of every sequence that has tokens."""
+        c = self.paged
+        requests, max_pages = c.page_table.shape
+        N.check(N.lib().tn_kv_pages_resize(
+            P(c.page_table.data_ptr()), max_pages, max_pages, P(c.lengths.data_ptr()), None, 1, requests,
+            P(c.free_pages.data_ptr()), P(c.free_count.data_ptr()), c.free_pages.shape[0], c.page_size,
+            P(self._slots.data_ptr()), P(self._positions.data_ptr()), requests, P(self._query_start.data_ptr()),
+            P(c.status.data_ptr()), stream))
+
+    def _attn_paged(self, li, out, stream, q8: bool) -> None:
+        """Rotary embedding, append and attention of layer li's new tokens from
+        self.qkv_out, into `out` and, with q8, its planar Q8_0 into the linears'
+        activations."""
+        c, s = self.paged, self.s
+        pool = c.pools[li]
+        requests, max_pages = c.page_table.shape
+        codes = (P(t.data_ptr()) if q8 else None for t in (self.codes, self.scales, self.offsets))
+        N.check(N.lib().tn_sdpa_q4_decode_step(
+            P(self.qkv_out.data_ptr()), P(self.rope.data_ptr()), self.rope.shape[0], P(pool.data_ptr()), pool.shape[0],
+            self.hq, self.hkv, s.head_dim, c.page_size, P(c.page_table.data_ptr()), max_pages, max_pages,
+            P(c.lengths.data_ptr()), requests, P(out.data_ptr()), None, *codes, 1.0 / math.sqrt(s.head_dim),
+            P(self._attn_ws.data_ptr()), self._attn_ws.numel(), stream))
+
+    def _advance(self):
+        """The position that the argmax kernel moves on (a paged cache's lengths moved with its pages)."""
+        return None if self.paged is not None else P(self.pos.data_ptr())
 
     @staticmethod
     def _stream():
@@ -482,10 +570,13 @@ class Q4LlamaDecoder:
 
     def step(self, stream=None) -> None:
         """One token for every sequence: reads tokens' embeddings in self.h and
-        the position self.pos; leaves the next tokens in self.tokens, their
-        embeddings in self.h, and self.pos advanced by one."""
+        the position self.pos (a paged cache: its lengths); leaves the next
+        tokens in self.tokens, their embeddings in self.h, and the position
+        advanced by one. Of an idle sequence of a paged cache they mean nothing."""
         if self._mega is not None:
             return self._step_mega(stream or self._stream())
+        if self.paged is not None:
+            self._pages(stream or self._stream())
         if self.fused:
             return self._step_fused(stream or self._stream())
         if self.rowwise:
@@ -496,19 +587,23 @@ class Q4LlamaDecoder:
         for li, lw in enumerate(self.layers):
             self._norm(None if li == 0 else self.delta, lw["attn_norm"], stream)
             self._linear(lw["qkv"], self.qkv_out, self.qkv_l, s.hidden, stream)
-            kc, vc = self.k_cache[li], self.v_cache[li]
-            N.check(L.tn_llama_rope_append(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
-                                           P(self.pos.data_ptr()), 0, B, Hq, Hkv, D, P(self.q_rot.data_ptr()),
-                                           P(kc.data_ptr()), P(vc.data_ptr()), kc.stride(0), kc.stride(1), stream))
-            N.check(L.tn_sdpa_decode_cache(P(self.q_rot.data_ptr()), P(kc.data_ptr()), P(vc.data_ptr()),
-                                           P(self.attn_l.data_ptr()), None, N.TN_BF16, B, Hq, Hkv, D, self.cap,
-                                           self._qstr, self._kstr, self._kstr, P(self.pos.data_ptr()), 1,
-                                           1.0 / math.sqrt(D), stream))
+            if self.paged is not None:
+                self._attn_paged(li, self.attn_l, stream, q8=self.tp is None)
+            else:
+                kc, vc = self.k_cache[li], self.v_cache[li]
+                N.check(L.tn_llama_rope_append(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
+                                               P(self.pos.data_ptr()), 0, B, Hq, Hkv, D, P(self.q_rot.data_ptr()),
+                                               P(kc.data_ptr()), P(vc.data_ptr()), kc.stride(0), kc.stride(1), stream))
+                N.check(L.tn_sdpa_decode_cache(P(self.q_rot.data_ptr()), P(kc.data_ptr()), P(vc.data_ptr()),
+                                               P(self.attn_l.data_ptr()), None, N.TN_BF16, B, Hq, Hkv, D, self.cap,
+                                               self._qstr, self._kstr, self._kstr, P(self.pos.data_ptr()), 1,
+                                               1.0 / math.sqrt(D), stream))
             self._gather(self.attn_l, self.attn, 4 * li, stream)
             HD = s.heads * D
-            N.check(L.tn_q8_0_quantize_planar(P(self.attn.data_ptr()), N.TN_BF16, HD, P(self.codes.data_ptr()),
-                                              HD, P(self.scales.data_ptr()), P(self.offsets.data_ptr()), B, HD,
-                                              stream))
+            if self.paged is None or self.tp is not None:
+                N.check(L.tn_q8_0_quantize_planar(P(self.attn.data_ptr()), N.TN_BF16, HD, P(self.codes.data_ptr()),
+                                                  HD, P(self.scales.data_ptr()), P(self.offsets.data_ptr()), B, HD,
+                                                  stream))
             self._linear(lw["o"], self.delta_l, self.h_l, HD, stream)
             self._gather(self.delta_l, self.delta, 4 * li + 1, stream)
             self._norm(self.delta, lw["mlp_norm"], stream)
@@ -524,7 +619,7 @@ class Q4LlamaDecoder:
         self._gather(self.logits_l, self.logits, 4 * self.n_layers, stream)
         N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
                                         P(self.embed.data_ptr()), s.hidden, P(self.h.data_ptr()),
-                                        P(self.pos.data_ptr()), stream))
+                                        self._advance(), stream))
         self._step_end(stream)
 
     def _fused_linear(self, mode, x, x_stride, delta, h_out, norm_w, w, y, n, k, stream, flags=0, link=None,
@@ -563,12 +658,15 @@ class Q4LlamaDecoder:
         for li, lw in enumerate(self.layers):
             self._fused_linear(N.TN_X_RMSNORM, ha, H, None if li == 0 else self.delta, hb, lw["attn_norm"],
                                lw["qkv"], self.qkv_out, self.qkv_l, H, stream)
-            kc, vc = self.k_cache[li], self.v_cache[li]
-            N.check(L.tn_sdpa_decode_step_q8(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
-                                             P(kc.data_ptr()), P(vc.data_ptr()), P(self.attn_l.data_ptr()), None,
-                                             P(self.codes.data_ptr()), P(self.scales.data_ptr()),
-                                             P(self.offsets.data_ptr()), B, Hq, Hkv, D, self.cap, self._kstr,
-                                             self._kstr, P(self.pos.data_ptr()), 1.0 / math.sqrt(D), stream))
+            if self.paged is not None:
+                self._attn_paged(li, self.attn_l, stream, q8=True)
+            else:
+                kc, vc = self.k_cache[li], self.v_cache[li]
+                N.check(L.tn_sdpa_decode_step_q8(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
+                                                 P(kc.data_ptr()), P(vc.data_ptr()), P(self.attn_l.data_ptr()), None,
+                                                 P(self.codes.data_ptr()), P(self.scales.data_ptr()),
+                                                 P(self.offsets.data_ptr()), B, Hq, Hkv, D, self.cap, self._kstr,
+                                                 self._kstr, P(self.pos.data_ptr()), 1.0 / math.sqrt(D), stream))
             self._linear(lw["o"], self.delta, H, Hq * D, stream, link=links[("o", li)])
             self._fused_linear(N.TN_X_RMSNORM, hb, H, self.delta, ha, lw["mlp_norm"], lw["gate_up"], self.act_l,
                                2 * self.i_l, H, stream, N.TN_EPILOGUE_SILU_MUL_PAIRS, q8=q8out)
@@ -582,7 +680,7 @@ class Q4LlamaDecoder:
         self._gather(self.logits_l, self.logits, 0, stream)
         N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
                                         P(self.embed.data_ptr()), s.hidden, P(ha.data_ptr()),
-                                        P(self.pos.data_ptr()), stream))
+                                        self._advance(), stream))
         self._step_end(stream)
 
     def _step_rowwise_rows(self, stream) -> None:
@@ -600,16 +698,20 @@ class Q4LlamaDecoder:
         for li, lw in enumerate(self.layers):
             self._norm(None if li == 0 else self.delta, lw["attn_norm"], stream)
             self._linear(lw["qkv"], self.qkv_out, self.qkv_l, H, stream)
-            kc, vc = self.k_cache[li], self.v_cache[li]
-            N.check(L.tn_llama_rope_append(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
-                                           P(self.pos.data_ptr()), 0, B, Hq, Hkv, D, P(self.q_rot.data_ptr()),
-                                           P(kc.data_ptr()), P(vc.data_ptr()), kc.stride(0), kc.stride(1), stream))
-            N.check(L.tn_sdpa_decode_cache(P(self.q_rot.data_ptr()), P(kc.data_ptr()), P(vc.data_ptr()),
-                                           P(self.attn_l.data_ptr()), None, N.TN_BF16, B, Hq, Hkv, D, self.cap,
-                                           self._qstr, self._kstr, self._kstr, P(self.pos.data_ptr()), 1,
-                                           1.0 / math.sqrt(D), stream))
-            N.check(L.tn_q8_0_quantize_planar(P(self.attn_l.data_ptr()), N.TN_BF16, HD, P(self.codes.data_ptr()), HD,
-                                              P(self.scales.data_ptr()), P(self.offsets.data_ptr()), B, HD, stream))
+            if self.paged is not None:
+                self._attn_paged(li, self.attn_l, stream, q8=True)
+            else:
+                kc, vc = self.k_cache[li], self.v_cache[li]
+                N.check(L.tn_llama_rope_append(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
+                                               P(self.pos.data_ptr()), 0, B, Hq, Hkv, D, P(self.q_rot.data_ptr()),
+                                               P(kc.data_ptr()), P(vc.data_ptr()), kc.stride(0), kc.stride(1), stream))
+                N.check(L.tn_sdpa_decode_cache(P(self.q_rot.data_ptr()), P(kc.data_ptr()), P(vc.data_ptr()),
+                                               P(self.attn_l.data_ptr()), None, N.TN_BF16, B, Hq, Hkv, D, self.cap,
+                                               self._qstr, self._kstr, self._kstr, P(self.pos.data_ptr()), 1,
+                                               1.0 / math.sqrt(D), stream))
+                N.check(L.tn_q8_0_quantize_planar(P(self.attn_l.data_ptr()), N.TN_BF16, HD, P(self.codes.data_ptr()),
+                                                  HD, P(self.scales.data_ptr()), P(self.offsets.data_ptr()), B, HD,
+                                                  stream))
             self._linear(lw["o"], self.delta, H, HD, stream, link=links[("o", li)])
             self._norm(self.delta, lw["mlp_norm"], stream)
             self._linear(lw["gate_up"], self.act_l, 2 * self.i_l, H, stream, N.TN_EPILOGUE_SILU_MUL_PAIRS)
@@ -622,7 +724,7 @@ class Q4LlamaDecoder:
         self._gather(self.logits_l, self.logits, 0, stream)
         N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
                                         P(self.embed.data_ptr()), s.hidden, P(self.h.data_ptr()),
-                                        P(self.pos.data_ptr()), stream))
+                                        self._advance(), stream))
         self._step_end(stream)
 
     def _step_fused(self, stream) -> None:
@@ -639,8 +741,12 @@ class Q4LlamaDecoder:
             self._fused_linear(N.TN_X_RMSNORM, ha, H, None if li == 0 else self.delta, hb, lw["attn_norm"],
                                lw["qkv"], self.qkv_out, self.qkv_l, H, stream,
                                link=links[("qkv", li)] if fg and li > 0 else None)
-            kc, vc = self.k_cache[li], self.v_cache[li]
-            if self.tp is None:
+            if self.paged is not None:
+                self._attn_paged(li, self.attn_l, stream, q8=self.tp is None)
+                if self.tp is None:
+                    self._linear(lw["o"], self.delta, H, HD, stream)
+            elif self.tp is None:
+                kc, vc = self.k_cache[li], self.v_cache[li]
                 # one GPU: the attention's merging CTAs also write its planar Q8_0,
                 # and o_proj stages those codes (no per-CTA bf16 -> Q8 prologue)
                 N.check(L.tn_sdpa_decode_step_q8(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
@@ -650,10 +756,12 @@ class Q4LlamaDecoder:
                                                  self._kstr, P(self.pos.data_ptr()), 1.0 / math.sqrt(D), stream))
                 self._linear(lw["o"], self.delta, H, HD, stream)
             else:
+                kc, vc = self.k_cache[li], self.v_cache[li]
                 N.check(L.tn_sdpa_decode_step(P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()),
                                               P(kc.data_ptr()), P(vc.data_ptr()), P(self.attn_l.data_ptr()), None, B,
                                               Hq, Hkv, D, self.cap, self._kstr, self._kstr, P(self.pos.data_ptr()),
                                               1.0 / math.sqrt(D), stream))
+            if self.tp is not None:
                 self._gather(self.attn_l, self.attn, 4 * li, stream)
                 self._fused_linear(N.TN_X_BF16, self.attn, HD, None, None, None, lw["o"], self.delta_l, self.h_l, HD,
                                    stream, link=links[("o", li)] if fg else None)
@@ -683,7 +791,7 @@ class Q4LlamaDecoder:
         self._gather(self.logits_l, self.logits, 4 * self.n_layers, stream)
         N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
                                         P(self.embed.data_ptr()), s.hidden, P(ha.data_ptr()),
-                                        P(self.pos.data_ptr()), stream))
+                                        self._advance(), stream))
         self._step_end(stream)
 
     def _build_links(self) -> dict:
@@ -729,7 +837,8 @@ class Q4LlamaDecoder:
         parts = {
             "qkv_rmsnorm_gemv": lambda lw, li, st: self._fused_linear(
                 N.TN_X_RMSNORM, ha, H, self.delta, hb, lw["attn_norm"], lw["qkv"], self.qkv_out, self.qkv_l, H, st),
-            "sdpa_decode_step_q8": lambda lw, li, st: N.check(L.tn_sdpa_decode_step_q8(
+            "sdpa_decode_step_q8": (lambda lw, li, st: self._attn_paged(li, self.attn_l, st, q8=True))
+            if self.paged is not None else lambda lw, li, st: N.check(L.tn_sdpa_decode_step_q8(
                 P(self.qkv_out.data_ptr()), P(self.inv_freq.data_ptr()), P(self.k_cache[li].data_ptr()),
                 P(self.v_cache[li].data_ptr()), P(self.attn_l.data_ptr()), None, P(self.codes.data_ptr()),
                 P(self.scales.data_ptr()), P(self.offsets.data_ptr()), B, Hq, Hkv, D, self.cap, self._kstr,
