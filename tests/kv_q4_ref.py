@@ -44,7 +44,7 @@ def dense_request(pool, table_row, length, page_size):
     return tuple(x[pages].transpose(0, 1).flatten(1, 2)[:, :length].double() for x in kv.kv_q4_dense(pool))
 
 
-def attention(q, pool, table, lengths, page_size, query_start=None, scale=None):
+def attention(q, pool, table, lengths, page_size, query_start=None, scale=None, tiles=False):
     """(out, lse, bound, lse_bound), all float64; rows that belong to no request are NaN.
 
     The bounds, first order, for kernels that multiply exact 4-bit codes with queries and probabilities carried in
@@ -60,6 +60,10 @@ def attention(q, pool, table, lengths, page_size, query_start=None, scale=None):
       below float16's normal numbers those roundings are half a subnormal step, 2^-25, where the row's largest
       probability, times a scale of the larger of 1 and twice the largest scale d, stands for 2^10 at least: at most
       2 * 2^-35 max(1, 2 d), times a code of at most 8, for every key that the row sees;
+      in the tcgen05 tiles (`tiles`) keys and values are float16 themselves, a group of 16 tokens taken to a largest
+      scale below 1 by a power of two, at most twice its largest scale: a scale 2^-14 or less of that is rounded to
+      subnormals, half a step 2^-25, times a code of at most 8: 2^-22 of the power, 2^-21 of the largest scale, in
+      every element of a key (times its query element) and of a value (times its probability);
       the result is rounded to its type: half a step of its value, or half the spacing of the subnormals."""
     h = {torch.float32: 2.0**-22, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-10}[q.dtype]
     step = HALF_STEP[q.dtype]
@@ -84,6 +88,9 @@ def attention(q, pool, table, lengths, page_size, query_start=None, scale=None):
         ds = scale * 2.0**-24 * ((dim + 8) * (x.abs() @ k.abs().transpose(1, 2))
                                  + x.abs().amax(-1, keepdim=True) * k.abs().sum(-1)[:, None])
         sees = torch.arange(length)[None] < (length - n + 1 + torch.arange(n))[:, None]
+        dmax = [(x.abs().amax() / 8).item() for x in (k, v)]  # a block's largest element has code 0: eight scales
+        if tiles:
+            ds = ds + scale * 2.0**-21 * dmax[0] * x.abs().sum(-1, keepdim=True)
         s = s.masked_fill(~sees, -math.inf)
         some = sees.any(-1)
         e = torch.logsumexp(s, -1)
@@ -93,16 +100,15 @@ def attention(q, pool, table, lengths, page_size, query_start=None, scale=None):
         o = p @ v
         out[rows] = o.transpose(0, 1)
         lse[rows] = torch.where(some, e, 0.0).transpose(0, 1)
-        dmax = v.abs().amax() / 8  # the largest element of a block has code 0: eight scales
-        floor = sees.sum(-1)[:, None] * 16 * 2.0**-35 * max(1.0, 2 * dmax.item())
+        floor = sees.sum(-1)[:, None] * 16 * 2.0**-35 * max(1.0, 2 * dmax[1]) + (2.0**-21 * dmax[1] if tiles else 0.0)
         bound[rows] = ((rel + h)[..., None] * (p @ v.abs()) + floor + (step * o.abs()).clamp(min=HALF_SUBNORMAL[q.dtype]) + 1e-30).transpose(0, 1)
         lse_bound[rows] = (rel + 2.0**-22 * e.abs()).transpose(0, 1)
     return out, lse, bound, lse_bound
 
 
-def check_attention(got, q, pool, table, lengths, page_size, query_start=None, scale=None):
+def check_attention(got, q, pool, table, lengths, page_size, query_start=None, scale=None, tiles=False):
     out, lse = (x.double().cpu() for x in got)
-    want, want_lse, bound, lse_bound = attention(q, pool, table, lengths, page_size, query_start, scale)
+    want, want_lse, bound, lse_bound = attention(q, pool, table, lengths, page_size, query_start, scale, tiles)
     rows = ~want_lse.isnan().any(-1)
     assert torch.isfinite(out[rows]).all()
     over = ((out - want).abs() - bound)[rows]

@@ -217,6 +217,64 @@ def test_many_token_attention(cuda_device, dtype, heads, kv_heads, dim, page_siz
         check_attention(got, q, st.pool, st.table, st.lengths, page_size, start)
 
 
+@pytest.mark.parametrize("heads, kv_heads, dim, page_size, new, lengths", [
+    (32, 4, 128, 64, [800], [900]), (8, 2, 128, 16, [3300, 1, 700], [3300, 7, 5000]),
+    (9, 3, 64, 32, [1000, 0, 2000], [3000, 5, 2100]), (64, 8, 64, 128, [400, 3], [390, 100]),
+    (16, 16, 128, 1024, [129, 130, 700, 900], [129, 1000, 701, 0]), (30, 2, 64, 16, [513, 400], [600, 405])])
+def test_attention_of_whole_tiles(cuda_device, heads, kv_heads, dim, page_size, new, lengths):
+    """Enough bf16 rows for the tensor-core tiles; the same call with a small bound on a request's tokens, or in float16,
+    takes the other kernel. More tokens than keys among them: zeros."""
+    st = State(lengths, kv_heads, dim, page_size, cuda_device, seed=sum(new), magnitude=2.0)
+    q = st.randn(sum(new), heads, dim, dtype=BF)
+    start = starts(new, cuda_device)
+    for most, x, tiles in ((max(new), q, 1), (1, q, 0), (max(new), q.to(F16), 0)):
+        N.reset_counters()
+        got = kv.sdpa_q4_cache(x, st.pool, st.table, st.lengths, query_start=start, max_tokens=most)
+        N.device_status()
+        assert N.counters()["sdpa_prefill_launches"] == tiles
+        check_attention(got, x, st.pool, st.table, st.lengths, page_size, start, tiles=bool(tiles))
+
+
+def test_tiles_with_odd_contents(cuda_device):
+    """Scales over their range in keys and values, queries of any magnitude, missing pages and garbage behind the last
+    token, in the tensor-core tiles."""
+    new, lengths = [500, 400], [530, 1001]
+    st = State(lengths, 2, 64, 64, cuda_device)
+    slots = torch.arange(st.pool.shape[0] * 64, device=cuda_device)
+    k, v = st.randn(len(slots), 2, 64), st.randn(len(slots), 2, 64)
+    v[0::4] *= 2.0**13
+    v[1::4, :, :32] *= 2.0**-12
+    v[2::4] = 0
+    k[3::5] *= 2.0**-9
+    kv.kv_q4_append(k, v, st.pool, slots)
+    q = st.randn(900, 32, 64)
+    q[::3] *= 2.0**-60
+    q[1::3] *= 4
+    q[2] = 0
+    q = q.to(BF)
+    start = starts(new, cuda_device)
+    want = kv.sdpa_q4_cache(q, st.pool, st.table, st.lengths, query_start=start)
+    N.device_status()
+    check_attention(want, q, st.pool, st.table, st.lengths, 64, start, tiles=True)
+    bad = torch.full((64, 2, 64), float("nan"), device=cuda_device)
+    bad[::2] = float("inf")
+    behind = torch.cat([st.table[0, 8] * 64 + torch.arange(18, 64, device=cuda_device),
+                        st.table[1, 15] * 64 + torch.arange(41, 64, device=cuda_device)]).long()
+    kv.kv_q4_append(bad.repeat(2, 1, 1)[:len(behind)], bad.repeat(2, 1, 1)[:len(behind)], st.pool, behind)
+    got = kv.sdpa_q4_cache(q, st.pool, st.table, st.lengths, query_start=start)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    st.table[0, 1], st.table[0, 3] = 1 << 30, -1
+    got = kv.sdpa_q4_cache(q, st.pool, st.table, st.lengths, query_start=start)
+    with pytest.raises(RuntimeError, match="page id"):
+        N.device_status()
+    assert torch.equal(got[0][500:], want[0][500:]) and torch.isfinite(got[0]).all()
+    # the keys of the missing pages are left out: as if the request had only the others
+    kept = st.table[:1, [0, 2, 4, 5, 6, 7, 8]].contiguous()
+    last = torch.tensor([530 - 128], dtype=torch.int32, device=cuda_device)
+    check_attention((got[0][400:500], got[1][400:500]), q[400:500], st.pool, kept, last, 64, starts([100], cuda_device),
+                    tiles=True)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_more_tokens_than_keys(cuda_device, dtype, dim):

@@ -9,21 +9,10 @@
 #include <atomic>
 #include <chrono>
 
-#include "kv_q4.cuh"
+#include "sdpa_q4.cuh"
 
 namespace tn {
 namespace {
-
-struct Attend {
-    const void *q;
-    int64_t q_token, q_head;  // element strides
-    KvPool c;
-    const int *query_start;  // [requests + 1], or NULL: token r is request r's only one
-    void *out;               // [tokens][heads][D]
-    float *lse;              // [tokens][heads] or NULL
-    int tokens, heads, rep;
-    float scale;
-};
 
 // ---- the kernel
 //
@@ -143,55 +132,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-
-// (a & mask) | bits as one instruction: `bits` in a register of its own, since an instruction takes one constant only.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
-    return r;
-}
-
-// The nibbles n and n + 4 of a word as half2, n = 0 .. 3: codes minus 8, except
-// that with RAW the odd ones come as 64 + code.
-template <bool RAW>
-__device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&e)[4], uint32_t low, uint32_t high) {
-    constexpr uint32_t kLow = 0x64086408u, kHigh = 0x54805480u;  // 1032, 72
-    const uint32_t u = w >> 8;
-    e[0] = sub_f16x2(and_or(w, 0x000f000fu, low), kLow);
-    e[1] = and_or(w, 0x00f000f0u, high);
-    e[2] = sub_f16x2(and_or(u, 0x000f000fu, low), kLow);
-    e[3] = and_or(u, 0x00f000f0u, high);
-    if constexpr (!RAW) {
-        e[1] = sub_f16x2(e[1], kHigh);
-        e[3] = sub_f16x2(e[3], kHigh);
-    }
-}
-
 // A place in the line of units: group g of item (b, tile u, head h), whose
 // groups this CTA has from `from` to `upto`. `rel` is the place of the item's
 // group 0 against the first of the CTA's `len` places.
@@ -202,12 +142,7 @@ struct Cursor {
 
     __device__ __forceinline__ void load_request(const Attend &p) {
         S = p.c.length(b);
-        first = b;
-        n = 1;
-        if (p.query_start) {
-            first = min(max(p.query_start[b], 0), p.tokens);
-            n = max(min(p.query_start[b + 1], p.tokens) - first, 0);
-        }
+        n = p.query_tokens(b, &first);
         tiles = (n * p.rep + RT - 1) / RT;
     }
     // units that the tile's last row sees; 1 where it sees none, so that someone writes its zeros
@@ -1194,8 +1129,27 @@ int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op)
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * (Shape<T, D, NT>::W + 4)), Shape<T, D, NT>::SMEM, stream, op, p);
 }
 
+// Whether a call's query rows are better taken 256 at a time by the tcgen05
+// kernel. Both read the cache once for every tile of rows; per 64 keys this
+// kernel's tiles of 16 rows cost 2.7 ns each (all SMs together), and the other's
+// pairs of tiles, one an SM, 2460 ns a wave of 148 CTAs (1600 where the rows
+// fill one tile of 128 only). Measured, 32 heads on 8, D 128: 4 requests of 64
+// tokens at 16384: 377 us here, 628 there; 4 of 128: 737 and 631; 16 of 17: 465
+// and 419; 16 of 256: 5747 and 2497; 2 requests of 9 heads on 3, 256 tokens: 226
+// and 621. (D 64 has the same ratios.)
+bool fills_tiles(int64_t tokens, int64_t requests, int64_t kv_heads, int64_t rep, int64_t max_query) {
+    if (max_query * rep <= 64) return false;
+    requests = std::min(requests, tokens);
+    const int64_t rows = (tokens * rep + requests - 1) / requests;  // a request, on average
+    const double here = 2.7 * (double)((rows + 15) / 16 * requests * kv_heads);
+    const double waves = std::max(1.0, (double)((rows + 255) / 256 * requests * kv_heads) / 148.0);
+    return here > waves * (rows > 128 ? 2460.0 : 1600.0);
+}
+
 template <typename T, int D>
 int launch_attend(Split &p, int64_t max_query, void *workspace, cudaStream_t stream) {
+    if (std::is_same<T, __nv_bfloat16>::value && fills_tiles(p.a.tokens, p.a.c.requests, p.a.c.kv_heads, p.a.rep, max_query))
+        return launch_sdpa_q4_prefill(p.a, D, stream);
     return tile_rows(max_query, p.a.rep) == 8 ? launch_split<T, D, 1, false>(p, workspace, stream, "tn_sdpa_q4_cache")
                                               : launch_split<T, D, 2, false>(p, workspace, stream, "tn_sdpa_q4_cache");
 }
