@@ -44,9 +44,8 @@ __global__ void __launch_bounds__(kThreads) kv_q4_append_kernel(const Append p) 
         load8<T>(static_cast<const T *>(p.k) + token * p.k_token + head * p.k_head + e, k);
         load8<T>(static_cast<const T *>(p.v) + token * p.v_token + head * p.v_head + e, v);
     }
-    const float kd = __fdiv_rn(q4_0_extreme(k), -8.0f), vd = __fdiv_rn(q4_0_extreme(v), -8.0f);
-    const uint32_t kw = q4_0_k_word(k, kd != 0.0f ? __fdiv_rn(1.0f, kd) : 0.0f);
-    const uint32_t vw = q4_0_v_halves(v, vd != 0.0f ? __fdiv_rn(1.0f, vd) : 0.0f);
+    const float kd = q4_0_scale(q4_0_extreme(k)), vd = q4_0_scale(q4_0_extreme(v));
+    const uint32_t kw = q4_0_k_word(k, q4_0_inverse(kd)), vw = q4_0_v_halves(v, q4_0_inverse(vd));
     // an even token whose odd neighbour's row is in the other half of the lanes: their 16-bit pieces as words
     const uint32_t vw2 = __shfl_xor_sync(0xffffffffu, vw, ROW_LANES);
     const int64_t slot2 = __shfl_xor_sync(0xffffffffu, slot, ROW_LANES);

@@ -127,12 +127,29 @@ __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
 __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
 // The Q4_0 code of x in a block with reciprocal scale `inv`: trunc(x * inv + 8.5)
-// in [0, 15], NaN to 0 (Rust's `as u8`, then min 15). Explicitly rounded, so
-// that no contraction changes a byte.
-__device__ __forceinline__ uint32_t q4_0_code(float x, float inv) {
+// in [0, 15], NaN to 0 (Rust's `as u8`, then min 15), in the low bits of a float
+// at 2^23, whose last place is 1 and whose sum rounds toward zero. Explicitly
+// rounded, so that no contraction changes a byte.
+constexpr uint32_t kCodeBase = 0x4b000000u;  // the bits of 2^23
+__device__ __forceinline__ uint32_t q4_0_code_at_2_23(float x, float inv) {
     const float v = __fadd_rn(__fmul_rn(x, inv), 8.5f);
-    return !(v > 0.0f) ? 0u : (v >= 15.0f ? 15u : __float2uint_rz(v));
+    return __float_as_uint(__fadd_rz(fminf(fmaxf(v, 0.0f), 15.0f), 8388608.0f));
 }
+// Codes at the nibbles `at[i]` of a word; the floats' upper bits, the same of every one, go off at the end.
+template <int N>
+__device__ __forceinline__ uint32_t q4_0_word(const float (&x)[8], float inv, const int (&at)[N]) {
+    uint32_t w = 0, base = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w += q4_0_code_at_2_23(x[i], inv) * (1u << (4 * at[i]));
+        base += kCodeBase * (1u << (4 * at[i]));
+    }
+    return w - base;
+}
+// d = m / -8 and 1 / d (0 where d is 0) of a block, as IEEE float32 divisions give them: the first is a product by a
+// power of two.
+__device__ __forceinline__ float q4_0_scale(float m) { return __fmul_rn(m, -0.125f); }
+__device__ __forceinline__ float q4_0_inverse(float d) { return d != 0.0f ? __frcp_rn(d) : 0.0f; }
 
 // The element of largest magnitude of a block of 32 held 8 a lane by 4
 // neighbouring lanes in element order; the first of equals, as
@@ -157,17 +174,12 @@ __device__ __forceinline__ float q4_0_extreme(const float (&x)[8]) {
 // 8 elements a lane (lane t of the block's 4) -> the lane's K word, or its two
 // V pieces (g = 2t low, g = 2t + 1 high).
 __device__ __forceinline__ uint32_t q4_0_k_word(const float (&x)[8], float inv) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-        w |= (q4_0_code(x[2 * n], inv) << (4 * n)) | (q4_0_code(x[2 * n + 1], inv) << (16 + 4 * n));
-    return w;
+    constexpr int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+    return q4_0_word<8>(x, inv, at);
 }
 __device__ __forceinline__ uint32_t q4_0_v_halves(const float (&x)[8], float inv) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= q4_0_code(x[i], inv) << (4 * i);
-    return w;
+    constexpr int at[8] = {0, 1, 2, 3, 4, 5, 6, 7};
+    return q4_0_word<8>(x, inv, at);
 }
 
 }  // namespace tn

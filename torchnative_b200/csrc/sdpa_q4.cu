@@ -226,8 +226,7 @@ __device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = round_bf16(block < H ? x[i] * c[i] - y[i] * s[i] : x[i] * c[i] + y[i] * s[i]);
     }
-    const float d = __fdiv_rn(q4_0_extreme(x), -8.0f);
-    const float inv = (d != 0.0f) ? __fdiv_rn(1.0f, d) : 0.0f;
+    const float d = q4_0_scale(q4_0_extreme(x)), inv = q4_0_inverse(d);
     if (lane >= 8 * NB) return;
     const int key = pos & 15;
     const __half d16 = __float2half_rn(d);

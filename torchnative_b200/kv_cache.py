@@ -26,8 +26,10 @@ import torch
 from . import _native as N
 
 GROUP = 16  # tokens of one head that lie together
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
-_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_U8, _I32, _I64, _F32, _BF16 = torch.uint8, torch.int32, torch.int64, torch.float32, torch.bfloat16
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 _TwoStrides = ctypes.c_int64 * 2
 _CODE = {torch.float32: N.TN_F32, torch.bfloat16: N.TN_BF16, torch.float16: N.TN_F16}
 _STATUS = {1: "not enough free pages", 2: "a request's length is outside [0, max_pages * page_size]",
@@ -51,10 +53,9 @@ def _require_cuda(op: str, device: torch.device) -> None:
                                   "torchnative's CPU path")
 
 
-def _call(device: torch.device, fn, *args) -> None:
-    """One library call on the device's current stream; the library takes the
-    current device, which may be another one."""
-    index = device.index
+def _call(index: int, fn, *args) -> None:
+    """One library call on device `index`'s current stream; the library takes
+    the current device, which may be another one."""
     if index == _current_device():
         status = fn(*args, _current_stream(index))
     else:
@@ -64,25 +65,41 @@ def _call(device: torch.device, fn, *args) -> None:
         N.check(status)
 
 
+_templates: dict = {}
+
+
+def _empty(index: int, dtype: torch.dtype, *shape: int) -> torch.Tensor:
+    """torch.empty on device `index`; like a template without memory of its own,
+    it takes half the host's time."""
+    key = (index, dtype, shape)
+    t = _templates.get(key)
+    if t is None:
+        if len(_templates) >= 1024:
+            _templates.clear()
+        t = _templates[key] = torch.empty(1, dtype=dtype, device=torch.device("cuda", index)).expand(shape)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 _scratch: dict = {}
 
 
-def _workspace(device: torch.device, tokens: int, heads: int, kv_heads: int, dim: int, most: int) -> torch.Tensor:
+def _workspace(device: torch.device, index: int, rows: int, dim: int, *shape: int) -> torch.Tensor:
     """The attention calls' scratch: one a stream, since calls on a stream run
     one after the other; a captured call gets memory of its graph's own, since
     graphs captured on one stream may be replayed on several."""
-    key = (device.index, _current_stream(device.index), heads // kv_heads * most > 8, dim)
+    key = (index, _current_stream(index), rows > 8, dim)
     ws = _scratch.get(key)
-    if ws is None or torch._C._cuda_isCurrentStreamCapturing():
-        ws = torch.empty(N.lib().tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, dim, most), dtype=torch.uint8,
-                         device=device)
-        if not torch._C._cuda_isCurrentStreamCapturing():
+    capturing = _capturing()
+    if ws is None or capturing:
+        tokens, heads, kv_heads, most = shape
+        ws = torch.empty(N.lib().tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, dim, most), dtype=_U8, device=device)
+        if not capturing:
             _scratch[key] = ws
     return ws
 
 
 def _table_shape(op: str, page_table: torch.Tensor, lengths: torch.Tensor):
-    if page_table.dim() != 2 or lengths.dim() != 1 or page_table.shape[0] != lengths.shape[0]:
+    if page_table.dim() != 2 or lengths.shape != page_table.shape[:1]:
         raise RuntimeError(f"{op}: page_table {list(page_table.shape)} and lengths {list(lengths.shape)} do not "
                            "describe the same requests ([requests, max_pages] and [requests])")
     return page_table.shape
@@ -90,10 +107,11 @@ def _table_shape(op: str, page_table: torch.Tensor, lengths: torch.Tensor):
 
 def _pool_shape(op: str, pool: torch.Tensor):
     """(pages, KV heads, page size, head dimension) of a pool [pages, heads, page_size / 16, 18 D]."""
-    if pool.dim() != 4 or pool.shape[3] % 18:
+    shape = pool.shape
+    if len(shape) != 4 or shape[3] % 18:
         raise RuntimeError(f"{op}: a pool is [pages, kv_heads, page_size / {GROUP}, 18 * head_dim], got "
-                           f"{list(pool.shape)}")
-    pages, heads, groups, row = pool.shape
+                           f"{list(shape)}")
+    pages, heads, groups, row = shape
     return pages, heads, groups * GROUP, row // 18
 
 
@@ -116,14 +134,14 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     a call that cannot be met changes nothing, gives no token a slot and sets
     `status` (see `PagedQ4Cache.check`)."""
     op = "kv_pages_resize"
-    device = page_table.device
-    i32 = torch.int32
-    _require_cuda(op, device)
-    _require(op, device, "page_table", page_table, i32)
-    _require(op, device, "lengths", lengths, i32)
-    _require(op, device, "free_pages", free_pages, i32)
-    _require(op, device, "free_count", free_count, i32)
-    _require(op, device, "status", status, i32)
+    device, index = page_table.device, page_table.get_device()
+    if not (index >= 0 and page_table.dtype is lengths.dtype is free_pages.dtype is free_count.dtype is status.dtype is _I32
+            and index == lengths.get_device() == free_pages.get_device() == free_count.get_device() == status.get_device()
+            and page_table.is_contiguous() and lengths.is_contiguous() and free_pages.is_contiguous()):
+        _require_cuda(op, device)
+        for name, t in (("page_table", page_table), ("lengths", lengths), ("free_pages", free_pages),
+                        ("free_count", free_count), ("status", status)):
+            _require(op, device, name, t, _I32)
     requests, max_pages = _table_shape(op, page_table, lengths)
     if free_pages.dim() != 1 or free_count.numel() != 1 or status.numel() != 1:
         raise RuntimeError(f"{op}: free_pages is [pages], free_count and status one number each")
@@ -133,14 +151,14 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     if new_lengths is not None:
         if grow:
             raise RuntimeError(f"{op}: new_lengths or grow, not both")
-        _require(op, device, "new_lengths", new_lengths, i32)
+        _require(op, device, "new_lengths", new_lengths, _I32)
         if new_lengths.shape != lengths.shape:
             raise RuntimeError(f"{op}: new_lengths {list(new_lengths.shape)} do not fit lengths {list(lengths.shape)}")
         new = new_lengths.data_ptr()
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
-    positions = torch.empty(max_tokens, dtype=i32, device=device)
-    query_start = lengths.new_empty(requests + 1)
-    _call(device, N.lib().tn_kv_pages_resize, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
+    slots = _empty(index, _I64, max_tokens)
+    positions = _empty(index, _I32, max_tokens)
+    query_start = _empty(index, _I32, requests + 1)
+    _call(index, N.lib().tn_kv_pages_resize, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
           int(grow), requests, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size,
           slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr())
     return slots, positions, query_start
@@ -158,8 +176,17 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+_contiguous_rows: dict = {}
+
+
 def _row_strides(t: torch.Tensor):
     """Element strides of token and head; a size-1 dimension is never stepped through."""
+    if t.is_contiguous():
+        key = t.shape[1:]
+        strides = _contiguous_rows.get(key)
+        if strides is None:
+            strides = _contiguous_rows[key] = _TwoStrides(key[0] * key[1], key[1])
+        return strides
     token, head, _ = t.stride()
     return _TwoStrides(token if t.shape[0] > 1 else 0, head if t.shape[1] > 1 else 0)
 
@@ -170,22 +197,27 @@ def kv_q4_append(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor, slo
     negative one skips its token), in place. Codes and scales are those of
     `torch._C._quantize(..., "q4_0")`."""
     op = "kv_q4_append"
-    device = pool.device
-    _require_cuda(op, device)
-    _require(op, device, "pool", pool, torch.uint8)
-    _require(op, device, "slots", slots, torch.int64)
+    index = pool.get_device()
+    code = _CODE.get(key.dtype)
+    if not (index >= 0 and pool.dtype is _U8 and slots.dtype is _I64 and code is not None and value.dtype is key.dtype
+            and index == key.get_device() == value.get_device() == slots.get_device() and pool.is_contiguous()
+            and slots.is_contiguous()):
+        device = pool.device
+        _require_cuda(op, device)
+        _require(op, device, "pool", pool, _U8)
+        _require(op, device, "slots", slots, _I64)
+        if code is None or value.dtype != key.dtype:
+            raise NotImplementedError(f"{op}: key and value must both be float32, float16 or bfloat16, got {key.dtype} "
+                                      f"and {value.dtype}")
+        raise RuntimeError(f"{op}: Expected all tensors to be on the same device, but found {device}, {key.device} (key) "
+                           f"and {value.device} (value)")
     pages, heads, page_size, dim = _pool_shape(op, pool)
-    if key.dtype not in _CODE or value.dtype != key.dtype:
-        raise NotImplementedError(f"{op}: key and value must both be float32, float16 or bfloat16, got {key.dtype} and "
-                                  f"{value.dtype}")
-    if key.device != device or value.device != device:
-        raise RuntimeError(f"{op}: Expected all tensors to be on the same device")
-    tokens = slots.shape[0]
-    if slots.dim() != 1 or tuple(key.shape) != (tokens, heads, dim) or key.shape != value.shape:
+    tokens = slots.shape[0] if slots.dim() == 1 else -1
+    if key.shape != (tokens, heads, dim) or key.shape != value.shape:
         raise RuntimeError(f"{op}: key {list(key.shape)}, value {list(value.shape)} and slots {list(slots.shape)} do "
                            f"not fit a pool of {heads} heads of {dim}")
     key, value = _rows(key), _rows(value)
-    _call(device, N.lib().tn_kv_q4_append, key.data_ptr(), value.data_ptr(), _CODE[key.dtype], _row_strides(key),
+    _call(index, N.lib().tn_kv_q4_append, key.data_ptr(), value.data_ptr(), code, _row_strides(key),
           _row_strides(value), tokens, slots.data_ptr(), pool.data_ptr(), pages, heads, dim, page_size)
 
 
@@ -199,36 +231,39 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
     request's are not written. `max_tokens`, a bound on one request's query
     tokens, chooses the kernel (None: all of them)."""
     op = "sdpa_q4_cache"
-    device = query.device
-    _require_cuda(op, device)
-    if query.dtype not in _CODE:
-        raise NotImplementedError(f"{op}: the query must be float32, float16 or bfloat16, got {query.dtype}")
-    _require(op, device, "pool", pool, torch.uint8)
-    _require(op, device, "page_table", page_table, torch.int32)
-    _require(op, device, "lengths", lengths, torch.int32)
+    device, index = query.device, query.get_device()
+    code = _CODE.get(query.dtype)
+    if not (index >= 0 and code is not None and pool.dtype is _U8 and page_table.dtype is lengths.dtype is _I32
+            and index == pool.get_device() == page_table.get_device() == lengths.get_device() and pool.is_contiguous()
+            and page_table.is_contiguous() and lengths.is_contiguous()):
+        _require_cuda(op, device)
+        if code is None:
+            raise NotImplementedError(f"{op}: the query must be float32, float16 or bfloat16, got {query.dtype}")
+        _require(op, device, "pool", pool, _U8)
+        _require(op, device, "page_table", page_table, _I32)
+        _require(op, device, "lengths", lengths, _I32)
     pages, kv_heads, page_size, dim = _pool_shape(op, pool)
     requests, max_pages = _table_shape(op, page_table, lengths)
     if query.dim() != 3 or query.shape[2] != dim:
         raise RuntimeError(f"{op}: query {list(query.shape)} must be [tokens, heads, {dim}]")
-    tokens, heads = query.shape[:2]
-    start = None
+    tokens, heads, _ = query.shape
+    if heads == 0 or heads % kv_heads:
+        raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
+    start, most = None, 1
     if query_start is not None:
-        _require(op, device, "query_start", query_start, torch.int32)
+        _require(op, device, "query_start", query_start, _I32)
         if query_start.numel() != requests + 1:
             raise RuntimeError(f"{op}: query_start must have requests + 1 = {requests + 1} entries, got "
                                f"{query_start.numel()}")
         start = query_start.data_ptr()
-    if heads == 0 or heads % kv_heads:
-        raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
-    most = 1 if start is None else tokens if max_tokens is None else max(1, min(max_tokens, tokens))
+        most = tokens if max_tokens is None else max(1, min(max_tokens, tokens))
     query = _rows(query)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
-    ws = _workspace(device, tokens, heads, kv_heads, dim, most)
-    _call(device, N.lib().tn_sdpa_q4_cache, query.data_ptr(), _CODE[query.dtype], _row_strides(query), tokens, heads,
-          pool.data_ptr(), pages, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages,
-          lengths.data_ptr(), requests, start, most, out.data_ptr(), lse.data_ptr(), 0.0 if scale is None else
-          float(scale), ws.data_ptr(), ws.numel())
+    lse = _empty(index, _F32, tokens, heads)
+    ws = _workspace(device, index, heads // kv_heads * most, dim, tokens, heads, kv_heads, most)
+    _call(index, N.lib().tn_sdpa_q4_cache, query.data_ptr(), code, _row_strides(query), tokens, heads, pool.data_ptr(),
+          pages, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
+          start, most, out.data_ptr(), lse.data_ptr(), 0.0 if scale is None else float(scale), ws.data_ptr(), ws.numel())
     return out, lse
 
 
@@ -242,17 +277,22 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
     heads D / 32]) also receives its planar Q8_0, the next linear's
     activations. A request of length 0 appends nothing and gives zeros."""
     op = "sdpa_q4_decode_step"
-    device = qkv.device
-    _require_cuda(op, device)
-    bf = torch.bfloat16
-    _require(op, device, "qkv", qkv, bf)
-    _require(op, device, "rope", rope, bf)
-    _require(op, device, "pool", pool, torch.uint8)
-    _require(op, device, "page_table", page_table, torch.int32)
-    _require(op, device, "lengths", lengths, torch.int32)
+    device, index = qkv.device, qkv.get_device()
+    if not (index >= 0 and qkv.dtype is rope.dtype is _BF16 and pool.dtype is _U8
+            and page_table.dtype is lengths.dtype is _I32 and index == rope.get_device() == pool.get_device()
+            == page_table.get_device() == lengths.get_device() and qkv.is_contiguous() and rope.is_contiguous()
+            and pool.is_contiguous() and page_table.is_contiguous() and lengths.is_contiguous()):
+        _require_cuda(op, device)
+        _require(op, device, "qkv", qkv, _BF16)
+        _require(op, device, "rope", rope, _BF16)
+        _require(op, device, "pool", pool, _U8)
+        _require(op, device, "page_table", page_table, _I32)
+        _require(op, device, "lengths", lengths, _I32)
     pages, kv_heads, page_size, dim = _pool_shape(op, pool)
     requests, max_pages = _table_shape(op, page_table, lengths)
-    if tuple(qkv.shape) != (requests, (heads + 2 * kv_heads) * dim):
+    if heads <= 0 or heads % kv_heads:
+        raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
+    if qkv.shape != (requests, (heads + 2 * kv_heads) * dim):
         raise RuntimeError(f"{op}: qkv {list(qkv.shape)} must be [{requests}, {(heads + 2 * kv_heads) * dim}]")
     if rope.dim() != 2 or rope.shape[1] != dim:
         raise RuntimeError(f"{op}: rope {list(rope.shape)} must be [positions, {dim}]")
@@ -260,17 +300,15 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
     if q8 is not None:
         codes, scales, offsets = q8
         _require(op, device, "codes", codes, torch.int8)
-        _require(op, device, "scales", scales, torch.float32)
-        _require(op, device, "offsets", offsets, torch.float32)
+        _require(op, device, "scales", scales, _F32)
+        _require(op, device, "offsets", offsets, _F32)
         if codes.numel() != requests * heads * dim or not scales.numel() == offsets.numel() == codes.numel() // 32:
             raise RuntimeError(f"{op}: q8 must be codes [{requests}, {heads * dim}], scales and offsets "
                                f"[{requests}, {heads * dim // 32}]")
         codes, scales, offsets = codes.data_ptr(), scales.data_ptr(), offsets.data_ptr()
-    if heads <= 0 or heads % kv_heads:
-        raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
-    out = torch.empty((requests, heads, dim), dtype=bf, device=device)
-    ws = _workspace(device, requests, heads, kv_heads, dim, 1)
-    _call(device, N.lib().tn_sdpa_q4_decode_step, qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
+    out = _empty(index, _BF16, requests, heads, dim)
+    ws = _workspace(device, index, heads // kv_heads, dim, requests, heads, kv_heads, 1)
+    _call(index, N.lib().tn_sdpa_q4_decode_step, qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
           heads, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
           out.data_ptr(), None, codes, scales, offsets, 0.0 if scale is None else float(scale), ws.data_ptr(),
           ws.numel())
