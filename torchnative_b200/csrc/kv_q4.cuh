@@ -151,22 +151,50 @@ __device__ __forceinline__ uint32_t q4_0_word(const float (&x)[8], float inv, co
 __device__ __forceinline__ float q4_0_scale(float m) { return __fmul_rn(m, -0.125f); }
 __device__ __forceinline__ float q4_0_inverse(float d) { return d != 0.0f ? __frcp_rn(d) : 0.0f; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float y;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 // The element of largest magnitude of a block of 32 held 8 a lane by 4
 // neighbouring lanes in element order; the first of equals, as
-// BlockQ4_0::from_float's loop finds it (NaN never wins its comparison).
+// BlockQ4_0::from_float's loop finds it (NaN never wins its comparison): the
+// block's maximum or its minimum, and only where their magnitudes are the same,
+// which is looked at by the whole warp, the elements one after the other.
 __device__ __forceinline__ float q4_0_extreme(const float (&x)[8]) {
-    float amax = 0.0f, m = 0.0f;
+    float hi = max3(0.0f, x[0], x[1]), lo = min3(0.0f, x[0], x[1]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(x[i]);
-        if (amax < a) amax = a, m = x[i];
+    for (int i = 2; i < 8; i += 2) {
+        hi = max3(hi, x[i], x[i + 1]);
+        lo = min3(lo, x[i], x[i + 1]);
     }
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) {
-        const float oa = __shfl_xor_sync(0xffffffffu, amax, off), om = __shfl_xor_sync(0xffffffffu, m, off);
-        // the lower lane's element comes first: of equals it wins
-        const bool other = (threadIdx.x & off) ? !(oa < amax) : (amax < oa);
-        if (other) amax = oa, m = om;
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    }
+    float m = hi > -lo ? hi : lo;
+    if (__any_sync(0xffffffffu, hi == -lo)) {
+        float amax = 0.0f, first = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = fabsf(x[i]);
+            if (amax < a) amax = a, first = x[i];
+        }
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+            const float oa = __shfl_xor_sync(0xffffffffu, amax, off), om = __shfl_xor_sync(0xffffffffu, first, off);
+            // the lower lane's element comes first: of equals it wins
+            const bool other = (threadIdx.x & off) ? !(oa < amax) : (amax < oa);
+            if (other) amax = oa, first = om;
+        }
+        m = first;
     }
     return m;
 }

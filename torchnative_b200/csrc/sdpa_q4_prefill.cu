@@ -97,12 +97,6 @@ __device__ __forceinline__ uint64_t add2p(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
 // A lane's words of one group (16 tokens): two K vectors (tokens lane / 4 and + 8, t = lane % 4), the two V vectors of
 // elements 8 q .. 8 q + 7 of each block (tokens 8 h + 2 t and + 1; lane = 16 h + 4 q + t), and their scales.
 template <int D>
