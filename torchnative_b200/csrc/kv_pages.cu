@@ -82,7 +82,7 @@ __device__ __forceinline__ int64_t slot_of(const Resize &p, int b, int position)
 __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize p) {
     extern __shared__ int sm[];
     const int B = p.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int *old_len = sm, *new_len = sm + B, *give_at = sm + 2 * B, *take_at = sm + 3 * B, *tok_at = sm + 4 * B;
+    int *old_len = sm, *new_len = sm + B, *give_at = sm + 2 * B, *take_at = give_at + B + 1, *tok_at = take_at + B + 1;
     __shared__ long long warp_sum[3][kThreads / 32];
     __shared__ long long total[3];
     __shared__ int bad_length;
@@ -168,20 +168,42 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
     const int top = top0 + (int)gives;
     if (tid == 0) {
         p.query_start[B] = (int)tokens;
+        give_at[B] = (int)gives;
+        take_at[B] = (int)takes;
         *p.free_count = top - (int)takes;
     }
     __syncthreads();
-    // pages given back, the last one first, so that a roll-back leaves the stack as it was
-    for (int i = tid; i < (int)gives; i += kThreads) {
-        const int b = find(give_at, B, i);
-        const int64_t at = b * p.table_stride + pages_of(new_len[b], p.page_shift) + (i - give_at[b]);
-        p.free_pages[top - 1 - i] = p.table[at];
-        p.table[at] = -1;
+    // Pages given back, the last one first, so that a roll-back leaves the stack as it was; then the pages taken. Of
+    // many, four neighbours a thread: one search, and four loads on their way at once.
+    const int each_give = gives > kThreads ? 4 : 1, each_take = takes > kThreads ? 4 : 1;
+    for (int i0 = tid * each_give; i0 < (int)gives; i0 += kThreads * each_give) {
+        int b = find(give_at, B, i0), page[4];
+        int64_t at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k >= each_give || i0 + k >= (int)gives) continue;
+            while (give_at[b + 1] <= i0 + k) ++b;
+            at[k] = b * p.table_stride + pages_of(new_len[b], p.page_shift) + (i0 + k - give_at[b]);
+            page[k] = p.table[at[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k >= each_give || i0 + k >= (int)gives) continue;
+            p.free_pages[top - 1 - i0 - k] = page[k];
+            p.table[at[k]] = -1;
+        }
     }
     __syncthreads();
-    for (int i = tid; i < (int)takes; i += kThreads) {
-        const int b = find(take_at, B, i);
-        p.table[b * p.table_stride + pages_of(old_len[b], p.page_shift) + (i - take_at[b])] = p.free_pages[top - 1 - i];
+    for (int i0 = tid * each_take; i0 < (int)takes; i0 += kThreads * each_take) {
+        int b = find(take_at, B, i0), page[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) page[k] = k < each_take && i0 + k < (int)takes ? p.free_pages[top - 1 - i0 - k] : -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k >= each_take || i0 + k >= (int)takes) continue;
+            while (take_at[b + 1] <= i0 + k) ++b;
+            p.table[b * p.table_stride + pages_of(old_len[b], p.page_shift) + (i0 + k - take_at[b])] = page[k];
+        }
     }
     if (p.max_tokens > kSlotsInOne) return;
     __syncthreads();
@@ -268,7 +290,7 @@ extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t
     tn::Resize p{page_table, table_stride, (int)max_pages, lengths, new_lengths, (int)grow, (int)requests, free_pages,
                  free_count, (int)num_pages, shift, slots, positions, (int)max_tokens, query_start, status,
                  ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0};
-    const int smem = (int)(5 * requests * sizeof(int));
+    const int smem = (int)((5 * requests + 2) * sizeof(int));
     if (smem > 48 * 1024 - 1024) {
         int st = tn::check_cuda(
             cudaFuncSetAttribute(tn::kv_pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
