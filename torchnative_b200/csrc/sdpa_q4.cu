@@ -435,7 +435,10 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
     constexpr int NB = Q::NB, RT = 8 * NT, W = H::W, STAGES = H::STAGES, THREADS = 32 * W;
     constexpr bool F32 = H::F32, BF = H::BF;
     constexpr int NQ = H::NQ, NP = H::NP;
-    constexpr int COPY_WARPS = STEP ? 2 : 3;  // a decode step has a warp for the new tokens
+    // A decode step has a warp for the new tokens. (No more than stages: a copy warp's last stage, COPY_WARPS before, was free by
+    // the time its turn came, so that the one it waits for now is at most one phase of its barrier behind.)
+    constexpr int COPY_WARPS = STEP ? 2 : 3;
+    static_assert(COPY_WARPS <= STAGES, "a wait tells two phases apart, not three");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full[2], q_empty[2], new_full[2];
     __shared__ uint8_t gone_sm[STAGES][W];  // per unit, a bit for each group without a page
