@@ -47,9 +47,12 @@ namespace {
 constexpr int kMaxGrid = 148;  // CTAs whose parts a workspace holds
 constexpr int kUnitGroups = 2, kUnit = kUnitGroups * kKvGroup;
 constexpr float kBias = 10.0f, kSlack = 5.0f;
-// What an item costs besides its units (queries, the warps' results joined), in units.
-constexpr int kItemCost = 12;
-// A CTA has 2^kMinPlaces places of the line before another one is used.
+// What an item costs besides its units (queries, the warps' results joined), in units: with 8, 12, 16, 20 the ragged
+// batch of 32 up to 8192 tokens (heads of 128, 8 of them) takes 47.6, 43.8, 42.0, 42.1 us, one request of 8192 12.9,
+// 13.0, 12.5, 13.1.
+constexpr int kItemCost = 16;
+// A CTA has 2^kMinPlaces places of the line before another one is used: with 8, 16, 32 of them one request of 2048
+// takes 10.3, 10.7, 13.9 us, 8192 tokens 13.4, 13.0, 15.1.
 constexpr int kMinPlaces = 4;
 
 // What the producer tells the consumers of an item.
@@ -1090,9 +1093,16 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
     }
 }
 
-// The rows of a tile: 8 hold every head that shares a KV head in decode (up to 8); more rows a request make
-// tiles of 16, which read the cache half as often.
+// The most rows that a tile of the call may have, for the size of its workspace.
 int tile_rows(int64_t max_query, int64_t rep) { return max_query * rep <= 8 ? 8 : 16; }
+
+// Whether a request's rows go in tiles of 16 rather than 8. Both read and unpack the cache once a tile; 16 rows cost 1.7
+// to 1.9 times 8 (16 requests at 2055, 8 KV heads of 128, bf16: 20 rows 44.8 us in two tiles of 16, 39.4 in three of 8;
+// 32 rows 45.1 and 48.3; 64 rows 74.2 and 82.5), in float32 with D 128, whose registers spill, twice (32 rows 64.8 and
+// 63.6).
+bool wide_tiles(int64_t rows) {
+    return 7 * ((rows + 15) / 16) <= 4 * ((rows + 7) / 8);
+}
 
 int64_t workspace_bytes(int rows, int64_t dim) { return (int64_t)kMaxGrid * 2 * (rows * (dim + 2) * 4 + 8); }
 
@@ -1152,8 +1162,10 @@ template <typename T, int D>
 int launch_attend(Split &p, int64_t max_query, void *workspace, cudaStream_t stream) {
     if (std::is_same<T, __nv_bfloat16>::value && fills_tiles(p.a.tokens, p.a.c.requests, p.a.c.kv_heads, p.a.rep, max_query))
         return launch_sdpa_q4_prefill(p.a, D, stream);
-    return tile_rows(max_query, p.a.rep) == 8 ? launch_split<T, D, 1, false>(p, workspace, stream, "tn_sdpa_q4_cache")
-                                              : launch_split<T, D, 2, false>(p, workspace, stream, "tn_sdpa_q4_cache");
+    if constexpr (!(sizeof(T) == 4 && D == 128)) {
+        if (wide_tiles(max_query * p.a.rep)) return launch_split<T, D, 2, false>(p, workspace, stream, "tn_sdpa_q4_cache");
+    }
+    return launch_split<T, D, 1, false>(p, workspace, stream, "tn_sdpa_q4_cache");
 }
 
 int check_cache(const char *op, const KvPool &c, int64_t requests, int64_t max_pages, int64_t table_stride,
