@@ -6,13 +6,15 @@
 // rows see nearly the same keys. Key tiles of 64 are unpacked once for both
 // query tiles. 16 warps:
 //   warps 0-3, 4-7   softmax of query tile 0, 1: thread r owns row r (TMEM lane
-//                    r) and all 64 columns of a key tile
-//   warp 8           MMA issuer (one thread): S_k = Q_k K_j^T into TMEM (double
-//                    buffered), then O_k += P_k V_{j-1} one tile behind
+//                    r) and all 64 columns
+//                    of a key tile; before, it puts its row of queries into TMEM
+//   warp 8           MMA issuer (one thread): S_k = Q_k K_j^T (Q from TMEM: with
+//                    16 products a tile its shared-memory reads would bound the
+//                    tensor pipe), then O_k += P_k V_{j-1} one tile behind
 //   warp 9           TMEM owner (512 columns)
-//   warps 12-15      unpack: the queries once, then warp w the w-th group of 16
-//                    tokens of each key tile, from global memory (the next
-//                    tile's words are loaded before this one's are unpacked)
+//   warps 12-15      unpack: warp w the w-th group of 16 tokens of each key tile,
+//                    from global memory (the next tile's words are loaded before
+//                    this one's are unpacked)
 // The products are f16: an element is (code - 8) times its block's scale, the
 // scale taken to [1/2, 1) by a power of two of the group's own, so that nothing
 // overflows; the powers come back in the softmax, those of the keys in the
@@ -35,10 +37,12 @@
 namespace tn {
 namespace {
 
-constexpr int BM = 128, NQT = 2, BN = 64, NK = 2, NV = 3, NINFO = 8;
+constexpr int BM = 128, NQT = 2, BN = 64, NK = 3, NV = 3, NINFO = 8;
 constexpr int THREADS = 16 * 32, SOFTMAX_REGS = 168, OTHER_REGS = 88;
 static_assert(256 * SOFTMAX_REGS + 256 * OTHER_REGS <= THREADS * 128, "what the CTA is launched with");
-constexpr int QPANEL = BM * 128, KPANEL = BN * 128, PTILE = BM * 128;  // rows of 64 16-bit elements
+constexpr int KPANEL = BN * 128, PTILE = BM * 128;  // rows of 64 16-bit elements
+// TMEM columns (512): scores, queries (two f16 a column), results
+constexpr int TS = 0, TQ = 128, TO = 256;
 constexpr float kBias = 10.0f, kSlack = 5.0f;  // a probability is 2^10 at its row's reference, 2^15 at most
 
 // What the unpacking warps say of a key tile, a value for each of its groups.
@@ -51,9 +55,9 @@ struct Info {
 template <int D>
 struct Layout {
     static constexpr int P = D / 64;  // panels of 64 columns
-    static constexpr int QTILE = P * QPANEL, KTILE = P * KPANEL;
-    static constexpr int Q = 0, K = NQT * QTILE, V = K + NK * 2 * KTILE, PR = V + NV * KTILE, INFO = PR + NQT * PTILE,
-                         BACK = INFO + NINFO * (int)sizeof(Info), BAR = BACK + NQT * BM * 4;
+    static constexpr int KTILE = P * KPANEL;
+    static constexpr int K = 0, V = K + NK * 2 * KTILE, PR = V + NV * KTILE, INFO = PR + NQT * PTILE,
+                         BAR = INFO + NINFO * (int)sizeof(Info);
     static constexpr int SMEM = BAR + 512 + 1024;
 };
 
@@ -163,10 +167,9 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sb = smem_u32(base);
     volatile Info *info = reinterpret_cast<volatile Info *>(base + L::INFO);
-    float *back = reinterpret_cast<float *>(base + L::BACK);  // a row's queries' power of two
     uint64_t *bars = reinterpret_cast<uint64_t *>(base + L::BAR);
     uint64_t *q_full = bars, *k_full = q_full + 1, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV,
-             *s_full = v_empty + NV /*[2][2]*/, *s_free = s_full + 4 /*[2][2]*/, *p_full = s_free + 4 /*[2]*/,
+             *s_full = v_empty + NV /*[2]*/, *s_free = s_full + 2 /*[2]*/, *p_full = s_free + 2 /*[2]*/,
              *o_done = p_full + 2 /*[2]*/, *info_full = o_done + 2 /*[NINFO]*/, *mma_done = info_full + NINFO;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -207,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
         }
     }
     if (tid == 32) {
-        mbar_init(q_full, 4);
+        mbar_init(q_full, 8);
         for (int i = 0; i < NK; ++i) {
             mbar_init(&k_full[i], 4);
             mbar_init(&k_empty[i], 1);
@@ -216,11 +219,9 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], 1);
         }
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&s_free[i], 4);
-        }
-        for (int i = 0; i < 2; ++i) {
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
         }
@@ -255,46 +256,6 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
         const int w = warp - 12, *table = a.c.table + b * a.c.table_stride;
         Words<D> x;
         if (ntm > 0) x.load(a.c, table, head, w, S, lane);
-        // queries: four lanes a row, eight rows of a warp at once
-        for (int r0 = w * 8; r0 < NQT * BM; r0 += 32) {
-            const int r = r0 + (lane >> 2), t = lane & 3, row = row_first + r;
-            float q[NB][8];
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[c][i] = 0.0f;
-            if (row < rows) {
-                const int tok = row / a.rep, hq = head * a.rep + row - tok * a.rep;
-                const T *src = static_cast<const T *>(a.q) + (first + tok) * a.q_token + hq * a.q_head;
-#pragma unroll
-                for (int c = 0; c < NB; ++c) load8<T>(src + c * 32 + t * 8, q[c]);
-            }
-            float scale = 1.0f, inv = 1.0f, amax = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(q[c][i]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            if (amax > 0.0f && amax < INFINITY) {  // to [2^13, 2^14)
-                const int e = min(max(267 - (int)(__float_as_uint(amax) >> 23), 1), 253);
-                scale = __uint_as_float((uint32_t)e << 23);
-                inv = __uint_as_float((uint32_t)(254 - e) << 23);
-            }
-            const uint32_t dst = sb + L::Q + (r >> 7) * L::QTILE + (r & 127) * 128;
-#pragma unroll
-            for (int c = 0; c < NB; ++c) {
-                const int chunk = 4 * c + t;
-                st_shared_v4(dst + (chunk >> 3) * QPANEL + (((chunk & 7) ^ (r & 7)) << 4),
-                             pack_f16(q[c][0] * scale, q[c][1] * scale), pack_f16(q[c][2] * scale, q[c][3] * scale),
-                             pack_f16(q[c][4] * scale, q[c][5] * scale), pack_f16(q[c][6] * scale, q[c][7] * scale));
-            }
-            if (t == 0) back[r] = inv;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-
         const int krow = 16 * w + (lane >> 2), t = lane & 3, q = lane >> 2 & 3, vrow = 16 * w + 8 * (lane >> 4) + 2 * t;
         for (int j = 0; j < ntm; ++j) {
             const Words<D> y = x;
@@ -390,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                     const uint32_t pb = sb + L::PR + k * PTILE, vb = sb + L::V + vs * L::KTILE;
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk)
-                        tc05::mma_ss(tmem + 256 + k * 128, tc05::desc_sw128(pb + kk * 32, 16, 1024),
+                        tc05::mma_ss(tmem + TO + k * 128, tc05::desc_sw128(pb + kk * 32, 16, 1024),
                                      tc05::desc_sw128(vb + kk * 2048, KPANEL, 1024), id_pv, (t > 0 || kk > 0) ? 1u : 0u);
                     tc05::commit(&o_done[k]);
                 }
@@ -398,25 +359,23 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                 return true;
             };
             for (int j = 0; j < ntm && ok; ++j) {
-                const int ks = j % NK, buf = j & 1;
+                const int ks = j % NK;
                 if (!wait_or_abort(&k_full[ks], (j / NK) & 1, abort, a.c.err)) break;
                 for (int k = 0; k < NQT && ok; ++k) {
                     if (j >= nt[k]) continue;
-                    if (j >= 2 && !wait_or_abort(&s_free[k * 2 + buf], ((j >> 1) - 1) & 1, abort, a.c.err)) {
+                    if (j >= 1 && !wait_or_abort(&s_free[k], (j - 1) & 1, abort, a.c.err)) {
                         ok = false;
                         break;
                     }
                     tc05::fence_after();
-                    const uint32_t qb = sb + L::Q + k * L::QTILE, kb = sb + L::K + ks * 2 * L::KTILE;
+                    const uint32_t kb = sb + L::K + ks * 2 * L::KTILE;
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t qo = (kk >> 2) * QPANEL + (kk & 3) * 32, ko = (kk >> 2) * KPANEL + (kk & 3) * 32;
-                        tc05::mma_ss(tmem + (k * 2 + buf) * BN, tc05::desc_sw128(qb + qo, 16, 1024),
-                                     tc05::desc_sw128(kb + ko, 16, 1024), id_qk, kk > 0);
-                        tc05::mma_ss(tmem + (k * 2 + buf) * BN, tc05::desc_sw128(qb + qo, 16, 1024),
-                                     tc05::desc_sw128(kb + L::KTILE + ko, 16, 1024), id_qk, 1u);
+                        const uint32_t q = tmem + TQ + k * 64 + kk * 8, ko = (kk >> 2) * KPANEL + (kk & 3) * 32;
+                        tc05::mma_ts(tmem + TS + k * BN, q, tc05::desc_sw128(kb + ko, 16, 1024), id_qk, kk > 0);
+                        tc05::mma_ts(tmem + TS + k * BN, q, tc05::desc_sw128(kb + L::KTILE + ko, 16, 1024), id_qk, 1u);
                     }
-                    tc05::commit(&s_full[k * 2 + buf]);
+                    tc05::commit(&s_full[k]);
                 }
                 tc05::commit(&k_empty[ks]);
                 if (ok && j >= 1) ok = pv(j - 1);
@@ -434,20 +393,58 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
         const int sees = S - n + tok + 1;                                   // keys of this row
         const int all_see = S - n + (row_first + BM * k) / a.rep + 1;       // keys of every row of the tile
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tO = tmem + lane_off + 256 + k * 128;
+        const uint32_t tO = tmem + lane_off + TO + k * 128;
+        // ---- this row's queries, in f16 into TMEM: the largest magnitude taken to [2^13, 2^14) by a power of two
+        float inv_q = 1.0f;
+        {
+            uint4 q[D / 8];
+            const T *src = static_cast<const T *>(a.q) + (first + tok) * a.q_token + (head * a.rep + row - tok * a.rep) * a.q_head;
+            uint32_t most = 0;  // of the magnitudes of a word's two elements (16-bit integers order as they do)
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                q[c] = row < rows ? *reinterpret_cast<const uint4 *>(src + c * 8) : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+            }
+            most = max(most & 0xffffu, most >> 16);
+            float scale = 1.0f;
+            if (most > 0 && most < 0x7f80u) {
+                const int e = min(max(267 - (int)(most >> 7), 1), 253);
+                scale = __uint_as_float((uint32_t)e << 23);
+                inv_q = __uint_as_float((uint32_t)(254 - e) << 23);
+            }
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 x = q[8 * h + c];
+                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[4 * c + i] = __uint_as_float(pack_f16(__uint_as_float(w[i] << 16) * scale,
+                                                                __uint_as_float(w[i] & 0xffff0000u) * scale));
+                }
+                tc05::st32(tmem + lane_off + TQ + k * 64 + h * 32, v);
+            }
+            tc05::wait_st();
+            tc05::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
         float m_used = -INFINITY, l = 0.0f;
-        bool ok = warp_wait(q_full, 0, abort, a.c.err);
+        bool ok = true;
         // p = 2^(s c2 - m); above 0, so that what is masked stays -inf
-        const float c2 = fmaxf(a.scale * 1.4426950408889634f * back[BM * k + r], 1.1754944e-38f);
+        const float c2 = fmaxf(a.scale * 1.4426950408889634f * inv_q, 1.1754944e-38f);
         for (int t = 0; t < nt && ok; ++t) {
-            const int buf = t & 1;
-            if (!warp_wait(&s_full[k * 2 + buf], (t >> 1) & 1, abort, a.c.err) ||
+            if (!warp_wait(&s_full[k], t & 1, abort, a.c.err) ||
                 !warp_wait(&info_full[t % NINFO], (t / NINFO) & 1, abort, a.c.err)) {
                 ok = false;
                 break;
             }
             tc05::fence_after();
-            // (at most four tiles on, the unpacking warps have to wait for this one's scores to be read: the ring of
+            // (at most five tiles on, the unpacking warps have to wait for this one's scores to be read: the ring of
             // eight holds)
             float ck[4], cv[4], ci[4];
             bool full = (t + 1) * BN <= all_see;
@@ -461,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             float sv[64];
             {
                 float v[32];
-                const uint32_t tS = tmem + lane_off + (k * 2 + buf) * BN;
+                const uint32_t tS = tmem + lane_off + TS + k * BN;
                 tc05::ld32(tS, v);
                 tc05::wait_ld();
 #pragma unroll
@@ -473,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             }
             tc05::fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[k * 2 + buf]);
+            if (lane == 0) mbar_arrive(&s_free[k]);
             if (!full) {
 #pragma unroll
                 for (int c = 0; c < 64; ++c)
