@@ -53,9 +53,10 @@ def _require_cuda(op: str, device: torch.device) -> None:
                                   "torchnative's CPU path")
 
 
-def _call(index: int, fn, *args) -> None:
+def _call(index: int, name: str, *args) -> None:
     """One library call on device `index`'s current stream; the library takes
     the current device, which may be another one."""
+    fn = getattr(N.lib(), name)
     if index == _current_device():
         status = fn(*args, _current_stream(index))
     else:
@@ -65,19 +66,22 @@ def _call(index: int, fn, *args) -> None:
         N.check(status)
 
 
+_empty_like, _contiguous = torch.empty_like, torch.contiguous_format
 _templates: dict = {}
 
 
-def _empty(index: int, dtype: torch.dtype, *shape: int) -> torch.Tensor:
-    """torch.empty on device `index`; like a template without memory of its own,
-    it takes half the host's time."""
-    key = (index, dtype, shape)
-    t = _templates.get(key)
+def _empty(dtype: torch.dtype, *place) -> torch.Tensor:
+    """torch.empty on place = (device index, *shape); like a template without
+    memory of its own, it takes half the host's time."""
+    shapes = _templates.get(dtype)
+    if shapes is None:
+        shapes = _templates[dtype] = {}
+    t = shapes.get(place)
     if t is None:
-        if len(_templates) >= 1024:
-            _templates.clear()
-        t = _templates[key] = torch.empty(1, dtype=dtype, device=torch.device("cuda", index)).expand(shape)
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+        if len(shapes) >= 1024:
+            shapes.clear()
+        t = shapes[place] = torch.empty(1, dtype=dtype, device=torch.device("cuda", place[0])).expand(place[1:])
+    return _empty_like(t, memory_format=_contiguous)
 
 
 _scratch: dict = {}
@@ -151,14 +155,15 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     if new_lengths is not None:
         if grow:
             raise RuntimeError(f"{op}: new_lengths or grow, not both")
-        _require(op, device, "new_lengths", new_lengths, _I32)
-        if new_lengths.shape != lengths.shape:
+        if not (new_lengths.dtype is _I32 and new_lengths.get_device() == index and new_lengths.is_contiguous()
+                and new_lengths.shape == lengths.shape):
+            _require(op, device, "new_lengths", new_lengths, _I32)
             raise RuntimeError(f"{op}: new_lengths {list(new_lengths.shape)} do not fit lengths {list(lengths.shape)}")
         new = new_lengths.data_ptr()
-    slots = _empty(index, _I64, max_tokens)
-    positions = _empty(index, _I32, max_tokens)
-    query_start = _empty(index, _I32, requests + 1)
-    _call(index, N.lib().tn_kv_pages_resize, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
+    slots = _empty(_I64, index, max_tokens)
+    positions = _empty(_I32, index, max_tokens)
+    query_start = _empty(_I32, index, requests + 1)
+    _call(index, "tn_kv_pages_resize", page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
           int(grow), requests, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size,
           slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr())
     return slots, positions, query_start
@@ -217,7 +222,7 @@ def kv_q4_append(key: torch.Tensor, value: torch.Tensor, pool: torch.Tensor, slo
         raise RuntimeError(f"{op}: key {list(key.shape)}, value {list(value.shape)} and slots {list(slots.shape)} do "
                            f"not fit a pool of {heads} heads of {dim}")
     key, value = _rows(key), _rows(value)
-    _call(index, N.lib().tn_kv_q4_append, key.data_ptr(), value.data_ptr(), code, _row_strides(key),
+    _call(index, "tn_kv_q4_append", key.data_ptr(), value.data_ptr(), code, _row_strides(key),
           _row_strides(value), tokens, slots.data_ptr(), pool.data_ptr(), pages, heads, dim, page_size)
 
 
@@ -251,17 +256,18 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
         raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
     start, most = None, 1
     if query_start is not None:
-        _require(op, device, "query_start", query_start, _I32)
-        if query_start.numel() != requests + 1:
+        if not (query_start.dtype is _I32 and query_start.get_device() == index and query_start.is_contiguous()
+                and query_start.numel() == requests + 1):
+            _require(op, device, "query_start", query_start, _I32)
             raise RuntimeError(f"{op}: query_start must have requests + 1 = {requests + 1} entries, got "
                                f"{query_start.numel()}")
         start = query_start.data_ptr()
         most = tokens if max_tokens is None else max(1, min(max_tokens, tokens))
     query = _rows(query)
-    out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    lse = _empty(index, _F32, tokens, heads)
+    out = _empty_like(query, memory_format=_contiguous)
+    lse = _empty(_F32, index, tokens, heads)
     ws = _workspace(device, index, heads // kv_heads * most, dim, tokens, heads, kv_heads, most)
-    _call(index, N.lib().tn_sdpa_q4_cache, query.data_ptr(), code, _row_strides(query), tokens, heads, pool.data_ptr(),
+    _call(index, "tn_sdpa_q4_cache", query.data_ptr(), code, _row_strides(query), tokens, heads, pool.data_ptr(),
           pages, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
           start, most, out.data_ptr(), lse.data_ptr(), 0.0 if scale is None else float(scale), ws.data_ptr(), ws.numel())
     return out, lse
@@ -306,9 +312,9 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
             raise RuntimeError(f"{op}: q8 must be codes [{requests}, {heads * dim}], scales and offsets "
                                f"[{requests}, {heads * dim // 32}]")
         codes, scales, offsets = codes.data_ptr(), scales.data_ptr(), offsets.data_ptr()
-    out = _empty(index, _BF16, requests, heads, dim)
+    out = _empty(_BF16, index, requests, heads, dim)
     ws = _workspace(device, index, heads // kv_heads, dim, requests, heads, kv_heads, 1)
-    _call(index, N.lib().tn_sdpa_q4_decode_step, qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
+    _call(index, "tn_sdpa_q4_decode_step", qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
           heads, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
           out.data_ptr(), None, codes, scales, offsets, 0.0 if scale is None else float(scale), ws.data_ptr(),
           ws.numel())
