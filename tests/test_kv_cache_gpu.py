@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from tests.kv_q4_ref import State, check_attention, resize
+from tests.kv_q4_ref import State, attention, check_attention, resize
 from torchnative_b200 import _native as N
 from torchnative_b200 import kv_cache as kv
 from torchnative_b200 import quant
@@ -194,6 +194,21 @@ def test_long_decode_attention(cuda_device, dtype, batch, length, heads, kv_head
     got = kv.sdpa_q4_cache(q, st.pool, st.table, st.lengths, scale=0.3)
     N.device_status()
     check_attention(got, q, st.pool, st.table, st.lengths, 64, scale=0.3)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_float32_sums_over_many_keys(cuda_device, dim):
+    """The error of float32 results on the whole, where a warp sums some hundred groups of keys. A probability is off by
+    2^-21 (its score, exponential and two terms, each 2^-22 or less and random from key to key), which is as much of the
+    result; a group's sum by two roundings, the sum over a hundred groups by sqrt(100) 2^-25, the join of twelve warps by
+    2^-23: 2^-20 together."""
+    st = State([20000], 2, dim, 64, cuda_device, seed=dim)
+    q = st.randn(128, 8, dim)
+    start = starts([128], cuda_device)
+    out, lse = (x.double().cpu() for x in kv.sdpa_q4_cache(q, st.pool, st.table, st.lengths, query_start=start, max_tokens=128))
+    want, want_lse, _, _ = attention(q, st.pool, st.table, st.lengths, 64, start)
+    assert ((out - want).norm() / want.norm()).item() <= 2.0**-20
+    assert ((lse - want_lse).norm() / want_lse.norm()).item() <= 2.0**-20
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
@@ -590,6 +605,36 @@ def test_captured_steps_replay_while_lengths_grow(cuda_device):
         c.check()
 
 
+def test_two_graphs_of_split_attention_at_the_same_time(cuda_device):
+    """Contexts that many CTAs share and join: two graphs captured on one stream, replayed on two, an eager call beside."""
+    states = [State([9000, 3000], 2, 128, 64, cuda_device, seed=i) for i in range(3)]
+    queries = [s.randn(2, 8, 128, dtype=BF) for s in states]
+    want = [kv.sdpa_q4_cache(q, s.pool, s.table, s.lengths) for q, s in zip(queries, states)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for q, s in zip(queries[:2], states):
+        with torch.cuda.stream(side):
+            kv.sdpa_q4_cache(q, s.pool, s.table, s.lengths)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs = [kv.sdpa_q4_cache(q, s.pool, s.table, s.lengths) for _ in range(8)]
+        graphs.append((g, outs))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        torch.cuda.synchronize()
+        for stream, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                g.replay()
+        mine = kv.sdpa_q4_cache(queries[2], states[2].pool, states[2].table, states[2].lengths)
+        torch.cuda.synchronize()
+        for (_, outs), w in zip(graphs, want):
+            assert all(torch.equal(a, b) for o in outs for a, b in zip(o, w))
+        assert all(torch.equal(a, b) for a, b in zip(mine, want[2]))
+    N.device_status()
+
+
 def test_another_stream(cuda_device):
     st = State([900, 33], 2, 128, 64, cuda_device)
     q = st.randn(2, 8, 128, dtype=BF)
@@ -602,6 +647,57 @@ def test_another_stream(cuda_device):
     torch.cuda.synchronize()
     for g in got + other:
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_a_pool_beyond_32_bit_offsets(cuda_device):
+    """5 GB of pages; the requests' lie at its end, and across byte 2^32."""
+    heads, dim, page = 8, 128, 64
+    num = 5 * 2**30 // (heads * page // 16 * 18 * dim)
+    pool = kv.kv_q4_pool(num, heads, dim, page, cuda_device)
+    st = State([130, 200], heads, dim, page, cuda_device)
+    at = 2**32 // (heads * page // 16 * 18 * dim)
+    pages = torch.tensor([num - 1, at, num - 3, at + 1, 0, num - 2, at - 1], dtype=torch.int32, device=cuda_device)
+    k, v = st.randn(330, heads, dim), st.randn(330, heads, dim)
+    table = torch.full((2, 4), -1, dtype=torch.int32, device=cuda_device)
+    table[0, :3], table[1, :4] = pages[:3], pages[3:]
+    pos = torch.cat([torch.arange(130), torch.arange(200)]).to(cuda_device)
+    row = torch.cat([torch.zeros(130), torch.ones(200)]).long().to(cuda_device)
+    slots = table[row, pos // page].long() * page + pos % page
+    assert slots.max() * heads * dim > 2**32 // 2
+    kv.kv_q4_append(k, v, pool, slots)
+    small = kv.kv_q4_pool(7, heads, dim, page, cuda_device)
+    small.copy_(pool[pages.long()])
+    same = torch.where(table >= 0, torch.arange(7, dtype=torch.int32, device=cuda_device)[
+        (table[..., None] == pages).long().argmax(-1)], -1).to(torch.int32)
+    q = st.randn(330, 16, dim, dtype=BF)
+    start = starts([130, 200], cuda_device)
+    for most, x, begin in ((1, q[:2], None), (8, q, start), (200, q, start)):
+        a = kv.sdpa_q4_cache(x, pool, table, st.lengths, query_start=begin, max_tokens=most)
+        b = kv.sdpa_q4_cache(x, small, same, st.lengths, query_start=begin, max_tokens=most)
+        assert all(torch.equal(i, j) for i, j in zip(a, b))
+        check_attention(b, x, small, same, st.lengths, page, begin, tiles=most == 200)
+    N.device_status()
+
+
+def test_an_empty_pool_and_no_rows(cuda_device):
+    pool = kv.kv_q4_pool(0, 2, 64, 16, cuda_device)
+    table = torch.zeros((2, 3), dtype=torch.int32, device=cuda_device)
+    lengths = torch.tensor([0, 20], dtype=torch.int32, device=cuda_device)
+    out, lse = kv.sdpa_q4_cache(torch.ones(2, 4, 64, device=cuda_device), pool, table, lengths)
+    with pytest.raises(RuntimeError, match="page id"):
+        N.device_status()
+    assert (out == 0).all() and (lse == 0).all()
+    x = torch.ones(1, 2, 64, device=cuda_device)
+    kv.kv_q4_append(x, x, pool, torch.zeros(1, dtype=torch.int64, device=cuda_device))
+    with pytest.raises(RuntimeError, match="slot"):
+        N.device_status()
+    kv.kv_q4_append(x[:0], x[:0], pool, torch.zeros(0, dtype=torch.int64, device=cuda_device))
+    start = torch.zeros(3, dtype=torch.int32, device=cuda_device)
+    out, lse = kv.sdpa_q4_cache(torch.ones(0, 4, 64, device=cuda_device), pool, table, lengths, query_start=start)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    none = kv.sdpa_q4_cache(torch.ones(3, 4, 64, device=cuda_device), pool, table, lengths, query_start=start)
+    assert none[0].shape == (3, 4, 64)  # rows of no request: not written
+    N.device_status()
 
 
 def test_refusals(cuda_device):
