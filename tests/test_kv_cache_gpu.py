@@ -28,7 +28,7 @@ def as_lists(cache):
 
 
 @pytest.mark.parametrize("requests, page_size, seed", [(1, 16, 0), (3, 64, 1), (33, 32, 2), (700, 16, 3), (1025, 128, 4),
-                                                       (2600, 16, 5)])
+                                                       (2600, 16, 5), (5000, 32, 6)])
 def test_resize_matches_plain(cuda_device, requests, page_size, seed):
     rng = random.Random(seed)
     width = 5
@@ -83,6 +83,27 @@ def test_resize_that_cannot_be_met_changes_nothing(cuda_device, new, tokens, cod
     cache.resize(64, grow=1)  # and the next one goes on
     assert cache.lengths.tolist() == [21, 0, 17]
     cache.check()
+
+
+@pytest.mark.parametrize("requests, width", [(3, 6000), (40, 500), (700, 24)])
+def test_resize_of_wide_tables(cuda_device, requests, width):
+    """Tables in which more pages may move than one CTA moves: long prompts in, some out, one that is refused, back."""
+    rng = random.Random(requests)
+    cache = kv.PagedQ4Cache(1, 1, 64, requests * width // 2, requests, width, 16, cuda_device)
+    lengths = [rng.randint(0, width * 12) for _ in range(requests)]
+    if requests == 3:
+        lengths = [width * 15 + 3, 17, width * 7]
+    for new, code in ((lengths, 0), ([0 if i % 3 == 0 else n // (1 + i % 2) for i, n in enumerate(lengths)], 0),
+                      ([width * 16] * requests, 1), ([width * 16 + 1] * requests, 2), (lengths, 0), ([0] * requests, 0)):
+        old = as_lists(cache)
+        tokens = sum(max(0, n - o) for o, n in zip(old[1], new)) + 5
+        got = cache.resize(tokens, new_lengths=torch.tensor(new, dtype=torch.int32, device=cuda_device))
+        want = resize(*old, new, 16, tokens)
+        assert want[7] == code
+        assert as_lists(cache) == (want[0], want[1], want[2], want[3])
+        assert tuple(x.tolist() for x in got) == (want[4], want[5], want[6])
+        assert cache.status.item() == code
+        cache.status.zero_()
 
 
 def test_resize_refuses_a_corrupt_stack(cuda_device):

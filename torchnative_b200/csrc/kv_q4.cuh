@@ -87,8 +87,9 @@ struct KvPool {
 // dependent launch): every kernel of the cache waits for that kernel's memory
 // itself, before it reads or writes anything.
 template <typename K, typename... Args>
-int launch_pdl(K kernel, dim3 grid, dim3 block, int smem, cudaStream_t stream, const char *what, Args... args) {
-    cudaLaunchAttribute attr[1];
+int launch_pdl_cluster(K kernel, dim3 grid, dim3 block, int smem, cudaStream_t stream, const char *what, int cluster,
+                       Args... args) {
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
@@ -97,8 +98,15 @@ int launch_pdl(K kernel, dim3 grid, dim3 block, int smem, cudaStream_t stream, c
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what, "cudaLaunchKernelEx");
+}
+template <typename K, typename... Args>
+int launch_pdl(K kernel, dim3 grid, dim3 block, int smem, cudaStream_t stream, const char *what, Args... args) {
+    return launch_pdl_cluster(kernel, grid, block, smem, stream, what, 1, args...);
 }
 
 int check_kv_pool(const char *op, const void *pool, int64_t num_pages, int64_t kv_heads, int64_t head_dim,
