@@ -383,9 +383,9 @@ TN_API int tn_sdpa_decode_step_q8(const void *qkv, const float *inv_freq, void *
 /* Bytes of one page of one layer (-1 on a bad argument). */
 TN_API int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t page_size);
 
-/* Block tables and slot maps from request lengths, in one launch: takes every
- * request from lengths[b] tokens to new_lengths[b] (device, not `lengths`
- * itself), or, with new_lengths NULL, every request that has tokens to grow more.
+/* Block tables and slot maps from request lengths: takes every request from
+ * lengths[b] tokens to new_lengths[b] (device, not `lengths` itself), or, with
+ * new_lengths NULL, every request that has tokens to grow more.
  * A request that shrinks gives its last pages back on the stack free_pages[0,
  * *free_count), one that grows takes from its top; stack order is such that
  * undoing a call restores the table and the stack. Then, for the new tokens

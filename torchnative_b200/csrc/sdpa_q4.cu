@@ -23,12 +23,19 @@ namespace {
 // of G takes the c-th part of the line: every CTA gets as much whatever the
 // lengths, which only the device knows.
 //
-// A CTA is W consumer warps and a producer warp, one CTA an SM. Unit i of a CTA
-// goes to warp i mod W, through stage i / W of a ring that the producer's bulk
-// copies fill; a stage is filled again when every warp is through with
-// it, so that the warps stay together: without that bound the SM's scheduler let
-// some run ahead, and the last ones ended alone (127 us of 82 at 2 x 100,000
-// tokens of 8 heads). The producer also prepares each item's queries.
+// A CTA is W consumer warps and four producer warps, one CTA an SM. Unit i of a
+// CTA goes to warp i mod W, through stage i / W of a ring that the copy warps'
+// bulk copies fill (three of them, in a decode step two: one's copies were issued
+// too slowly for twelve consumers; the third then brings the new tokens); a stage
+// is filled again when every warp is through with it, so that the warps stay
+// together: without that bound the SM's scheduler let some run ahead, and the
+// last ones ended alone (127 us for 82 at 2 x 100,000 tokens of 8 heads, then).
+// The first producer warp prepares each item's queries.
+//
+// What bounds it: instruction issue, ~550 instructions a unit (bf16, D 128) at
+// 0.6 to 0.69 a cycle and scheduler; 2 x 100,000 tokens of 8 heads of 128 take 57
+// us, 4.05 TB/s, 62% of a copy's rate; one request of 2048 10.4 us, nearly all of
+// it latency: ~3 us to the first products, ~4 us for the join.
 //
 // Per 16 tokens a warp computes, with m16n8k16 tensor instructions,
 //   S^T[16 tokens, 8 rows] = sum over blocks b of d_k[token, b] * (codes_b . q_b)

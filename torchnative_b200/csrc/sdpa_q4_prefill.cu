@@ -26,7 +26,9 @@
 // over. For f16 results those roundings would be as large as the result's: they
 // take the other kernel.)
 // What bounds it: the softmax warps' instructions, as in the dense kernel, and
-// the unpacking beside them on the same schedulers; the tensor pipe waits.
+// the unpacking beside them on the same schedulers, ~3800 cycles a key tile of
+// which the tensor pipe works a third. 2 x 1536 tokens at 9728, 32/8 heads of 128:
+// 1010 us, 447 TFLOP/s, of which the last wave of items (384 on 148 SMs) an eighth.
 // Every wait is bounded; one that gives up raises a CTA-wide abort flag.
 #include <algorithm>
 #include <atomic>
