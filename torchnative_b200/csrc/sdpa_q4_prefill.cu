@@ -39,12 +39,12 @@
 namespace tn {
 namespace {
 
-constexpr int BM = 128, NQT = 2, BN = 64, NK = 3, NV = 3, NINFO = 8;
+constexpr int BM = 128, NQT = 2, BN = 64, NK = 2, NV = 2, NINFO = 8;
 constexpr int THREADS = 16 * 32, SOFTMAX_REGS = 168, OTHER_REGS = 88;
 static_assert(256 * SOFTMAX_REGS + 256 * OTHER_REGS <= THREADS * 128, "what the CTA is launched with");
 constexpr int KPANEL = BN * 128, PTILE = BM * 128;  // rows of 64 16-bit elements
-// TMEM columns (512): scores, queries (two f16 a column), results
-constexpr int TS = 0, TQ = 128, TO = 256;
+// TMEM columns (512): scores (the keys' high terms, their low ones), results
+constexpr int TS = 0, TO = 256;
 constexpr float kBias = 10.0f, kSlack = 5.0f;  // a probability is 2^10 at its row's reference, 2^15 at most
 
 // What the unpacking warps say of a key tile, a value for each of its groups.
@@ -58,7 +58,7 @@ template <int D>
 struct Layout {
     static constexpr int P = D / 64;  // panels of 64 columns
     static constexpr int KTILE = P * KPANEL;
-    static constexpr int K = 0, V = K + NK * 2 * KTILE, PR = V + NV * KTILE, INFO = PR + NQT * PTILE,
+    static constexpr int Q = 0, K = Q + NQT * P * PTILE, V = K + NK * 2 * KTILE, PR = V + NV * KTILE, INFO = PR + NQT * PTILE,
                          BAR = INFO + NINFO * (int)sizeof(Info);
     static constexpr int SMEM = BAR + 512 + 1024;
 };
@@ -299,9 +299,9 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                         lo[k] = fma_f16x2(e[k], d, hi[k] ^ 0x80008000u);
                     }
                     const int chunk = 4 * c + t;
-                    const uint32_t at = dst + (chunk >> 3) * KPANEL + (((chunk & 7) ^ (krow & 7)) << 4);
+                    const uint32_t at = dst + (chunk >> 3) * 2 * KPANEL + (((chunk & 7) ^ (krow & 7)) << 4);
                     st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
-                    st_shared_v4(at + L::KTILE, lo[0], lo[1], lo[2], lo[3]);
+                    st_shared_v4(at + KPANEL, lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             fence_proxy_async_smem();
@@ -337,53 +337,57 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
         }
     } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp == 8 && lane == 0) {
-            // ---------------- MMA issuer
-            const uint32_t id_qk = tc05::idesc_f16(false, BM, BN, false);
+        if (warp == 8) {
+            // ---------------- MMA issuer: the whole warp comes along, its first lane's instructions count
+            const uint32_t one = lane == 0;
+            const uint32_t id_qk = tc05::idesc_f16(false, BM, 2 * BN, false);
             const uint32_t id_pv = tc05::idesc_f16(false, BM, D, true);
             const int nt[2] = {nt0, nt1};
-            bool ok = wait_or_abort(q_full, 0, abort, a.c.err);
+            bool ok = warp_wait(q_full, 0, abort, a.c.err);
+            const uint64_t q_desc = tc05::desc_sw128(sb + L::Q, 16, 1024);
+            const uint64_t k_desc = tc05::desc_sw128(sb + L::K, 16, 1024), p_desc = tc05::desc_sw128(sb + L::PR, 16, 1024),
+                           v_desc = tc05::desc_sw128(sb + L::V, KPANEL, 1024);
             auto pv = [&](int t) -> bool {
                 const int vs = t % NV;
-                if (!wait_or_abort(&v_full[vs], (t / NV) & 1, abort, a.c.err)) return false;
+                if (!warp_wait(&v_full[vs], (t / NV) & 1, abort, a.c.err)) return false;
                 for (int k = 0; k < NQT; ++k) {
                     if (t >= nt[k]) continue;
-                    if (!wait_or_abort(&p_full[k], t & 1, abort, a.c.err)) return false;
+                    if (!warp_wait(&p_full[k], t & 1, abort, a.c.err)) return false;
                     tc05::fence_after();
-                    const uint32_t pb = sb + L::PR + k * PTILE, vb = sb + L::V + vs * L::KTILE;
+                    const uint64_t pd = p_desc + (k * PTILE >> 4), vd = v_desc + (vs * L::KTILE >> 4);
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk)
-                        tc05::mma_ss(tmem + TO + k * 128, tc05::desc_sw128(pb + kk * 32, 16, 1024),
-                                     tc05::desc_sw128(vb + kk * 2048, KPANEL, 1024), id_pv, (t > 0 || kk > 0) ? 1u : 0u);
-                    tc05::commit(&o_done[k]);
+                        tc05::mma_ss_if(one, tmem + TO + k * 128, pd + (kk * 32 >> 4), vd + (kk * 2048 >> 4), id_pv,
+                                        (t > 0 || kk > 0) ? 1u : 0u);
+                    tc05::commit_if(one, &o_done[k]);
                 }
-                tc05::commit(&v_empty[vs]);
+                tc05::commit_if(one, &v_empty[vs]);
                 return true;
             };
             for (int j = 0; j < ntm && ok; ++j) {
                 const int ks = j % NK;
-                if (!wait_or_abort(&k_full[ks], (j / NK) & 1, abort, a.c.err)) break;
+                if (!warp_wait(&k_full[ks], (j / NK) & 1, abort, a.c.err)) break;
                 for (int k = 0; k < NQT && ok; ++k) {
                     if (j >= nt[k]) continue;
-                    if (j >= 1 && !wait_or_abort(&s_free[k], (j - 1) & 1, abort, a.c.err)) {
+                    if (j >= 1 && !warp_wait(&s_free[k], (j - 1) & 1, abort, a.c.err)) {
                         ok = false;
                         break;
                     }
                     tc05::fence_after();
-                    const uint32_t kb = sb + L::K + ks * 2 * L::KTILE;
+                    const uint64_t kd = k_desc + (ks * 2 * L::KTILE >> 4);
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t q = tmem + TQ + k * 64 + kk * 8, ko = (kk >> 2) * KPANEL + (kk & 3) * 32;
-                        tc05::mma_ts(tmem + TS + k * BN, q, tc05::desc_sw128(kb + ko, 16, 1024), id_qk, kk > 0);
-                        tc05::mma_ts(tmem + TS + k * BN, q, tc05::desc_sw128(kb + L::KTILE + ko, 16, 1024), id_qk, 1u);
+                        const uint32_t p = kk >> 2, at = kk & 3;
+                        tc05::mma_ss_if(one, tmem + TS + k * 2 * BN, q_desc + (((k * L::P + p) * PTILE + at * 32) >> 4),
+                                        kd + ((p * 2 * KPANEL + at * 32) >> 4), id_qk, kk > 0);
                     }
-                    tc05::commit(&s_full[k]);
+                    tc05::commit_if(one, &s_full[k]);
                 }
-                tc05::commit(&k_empty[ks]);
+                tc05::commit_if(one, &k_empty[ks]);
                 if (ok && j >= 1) ok = pv(j - 1);
             }
             if (ok && ntm > 0) pv(ntm - 1);
-            tc05::commit(mma_done);
+            tc05::commit_if(one, mma_done);
             if (!mbar_wait(mma_done, 0)) record_device_error(a.c.err, DEV_ERR_DRAIN);
         }
     } else {
@@ -417,21 +421,15 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                 inv_q = __uint_as_float((uint32_t)(254 - e) << 23);
             }
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-                float v[32];
+            for (int c = 0; c < D / 8; ++c) {
+                const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+                uint32_t v[4];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const uint4 x = q[8 * h + c];
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        v[4 * c + i] = __uint_as_float(pack_f16(__uint_as_float(w[i] << 16) * scale,
-                                                                __uint_as_float(w[i] & 0xffff0000u) * scale));
-                }
-                tc05::st32(tmem + lane_off + TQ + k * 64 + h * 32, v);
+                for (int i = 0; i < 4; ++i)
+                    v[i] = pack_f16(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale);
+                st_shared_v4(sb + L::Q + (k * L::P + (c >> 3)) * PTILE + r * 128 + (((c & 7) ^ (r & 7)) << 4), v[0], v[1], v[2], v[3]);
             }
-            tc05::wait_st();
-            tc05::fence_before();
+            fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
@@ -459,16 +457,16 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             }
             float sv[64];
             {
-                float v[32];
-                const uint32_t tS = tmem + lane_off + TS + k * BN;
-                tc05::ld32(tS, v);
-                tc05::wait_ld();
+                float hi[32], lo[32];
+                const uint32_t tS = tmem + lane_off + TS + k * 2 * BN;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sv[i] = v[i];
-                tc05::ld32(tS + 32, v);
-                tc05::wait_ld();
+                for (int h = 0; h < 2; ++h) {
+                    tc05::ld32(tS + 32 * h, hi);
+                    tc05::ld32(tS + BN + 32 * h, lo);
+                    tc05::wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sv[32 + i] = v[i];
+                    for (int i = 0; i < 32; i += 2) upk2(add2p(pk2(hi[i], hi[i + 1]), pk2(lo[i], lo[i + 1])), sv[32 * h + i], sv[32 * h + i + 1]);
+                }
             }
             tc05::fence_before();
             __syncwarp();
