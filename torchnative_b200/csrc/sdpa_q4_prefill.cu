@@ -39,7 +39,7 @@
 namespace tn {
 namespace {
 
-constexpr int BM = 128, NQT = 2, BN = 64, NK = 2, NV = 2, NINFO = 8;
+constexpr int BM = 128, NQT = 2, BN = 64, NK = 2, NV = 3, NINFO = 8, UNPACKERS = 7;
 constexpr int THREADS = 16 * 32, SOFTMAX_REGS = 168, OTHER_REGS = 88;
 static_assert(256 * SOFTMAX_REGS + 256 * OTHER_REGS <= THREADS * 128, "what the CTA is launched with");
 constexpr int KPANEL = BN * 128, PTILE = BM * 128;  // rows of 64 16-bit elements
@@ -103,20 +103,21 @@ __device__ __forceinline__ uint64_t add2p(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-// A lane's words of one group (16 tokens): two K vectors (tokens lane / 4 and + 8, t = lane % 4), the two V vectors of
-// elements 8 q .. 8 q + 7 of each block (tokens 8 h + 2 t and + 1; lane = 16 h + 4 q + t), and their scales.
+// A lane's codes and scales of the keys, or of the values, of one group (16 tokens). Keys: two vectors, tokens lane / 4
+// and + 8, t = lane % 4. Values: the two vectors of elements 8 q .. 8 q + 7 of each block, tokens 8 h + 2 t and + 1;
+// lane = 16 h + 4 q + t.
 template <int D>
 struct Words {
-    uint32_t k[2][D / 32], v[2][D / 32], ks[2][D / 64], vs[D / 32];
+    uint32_t codes[2][D / 32], scales[2][D / 64];
     bool gone;
 
-    __device__ __forceinline__ void load(const KvPool &c, const int *row, int head, int group, int S, int lane) {
+    __device__ __forceinline__ void load(const KvPool &c, const int *row, int head, int group, bool values, int S, int lane) {
         using Q = KvQ4<D>;
         constexpr int NB = D / 32;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) k[0][b] = k[1][b] = v[0][b] = v[1][b] = vs[b] = 0;
+        for (int b = 0; b < NB; ++b) codes[0][b] = codes[1][b] = 0;
 #pragma unroll
-        for (int b = 0; b < NB / 2; ++b) ks[0][b] = ks[1][b] = 0;
+        for (int b = 0; b < NB / 2; ++b) scales[0][b] = scales[1][b] = 0;
         gone = false;
         if (group * kKvGroup >= S) return;
         const uint8_t *src = c.group_of_row<D>(row, head, group);
@@ -125,25 +126,17 @@ struct Words {
         const int t = lane & 3, q = lane >> 2 & 3, h = lane >> 4, left = S - group * kKvGroup;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int key = (lane >> 2) + 8 * i;
-            const uint8_t *kp = src + Q::K_CODES + key * (D / 2) + t * NB * 4;
-            const uint8_t *vp = src + Q::V_CODES + h * 4 * D + ((2 * q + i) * 4 + t) * NB * 4;
-            if constexpr (NB == 4) {
-                *reinterpret_cast<uint4 *>(k[i]) = *reinterpret_cast<const uint4 *>(kp);
-                *reinterpret_cast<uint4 *>(v[i]) = *reinterpret_cast<const uint4 *>(vp);
-                if (key < left) *reinterpret_cast<uint2 *>(ks[i]) = *reinterpret_cast<const uint2 *>(src + Q::k_scale(key, 0));
-            } else {
-                *reinterpret_cast<uint2 *>(k[i]) = *reinterpret_cast<const uint2 *>(kp);
-                *reinterpret_cast<uint2 *>(v[i]) = *reinterpret_cast<const uint2 *>(vp);
-                if (key < left) ks[i][0] = *reinterpret_cast<const uint32_t *>(src + Q::k_scale(key, 0));
-            }
+            const int token = values ? 8 * h + 2 * t + i : (lane >> 2) + 8 * i;
+            const uint8_t *p = src + (values ? Q::V_CODES + h * 4 * D + ((2 * q + i) * 4 + t) * NB * 4
+                                             : Q::K_CODES + token * (D / 2) + t * NB * 4);
+            const uint8_t *d = src + (values ? Q::v_scale(token, 0) : Q::k_scale(token, 0));
             // what lies behind the last token may be anything: its scales are 0
-            const int token = 8 * h + 2 * t + i;
-            if (token < left) {
-                if constexpr (NB == 4)
-                    *reinterpret_cast<uint2 *>(vs + 2 * i) = *reinterpret_cast<const uint2 *>(src + Q::v_scale(token, 0));
-                else
-                    vs[i] = *reinterpret_cast<const uint32_t *>(src + Q::v_scale(token, 0));
+            if constexpr (NB == 4) {
+                *reinterpret_cast<uint4 *>(codes[i]) = *reinterpret_cast<const uint4 *>(p);
+                if (token < left) *reinterpret_cast<uint2 *>(scales[i]) = *reinterpret_cast<const uint2 *>(d);
+            } else {
+                *reinterpret_cast<uint2 *>(codes[i]) = *reinterpret_cast<const uint2 *>(p);
+                if (token < left) scales[i][0] = *reinterpret_cast<const uint32_t *>(d);
             }
         }
     }
@@ -227,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
         }
-        for (int i = 0; i < NINFO; ++i) mbar_init(&info_full[i], 4);
+        for (int i = 0; i < NINFO; ++i) mbar_init(&info_full[i], 8);
         mbar_init(mma_done, 1);
         *abort = 0;
         fence_mbar_init();
@@ -252,143 +245,149 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
     };
     const int nt0 = tiles_of(0), nt1 = tiles_of(1), ntm = max(nt0, nt1);
 
-    if (warp >= 12) {
+    if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        // ---------------- unpack
-        const int w = warp - 12, *table = a.c.table + b * a.c.table_stride;
-        Words<D> x;
-        if (ntm > 0) x.load(a.c, table, head, w, S, lane);
-        const int krow = 16 * w + (lane >> 2), t = lane & 3, q = lane >> 2 & 3, vrow = 16 * w + 8 * (lane >> 4) + 2 * t;
-        for (int j = 0; j < ntm; ++j) {
-            const Words<D> y = x;
-            if (j + 1 < ntm) x.load(a.c, table, head, 4 * (j + 1) + w, S, lane);
-            // the group's powers of two
-            int ek = 1, ev = 1;
+        if (warp >= 9) {
+            // ---------------- unpack: a key tile is eight pieces, the keys and the values of its four groups, and the pieces
+            // go to the seven warps in turn. A piece waits only for what pieces before it make possible. A parity names a phase
+            // only to a warp that knows the one before to be over: its last piece, seven back, tells it. That was a tile's
+            // K_1 .. V_3 before, so S_{j-3} or PV_{j-4} is over, or K_0 of the same tile, so S_{j-2} and PV_{j-3}, which
+            // was issued before it; and the phases before the ones waited for are S_{j-4} and PV_{j-6}.
+            static_assert(UNPACKERS == 7 && NK == 2 && NV == 3, "or the above has to be shown again");
+            const int *table = a.c.table + b * a.c.table_stride;
+            const int t = lane & 3, q = lane >> 2 & 3, pieces = 8 * ntm;
+            Words<D> x;
+            auto load = [&](int piece) { x.load(a.c, table, head, 4 * (piece >> 3) + (piece & 3), piece & 4, S, lane); };
+            if (warp - 9 < pieces) load(warp - 9);
+            for (int piece = warp - 9; piece < pieces; piece += UNPACKERS) {
+                const Words<D> y = x;
+                if (piece + UNPACKERS < pieces) load(piece + UNPACKERS);
+                const int j = piece >> 3, w = piece & 3, slot = j % NINFO, ks = j % NK, vs = j % NV;
+                // the group's power of two
+                int e = 1;
 #pragma unroll
-            for (int c = 0; c < NB / 2; ++c) ek = most_exponent(most_exponent(ek, y.ks[0][c]), y.ks[1][c]);
-#pragma unroll
-            for (int c = 0; c < NB; ++c) ev = most_exponent(ev, y.vs[c]);
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                ek = max(ek, __shfl_xor_sync(0xffffffffu, ek, off));
-                ev = max(ev, __shfl_xor_sync(0xffffffffu, ev, off));
-            }
-            ek = min(ek, 30);
-            ev = min(ev, 30);
-            const int slot = j % NINFO, ks = j % NK, vs = j % NV;
-            if (j >= NK && !warp_wait(&k_empty[ks], (j / NK - 1) & 1, abort, a.c.err)) break;
-            if (lane == 0) {
-                info[slot].k[w] = y.gone ? -1.0f : __uint_as_float((uint32_t)(ek + 113) << 23);
-                info[slot].v[w] = (float)(ev - 14);
-                info[slot].vinv[w] = __uint_as_float((uint32_t)(141 - ev) << 23);
-                mbar_arrive(&info_full[slot]);
-            }
-            const uint32_t kpow = power_f16x2(ek), vpow = power_f16x2(ev);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t dst = sb + L::K + ks * 2 * L::KTILE + (krow + 8 * i) * 128;
-#pragma unroll
-                for (int c = 0; c < NB; ++c) {
-                    const uint32_t d = mul_f16x2(__byte_perm(y.ks[i][c / 2], 0, c & 1 ? 0x3232 : 0x1010), kpow);
-                    uint32_t e[4];
-                    unpack_codes<false>(y.k[i][c], e, f16_1024, f16_64);
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        hi[k] = mul_f16x2(e[k], d);
-                        lo[k] = fma_f16x2(e[k], d, hi[k] ^ 0x80008000u);
+                for (int c = 0; c < NB / 2; ++c) e = most_exponent(most_exponent(e, y.scales[0][c]), y.scales[1][c]);
+                e = min((int)__reduce_max_sync(0xffffffffu, (unsigned)e), 30);
+                const uint32_t power = power_f16x2(e);
+                if (!(piece & 4)) {
+                    if (j >= NK && !warp_wait(&k_empty[ks], (j / NK - 1) & 1, abort, a.c.err)) break;
+                    if (lane == 0) {
+                        info[slot].k[w] = y.gone ? -1.0f : __uint_as_float((uint32_t)(e + 113) << 23);
+                        mbar_arrive(&info_full[slot]);
                     }
-                    const int chunk = 4 * c + t;
-                    const uint32_t at = dst + (chunk >> 3) * 2 * KPANEL + (((chunk & 7) ^ (krow & 7)) << 4);
-                    st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
-                    st_shared_v4(at + KPANEL, lo[0], lo[1], lo[2], lo[3]);
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[ks]);
-
-            if (j >= NV && !warp_wait(&v_empty[vs], (j / NV - 1) & 1, abort, a.c.err)) break;
-            const uint32_t dst = sb + L::V + vs * L::KTILE + vrow * 128;
+                    const int krow = 16 * w + (lane >> 2);
 #pragma unroll
-            for (int c = 0; c < NB; ++c) {
-                // the block's scales of the two tokens
-                const uint32_t d = mul_f16x2(__byte_perm(y.vs[c / 2], y.vs[NB / 2 + c / 2], c & 1 ? 0x7632 : 0x5410), vpow);
-                uint32_t e0[4], e1[4];
-                unpack_codes<false>(y.v[0][c], e0, f16_1024, f16_64);
-                unpack_codes<false>(y.v[1][c], e1, f16_1024, f16_64);
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t dst = sb + L::K + ks * 2 * L::KTILE + (krow + 8 * i) * 128;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e0[i] = mul_f16x2(e0[i], d);
-                    e1[i] = mul_f16x2(e1[i], d);
-                }
-                const int chunk = 4 * c + q;
-                const uint32_t at = dst + (chunk >> 3) * KPANEL;
-                st_shared_v4(at + (((chunk & 7) ^ (vrow & 7)) << 4), __byte_perm(e0[0], e0[1], 0x5410),
-                             __byte_perm(e0[2], e0[3], 0x5410), __byte_perm(e1[0], e1[1], 0x5410),
-                             __byte_perm(e1[2], e1[3], 0x5410));
-                st_shared_v4(at + 128 + (((chunk & 7) ^ ((vrow + 1) & 7)) << 4), __byte_perm(e0[0], e0[1], 0x7632),
-                             __byte_perm(e0[2], e0[3], 0x7632), __byte_perm(e1[0], e1[1], 0x7632),
-                             __byte_perm(e1[2], e1[3], 0x7632));
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[vs]);
-        }
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp == 8) {
-            // ---------------- MMA issuer: the whole warp comes along, its first lane's instructions count
-            const uint32_t one = lane == 0;
-            const uint32_t id_qk = tc05::idesc_f16(false, BM, 2 * BN, false);
-            const uint32_t id_pv = tc05::idesc_f16(false, BM, D, true);
-            const int nt[2] = {nt0, nt1};
-            bool ok = warp_wait(q_full, 0, abort, a.c.err);
-            const uint64_t q_desc = tc05::desc_sw128(sb + L::Q, 16, 1024);
-            const uint64_t k_desc = tc05::desc_sw128(sb + L::K, 16, 1024), p_desc = tc05::desc_sw128(sb + L::PR, 16, 1024),
-                           v_desc = tc05::desc_sw128(sb + L::V, KPANEL, 1024);
-            auto pv = [&](int t) -> bool {
-                const int vs = t % NV;
-                if (!warp_wait(&v_full[vs], (t / NV) & 1, abort, a.c.err)) return false;
-                for (int k = 0; k < NQT; ++k) {
-                    if (t >= nt[k]) continue;
-                    if (!warp_wait(&p_full[k], t & 1, abort, a.c.err)) return false;
-                    tc05::fence_after();
-                    const uint64_t pd = p_desc + (k * PTILE >> 4), vd = v_desc + (vs * L::KTILE >> 4);
+                        for (int c = 0; c < NB; ++c) {
+                            const uint32_t d = mul_f16x2(__byte_perm(y.scales[i][c / 2], 0, c & 1 ? 0x3232 : 0x1010), power);
+                            uint32_t e4[4];
+                            unpack_codes<false>(y.codes[i][c], e4, f16_1024, f16_64);
+                            uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int kk = 0; kk < BN / 16; ++kk)
-                        tc05::mma_ss_if(one, tmem + TO + k * 128, pd + (kk * 32 >> 4), vd + (kk * 2048 >> 4), id_pv,
-                                        (t > 0 || kk > 0) ? 1u : 0u);
-                    tc05::commit_if(one, &o_done[k]);
-                }
-                tc05::commit_if(one, &v_empty[vs]);
-                return true;
-            };
-            for (int j = 0; j < ntm && ok; ++j) {
-                const int ks = j % NK;
-                if (!warp_wait(&k_full[ks], (j / NK) & 1, abort, a.c.err)) break;
-                for (int k = 0; k < NQT && ok; ++k) {
-                    if (j >= nt[k]) continue;
-                    if (j >= 1 && !warp_wait(&s_free[k], (j - 1) & 1, abort, a.c.err)) {
-                        ok = false;
-                        break;
+                            for (int k = 0; k < 4; ++k) {
+                                hi[k] = mul_f16x2(e4[k], d);
+                                lo[k] = fma_f16x2(e4[k], d, hi[k] ^ 0x80008000u);
+                            }
+                            const int chunk = 4 * c + t;
+                            const uint32_t at = dst + (chunk >> 3) * 2 * KPANEL + (((chunk & 7) ^ (krow & 7)) << 4);
+                            st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+                            st_shared_v4(at + KPANEL, lo[0], lo[1], lo[2], lo[3]);
+                        }
                     }
-                    tc05::fence_after();
-                    const uint64_t kd = k_desc + (ks * 2 * L::KTILE >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t p = kk >> 2, at = kk & 3;
-                        tc05::mma_ss_if(one, tmem + TS + k * 2 * BN, q_desc + (((k * L::P + p) * PTILE + at * 32) >> 4),
-                                        kd + ((p * 2 * KPANEL + at * 32) >> 4), id_qk, kk > 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&k_full[ks]);
+                } else {
+                    if (lane == 0) {
+                        info[slot].v[w] = (float)(e - 14);
+                        info[slot].vinv[w] = __uint_as_float((uint32_t)(141 - e) << 23);
+                        mbar_arrive(&info_full[slot]);
                     }
-                    tc05::commit_if(one, &s_full[k]);
+                    if (j >= NV && !warp_wait(&v_empty[vs], (j / NV - 1) & 1, abort, a.c.err)) break;
+                    const int vrow = 16 * w + 8 * (lane >> 4) + 2 * t;
+                    const uint32_t dst = sb + L::V + vs * L::KTILE + vrow * 128;
+#pragma unroll
+                    for (int c = 0; c < NB; ++c) {
+                        // the block's scales of the two tokens
+                        const uint32_t d = mul_f16x2(__byte_perm(y.scales[0][c / 2], y.scales[1][c / 2], c & 1 ? 0x7632 : 0x5410), power);
+                        uint32_t e0[4], e1[4];
+                        unpack_codes<false>(y.codes[0][c], e0, f16_1024, f16_64);
+                        unpack_codes<false>(y.codes[1][c], e1, f16_1024, f16_64);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            e0[i] = mul_f16x2(e0[i], d);
+                            e1[i] = mul_f16x2(e1[i], d);
+                        }
+                        const int chunk = 4 * c + q;
+                        const uint32_t at = dst + (chunk >> 3) * KPANEL;
+                        st_shared_v4(at + (((chunk & 7) ^ (vrow & 7)) << 4), __byte_perm(e0[0], e0[1], 0x5410),
+                                     __byte_perm(e0[2], e0[3], 0x5410), __byte_perm(e1[0], e1[1], 0x5410),
+                                     __byte_perm(e1[2], e1[3], 0x5410));
+                        st_shared_v4(at + 128 + (((chunk & 7) ^ ((vrow + 1) & 7)) << 4), __byte_perm(e0[0], e0[1], 0x7632),
+                                     __byte_perm(e0[2], e0[3], 0x7632), __byte_perm(e1[0], e1[1], 0x7632),
+                                     __byte_perm(e1[2], e1[3], 0x7632));
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[vs]);
                 }
-                tc05::commit_if(one, &k_empty[ks]);
-                if (ok && j >= 1) ok = pv(j - 1);
             }
-            if (ok && ntm > 0) pv(ntm - 1);
-            tc05::commit_if(one, mma_done);
-            if (!mbar_wait(mma_done, 0)) record_device_error(a.c.err, DEV_ERR_DRAIN);
+        } else {
+            {
+                // ---------------- MMA issuer: the whole warp comes along, its first lane's instructions count
+                const uint32_t one = lane == 0;
+                const uint32_t id_qk = tc05::idesc_f16(false, BM, 2 * BN, false);
+                const uint32_t id_pv = tc05::idesc_f16(false, BM, D, true);
+                const int nt[2] = {nt0, nt1};
+                bool ok = warp_wait(q_full, 0, abort, a.c.err);
+                const uint64_t q_desc = tc05::desc_sw128(sb + L::Q, 16, 1024);
+                const uint64_t k_desc = tc05::desc_sw128(sb + L::K, 16, 1024), p_desc = tc05::desc_sw128(sb + L::PR, 16, 1024),
+                               v_desc = tc05::desc_sw128(sb + L::V, KPANEL, 1024);
+                auto pv = [&](int t) -> bool {
+                    const int vs = t % NV;
+                    if (!warp_wait(&v_full[vs], (t / NV) & 1, abort, a.c.err)) return false;
+                    for (int k = 0; k < NQT; ++k) {
+                        if (t >= nt[k]) continue;
+                        if (!warp_wait(&p_full[k], t & 1, abort, a.c.err)) return false;
+                        tc05::fence_after();
+                        const uint64_t pd = p_desc + (k * PTILE >> 4), vd = v_desc + (vs * L::KTILE >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < BN / 16; ++kk)
+                            tc05::mma_ss_if(one, tmem + TO + k * 128, pd + (kk * 32 >> 4), vd + (kk * 2048 >> 4), id_pv,
+                                            (t > 0 || kk > 0) ? 1u : 0u);
+                        tc05::commit_if(one, &o_done[k]);
+                    }
+                    tc05::commit_if(one, &v_empty[vs]);
+                    return true;
+                };
+                for (int j = 0; j < ntm && ok; ++j) {
+                    const int ks = j % NK;
+                    if (!warp_wait(&k_full[ks], (j / NK) & 1, abort, a.c.err)) break;
+                    for (int k = 0; k < NQT && ok; ++k) {
+                        if (j >= nt[k]) continue;
+                        if (j >= 1 && !warp_wait(&s_free[k], (j - 1) & 1, abort, a.c.err)) {
+                            ok = false;
+                            break;
+                        }
+                        tc05::fence_after();
+                        const uint64_t kd = k_desc + (ks * 2 * L::KTILE >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t p = kk >> 2, at = kk & 3;
+                            tc05::mma_ss_if(one, tmem + TS + k * 2 * BN, q_desc + (((k * L::P + p) * PTILE + at * 32) >> 4),
+                                            kd + ((p * 2 * KPANEL + at * 32) >> 4), id_qk, kk > 0);
+                        }
+                        tc05::commit_if(one, &s_full[k]);
+                    }
+                    tc05::commit_if(one, &k_empty[ks]);
+                    if (ok && j >= 1) ok = pv(j - 1);
+                }
+                if (ok && ntm > 0) pv(ntm - 1);
+                tc05::commit_if(one, mma_done);
+                if (!mbar_wait(mma_done, 0)) record_device_error(a.c.err, DEV_ERR_DRAIN);
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
@@ -444,8 +443,6 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                 break;
             }
             tc05::fence_after();
-            // (at most five tiles on, the unpacking warps have to wait for this one's scores to be read: the ring of
-            // eight holds)
             float ck[4], cv[4], ci[4];
             bool full = (t + 1) * BN <= all_see;
 #pragma unroll
