@@ -1165,25 +1165,26 @@ int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op)
 }
 
 // Whether a call's query rows are better taken 256 at a time by the tcgen05
-// kernel. Both read the cache once for every tile of rows; per 64 keys this
-// kernel's tiles of 16 rows cost 2.7 ns each (all SMs together), and the other's
-// pairs of tiles, one an SM, 2460 ns a wave of 148 CTAs (1600 where the rows
-// fill one tile of 128 only). Measured, 32 heads on 8, D 128: 4 requests of 64
-// tokens at 16384: 377 us here, 628 there; 4 of 128: 737 and 631; 16 of 17: 465
-// and 419; 16 of 256: 5747 and 2497; 2 requests of 9 heads on 3, 256 tokens: 226
-// and 621. (D 64 has the same ratios.)
-bool fills_tiles(int64_t tokens, int64_t requests, int64_t kv_heads, int64_t rep, int64_t max_query) {
+// kernel. Both read the cache once for every tile of rows; per 64 keys of D 128
+// (64) this kernel's tiles of 16 rows cost 2.8 (1.8) ns each, all SMs together,
+// and the other's pairs of tiles, one an SM, 2000 (1700) ns a wave of 148 CTAs
+// (1390, 1180 where the rows fill one tile of 128 only). Measured, 32 heads on 8,
+// here and there: 4 requests of 64 tokens at 16384 377 and 509 us (D 64: 239 and
+// 435); 4 of 96 at 8192 295 and 267 (190 and 223); 16 of 17 at 16384 465 and 355
+// (294 and 301); 8 of 64 at 8192 388 and 266 (246 and 222); 16 of 256 at 4096 1577
+// and 541 (999 and 445); 2 of 256 at 16384, 9 heads on 3: 227 and 507 (150 and 434).
+bool fills_tiles(int64_t tokens, int64_t requests, int64_t kv_heads, int64_t rep, int64_t dim, int64_t max_query) {
     if (max_query * rep <= 64) return false;
     requests = std::min(requests, tokens);
     const int64_t rows = (tokens * rep + requests - 1) / requests;  // a request, on average
-    const double here = 2.7 * (double)((rows + 15) / 16 * requests * kv_heads);
+    const double here = (dim == 128 ? 2.8 : 1.8) * (double)((rows + 15) / 16 * requests * kv_heads);
     const double waves = std::max(1.0, (double)((rows + 255) / 256 * requests * kv_heads) / 148.0);
-    return here > waves * (rows > 128 ? 2460.0 : 1600.0);
+    return here > waves * (dim == 128 ? (rows > 128 ? 2000.0 : 1390.0) : (rows > 128 ? 1700.0 : 1180.0));
 }
 
 template <typename T, int D>
 int launch_attend(Split &p, int64_t max_query, void *workspace, cudaStream_t stream) {
-    if (std::is_same<T, __nv_bfloat16>::value && fills_tiles(p.a.tokens, p.a.c.requests, p.a.c.kv_heads, p.a.rep, max_query))
+    if (std::is_same<T, __nv_bfloat16>::value && fills_tiles(p.a.tokens, p.a.c.requests, p.a.c.kv_heads, p.a.rep, D, max_query))
         return launch_sdpa_q4_prefill(p.a, D, stream);
     if constexpr (!(sizeof(T) == 4 && D == 128)) {
         if (wide_tiles(max_query * p.a.rep)) return launch_split<T, D, 2, false>(p, workspace, stream, "tn_sdpa_q4_cache");

@@ -6,15 +6,17 @@
 // rows see nearly the same keys. Key tiles of 64 are unpacked once for both
 // query tiles. 16 warps:
 //   warps 0-3, 4-7   softmax of query tile 0, 1: thread r owns row r (TMEM lane
-//                    r) and all 64 columns
-//                    of a key tile; before, it puts its row of queries into TMEM
-//   warp 8           MMA issuer (one thread): S_k = Q_k K_j^T (Q from TMEM: with
-//                    16 products a tile its shared-memory reads would bound the
-//                    tensor pipe), then O_k += P_k V_{j-1} one tile behind
-//   warp 9           TMEM owner (512 columns)
-//   warps 12-15      unpack: warp w the w-th group of 16 tokens of each key tile,
-//                    from global memory (the next tile's words are loaded before
-//                    this one's are unpacked)
+//                    r) and all 64 keys of a tile; before, it lays out its row
+//                    of queries
+//   warp 8           MMA issuer (one thread): S_k = Q_k K_j^T, the keys' high and
+//                    low terms as one product of 128 columns whose halves the
+//                    softmax adds (as two of 64 columns, with the queries in TMEM,
+//                    1009 us for 916 at the size below), then O_k += P_k V_{j-1} one
+//                    tile behind
+//   warps 9-15       unpack: the keys and the values of the tile's four groups of 16
+//                    tokens in turn, from global memory (a warp's next piece is
+//                    loaded before it unpacks this one); warps 12-15 alone, a group
+//                    each, were what bounded it: 916 us for 866. Warp 9 owns the TMEM.
 // The products are f16: an element is (code - 8) times its block's scale, the
 // scale taken to [1/2, 1) by a power of two of the group's own, so that nothing
 // overflows; the powers come back in the softmax, those of the keys in the
@@ -25,10 +27,11 @@
 // eighth of the bf16 result's own. (bf16 operands would lose 2^-8 three times
 // over. For f16 results those roundings would be as large as the result's: they
 // take the other kernel.)
-// What bounds it: the softmax warps' instructions, as in the dense kernel, and
-// the unpacking beside them on the same schedulers, ~3800 cycles a key tile of
-// which the tensor pipe works a third. 2 x 1536 tokens at 9728, 32/8 heads of 128:
-// 1010 us, 447 TFLOP/s, of which the last wave of items (384 on 148 SMs) an eighth.
+// What bounds it: the tensor pipe, which is never idle for long, at ~4000 cycles a
+// key tile (its products of 128 x 128 x 16 come one in 110 to 160 cycles; with two
+// terms of K a third of them is work that a bf16 K would not have), and the last
+// wave of items (384 on 148 SMs), an eighth. 2 x 1536 tokens at 9728, 32/8 heads of
+// 128: 866 us, 521 TFLOP/s.
 // Every wait is bounded; one that gives up raises a CTA-wide abort flag.
 #include <algorithm>
 #include <atomic>
