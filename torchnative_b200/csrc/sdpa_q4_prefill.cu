@@ -27,11 +27,11 @@
 // eighth of the bf16 result's own. (bf16 operands would lose 2^-8 three times
 // over. For f16 results those roundings would be as large as the result's: they
 // take the other kernel.)
-// What bounds it: the tensor pipe, which is never idle for long, at ~4000 cycles a
-// key tile (its products of 128 x 128 x 16 come one in 110 to 160 cycles; with two
-// terms of K a third of them is work that a bf16 K would not have), and the last
-// wave of items (384 on 148 SMs), an eighth. 2 x 1536 tokens at 9728, 32/8 heads of
-// 128: 866 us, 521 TFLOP/s.
+// What bounds it: the stream of products, of which hardly a moment is without one,
+// but each of 128 x 128 x 16 takes 110 to 160 cycles for the 64 of the pipe's peak
+// (which was active 41% of the cycles at 866 us); two terms of K make half as many
+// again; and the last wave of items (384 on 148 SMs), an eighth. 2 x 1536 tokens at
+// 9728, 32/8 heads of 128: 820 us, 550 TFLOP/s.
 // Every wait is bounded; one that gives up raises a CTA-wide abort flag.
 #include <algorithm>
 #include <atomic>
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                         if (j >= 1 && j < nt[k]) ok = warp_wait(&s_free[k], (j - 1) & 1, abort, a.c.err);
                     if (!ok) break;
                     tc05::fence_after();
-                    // The two tiles' products in turn: in a row on one tile each waits for the one before (864 us for
-                    // 820 at the size above).
+                    // The two tiles' products in turn: 864 us one tile after the other, 820 so. (The results' in turn,
+                    // too: 832, since the first tile's then wait for the second's probabilities.)
                     const uint64_t kd = k_desc + (ks * 2 * L::KTILE >> 4);
                     const uint32_t go[2] = {one && j < nt0, one && j < nt1};
 #pragma unroll
