@@ -397,11 +397,19 @@ TN_API int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t p
  * (slots and positions -1, query_start 0) and sets *status, if that is 0, to
  * 1: not enough pages, 2: a length outside [0, max_pages * page_size], 3: more
  * new tokens than max_tokens, 4: more free pages than num_pages. *status is
- * never cleared here. requests <= 8192. */
+ * never cleared here. requests <= 8192.
+ * tn_kv_pages_resize_granted also writes granted [requests]: each request's new
+ * tokens, 0 for all of a call that cannot be met. Decode steps that follow read
+ * it, so that they append nothing where no slot was given. */
 TN_API int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
                               const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
                               int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots,
                               int *positions, int64_t max_tokens, int *query_start, int *status, void *stream);
+TN_API int tn_kv_pages_resize_granted(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
+                                      const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
+                                      int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots,
+                                      int *positions, int64_t max_tokens, int *query_start, int *status,
+                                      int *granted, void *stream);
 
 /* Quantises key and value rows k, v [tokens][kv_heads][head_dim] (dtype F32,
  * F16 or BF16; element strides of token and head, unit inner stride, rows 16-byte
@@ -444,13 +452,23 @@ TN_API int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strides, 
  * bf16), append k and v to that slot in 4 bits, attend keys [0, lengths[b])
  * and, if codes is not NULL, write out's planar Q8_0 too (the bytes of
  * tn_q8_0_quantize_planar). A request of length 0 appends nothing and gives
- * zeros. out [requests][heads][head_dim]; heads / kv_heads <= 8. */
+ * zeros, and so does one with granted[b] <= 0 (granted: of the resize before;
+ * NULL: every request's length counts its new token). Without `granted` a step
+ * behind a resize that was refused writes over the last cached tokens.
+ * out [requests][heads][head_dim]; heads / kv_heads <= 8. */
 TN_API int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t rope_rows, void *pool,
                                   int64_t num_pages, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                   int64_t page_size, const int *page_table, int64_t table_stride,
                                   int64_t max_pages, const int *lengths, int64_t requests, void *out, float *lse,
                                   int8_t *codes, float *scales, float *offsets, double scale, void *workspace,
                                   int64_t workspace_bytes, void *stream);
+TN_API int tn_sdpa_q4_decode_step_granted(const void *qkv, const void *rope, int64_t rope_rows, void *pool,
+                                          int64_t num_pages, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t page_size, const int *page_table, int64_t table_stride,
+                                          int64_t max_pages, const int *lengths, int64_t requests, void *out,
+                                          float *lse, int8_t *codes, float *scales, float *offsets, double scale,
+                                          void *workspace, int64_t workspace_bytes, const int *granted,
+                                          void *stream);
 
 /* ------------------------------------------------ decode-step glue (bf16) --
  * The work between the hot operators in one greedy token of transformers'
@@ -477,9 +495,12 @@ TN_API int tn_llama_rope_append(const void *qkv, const float *inv_freq, const in
                                 void *q_out, void *k_cache, void *v_cache, int64_t cache_b_stride,
                                 int64_t cache_h_stride, void *stream);
 /* tokens[r] = argmax(logits[r]) (first index of the maximum); h[r] = embed[tokens[r]];
- * if pos_dev, *pos_dev += 1. */
+ * if pos_dev, *pos_dev += 1. With `granted` a row of granted[r] <= 0 keeps its token. */
 TN_API int tn_llama_argmax_embed(const void *logits, int64_t rows, int64_t V, int *tokens,
                                  const void *embed, int64_t H, void *h, int *pos_dev, void *stream);
+TN_API int tn_llama_argmax_embed_granted(const void *logits, int64_t rows, int64_t V, int *tokens,
+                                         const void *embed, int64_t H, void *h, int *pos_dev,
+                                         const int *granted, void *stream);
 /* h[r] = embed[tokens[r]]. */
 TN_API int tn_llama_embed(const int *tokens, int64_t rows, const void *embed, int64_t H, void *h,
                           void *stream);

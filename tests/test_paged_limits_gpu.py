@@ -1,0 +1,114 @@
+"""The paged 4-bit cache where something runs out: pages, a request's table, the engine's capacity. What cannot be met
+leaves pools, lengths and tokens as they were, and the next call that can be goes on from there."""
+
+import pytest
+import torch
+
+from tests.test_decode_paged_gpu import small, tokens
+from tests.test_kv_cache_gpu import rope_table
+from torchnative_b200 import _native as N
+from torchnative_b200 import kv_cache as kv
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def i32(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("batch, replay", [(2, False), (2, True), (6, False), (6, True)])
+def test_a_full_sequence_leaves_the_others_alone(cuda_device, batch, replay):
+    """One sequence at its capacity: the step changes nothing; without it the others go on as if it had never been."""
+    dec = small(batch, cuda_device)
+    rest = [20 + 3 * i for i in range(1, batch)]
+    dec.fill_prompt_cache([0] + rest)
+    dec.start(tokens(batch, cuda_device))
+    want = []
+    for _ in range(6):
+        dec.step()
+        want.append(dec.tokens[1:].tolist())
+    graph = dec.capture() if replay else None
+    step = graph.replay if replay else dec.step
+    dec.fill_prompt_cache([79] + rest)
+    dec.paged.check()
+    dec.start(tokens(batch, cuda_device))
+    step()  # the first sequence's last place
+    got = [dec.tokens[1:].tolist()]
+    before = [p.clone() for p in dec.paged.pools], dec.tokens.clone(), dec.h.clone(), dec.paged.lengths.tolist()
+    for _ in range(3):
+        step()
+        assert all(torch.equal(a, b) for a, b in zip(dec.paged.pools, before[0]))
+        assert torch.equal(dec.tokens, before[1]) and torch.equal(dec.h, before[2])
+        assert dec.paged.lengths.tolist() == before[3]
+    with pytest.raises(RuntimeError, match="length"):
+        dec.paged.check()
+    dec.paged.resize(0, new_lengths=i32([0] + before[3][1:], cuda_device))
+    for _ in range(5):
+        step()
+        got.append(dec.tokens[1:].tolist())
+    dec.paged.check()
+    assert got == want
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim", [(8, 2, 128), (3, 3, 64)])
+def test_a_step_behind_a_refused_resize_appends_nothing(cuda_device, heads, kv_heads, dim):
+    """Pages run out: the step gives zeros and leaves the pool, byte for byte; with pages again it is an ordinary one."""
+    cache = kv.PagedQ4Cache(1, kv_heads, dim, 3, 2, 4, 16, cuda_device)
+    g = torch.Generator().manual_seed(dim)
+    x = torch.randn((33, kv_heads, dim), generator=g).to(cuda_device)
+    slots, _, _ = cache.resize(33, new_lengths=i32([32, 1], cuda_device))
+    assert cache.granted.tolist() == [32, 1]
+    cache.append(0, x, x.flip(0), slots)
+    qkv = torch.randn((2, (heads + 2 * kv_heads) * dim), generator=g).to(BF).to(cuda_device)
+    rope = rope_table(64, dim, cuda_device)
+    nb = heads * dim // 32
+    q8 = (torch.ones((2, heads * dim), dtype=torch.int8, device=cuda_device), torch.ones((2, nb), device=cuda_device),
+          torch.ones((2, nb), device=cuda_device))
+    before = cache.pools[0].clone()
+    cache.resize(2, grow=1)
+    out = cache.decode_step(0, qkv, rope, heads, q8=q8)
+    assert cache.granted.tolist() == [0, 0]
+    assert (out == 0).all() and (q8[0] == 0).all() and (q8[1] == 0).all()
+    assert torch.equal(cache.pools[0], before)
+    with pytest.raises(RuntimeError, match="pages"):
+        cache.check()
+    cache.resize(0, new_lengths=i32([32, 0], cuda_device))  # the second request ends
+    cache.resize(1, grow=1)
+    assert cache.granted.tolist() == [1, 0]
+    out = cache.decode_step(0, qkv, rope, heads)
+    cache.check()
+    other = before.clone()
+    want = kv.sdpa_q4_decode_step(qkv, rope, other, cache.page_table, cache.lengths, heads)
+    assert torch.equal(out, want) and torch.equal(cache.pools[0], other) and (out[0] != 0).any()
+
+
+def test_rows_without_a_grant_keep_their_token(cuda_device):
+    g = torch.Generator().manual_seed(4)
+    logits = torch.randn((4, 999), generator=g).to(BF).to(cuda_device)
+    embed = torch.randn((999, 64), generator=g).to(BF).to(cuda_device)
+    had, granted = i32([7, 8, 9, 10], cuda_device), i32([1, 0, 3, -1], cuda_device)
+    h = torch.zeros((4, 64), dtype=BF, device=cuda_device)
+    for given in (granted, None):
+        got = had.clone()
+        N.check(N.lib().tn_llama_argmax_embed_granted(
+            logits.data_ptr(), 4, 999, got.data_ptr(), embed.data_ptr(), 64, h.data_ptr(), None,
+            None if given is None else given.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        best = logits.float().argmax(-1).to(torch.int32)
+        want = best if given is None else torch.where(given > 0, best, had)
+        assert torch.equal(got, want) and torch.equal(h, embed[want.long()])
+
+
+def test_granted_is_checked(cuda_device):
+    cache = kv.PagedQ4Cache(1, 1, 64, 4, 2, 2, 16, cuda_device)
+    args = (cache.page_table, cache.lengths, cache.free_pages, cache.free_count, cache.status, 16, 2)
+    qkv, rope = torch.zeros((2, 192), dtype=BF, device=cuda_device), rope_table(9, 64, cuda_device)
+    step = (qkv, rope, cache.pools[0], cache.page_table, cache.lengths, 1)
+    for bad, error, match in ((i32([0], cuda_device), RuntimeError, "granted"), (i32([0, 0], "cpu"), RuntimeError, "device"),
+                              (torch.zeros(2, device=cuda_device), NotImplementedError, "granted"),
+                              (i32([0, 0, 0, 0], cuda_device)[::2], RuntimeError, "contiguous")):
+        with pytest.raises(error, match=match):
+            kv.kv_pages_resize(*args, grow=1, granted=bad)
+        with pytest.raises(error, match=match):
+            kv.sdpa_q4_decode_step(*step, granted=bad)

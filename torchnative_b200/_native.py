@@ -107,16 +107,21 @@ SIGNATURES = {
                                     _D, _P]),
     "tn_kv_q4_page_bytes": (_I64, [_I64, _I64, _I64]),
     "tn_kv_pages_resize": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _P]),
+    "tn_kv_pages_resize_granted": (_I, [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _P, _P,
+                                        _P, _P]),
     "tn_kv_q4_append": (_I, [_P, _P, _I, _PI64, _PI64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "tn_sdpa_q4_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "tn_sdpa_q4_cache": (_I, [_P, _I, _PI64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _P,
                               _I64, _P, _P, _D, _P, _I64, _P]),
     "tn_sdpa_q4_decode_step": (_I, [_P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _P,
                                     _P, _P, _P, _D, _P, _I64, _P]),
+    "tn_sdpa_q4_decode_step_granted": (_I, [_P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _P,
+                                            _P, _P, _P, _P, _D, _P, _I64, _P, _P]),
     "tn_llama_add_rmsnorm_q8": (_I, [_P, _P, _P, _P, ctypes.c_float, _I64, _I64, _P, _P, _P, _P]),
     "tn_llama_silu_mul_q8": (_I, [_P, _I64, _I64, _P, _P, _P, _P]),
     "tn_llama_rope_append": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P]),
     "tn_llama_argmax_embed": (_I, [_P, _I64, _I64, _P, _P, _I64, _P, _P, _P]),
+    "tn_llama_argmax_embed_granted": (_I, [_P, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P]),
     "tn_llama_embed": (_I, [_P, _I64, _P, _I64, _P, _P]),
     "tn_llama_decode_layout_of": (_I, [_P, _P]),
     "tn_llama_decode_plan": (_I, [_P, _P, _I64, ctypes.POINTER(_P)]),

@@ -137,11 +137,13 @@ __global__ void rope_append_kernel(const __nv_bfloat16 *__restrict__ qkv, const 
 }
 
 // Greedy pick (first index of the maximum, torch.argmax) per row, then the
-// next token's embedding row; thread 0 of row 0 advances the position.
+// next token's embedding row; thread 0 of row 0 advances the position. A row
+// that was granted no token in this step keeps the one it has.
 __global__ void __launch_bounds__(1024) argmax_embed_kernel(const __nv_bfloat16 *__restrict__ logits, int V,
                                                             int *__restrict__ tokens,
                                                             const __nv_bfloat16 *__restrict__ embed, int H,
-                                                            __nv_bfloat16 *__restrict__ h, int *pos_dev) {
+                                                            __nv_bfloat16 *__restrict__ h, int *pos_dev,
+                                                            const int *granted) {
     pdl_launch_dependents();
     pdl_wait();
     __shared__ float bv[32];
@@ -199,8 +201,11 @@ __global__ void __launch_bounds__(1024) argmax_embed_kernel(const __nv_bfloat16 
             if (ov > best || (ov == best && oi < idx)) best = ov, idx = oi;
         }
         if (lane == 0) {
+            if (granted && granted[row] <= 0)
+                idx = tokens[row];
+            else
+                tokens[row] = idx;
             winner = idx;
-            tokens[row] = idx;
         }
     }
     __syncthreads();
@@ -285,12 +290,17 @@ extern "C" int tn_llama_rope_append(const void *qkv, const float *inv_freq, cons
                       (__nv_bfloat16 *)v_cache, cache_b_stride, cache_h_stride);
 }
 
-extern "C" int tn_llama_argmax_embed(const void *logits, int64_t rows, int64_t V, int *tokens, const void *embed,
-                                     int64_t H, void *h, int *pos_dev, void *stream) {
+extern "C" int tn_llama_argmax_embed_granted(const void *logits, int64_t rows, int64_t V, int *tokens, const void *embed,
+                                             int64_t H, void *h, int *pos_dev, const int *granted, void *stream) {
     if (rows <= 0) return TN_OK;
     return launch_pdl(tn::argmax_embed_kernel, dim3((unsigned)rows), dim3(1024), tn::stream_of(stream),
                       "tn_llama_argmax_embed", (const __nv_bfloat16 *)logits, (int)V, tokens,
-                      (const __nv_bfloat16 *)embed, (int)H, (__nv_bfloat16 *)h, pos_dev);
+                      (const __nv_bfloat16 *)embed, (int)H, (__nv_bfloat16 *)h, pos_dev, granted);
+}
+
+extern "C" int tn_llama_argmax_embed(const void *logits, int64_t rows, int64_t V, int *tokens, const void *embed,
+                                     int64_t H, void *h, int *pos_dev, void *stream) {
+    return tn_llama_argmax_embed_granted(logits, rows, V, tokens, embed, H, h, pos_dev, nullptr, stream);
 }
 
 extern "C" int tn_llama_embed(const int *tokens, int64_t rows, const void *embed, int64_t H, void *h, void *stream) {

@@ -62,6 +62,7 @@ struct Resize {
     int *positions;
     int max_tokens;
     int *query_start, *status;
+    int *granted;  // [requests] or NULL
     int aligned;  // slots and positions may be written in 16-byte vectors
 };
 
@@ -164,7 +165,10 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
                                                                           : BAD_NONE;
     if (bad) {  // nothing changes; no token has a slot
         if (me == 0 && *p.status == 0) *p.status = bad;
-        for (int b = me; b <= B; b += all) p.query_start[b] = 0;
+        for (int b = me; b <= B; b += all) {
+            p.query_start[b] = 0;
+            if (p.granted && b < B) p.granted[b] = 0;
+        }
         if (p.max_tokens <= kSlotsInOne) {
             for (int r = me; r < p.max_tokens; r += all) {
                 p.slots[r] = -1;
@@ -185,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
         if (blockIdx.x == 0) {
             p.query_start[b] = tok_at[b];
             p.lengths[b] = n;
+            if (p.granted) p.granted[b] = max(0, n - o);
         }
     }
     const int top = top0 + (int)gives;
@@ -289,10 +294,11 @@ extern "C" int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64
     return kv_heads * (page_size / tn::kKvGroup) * 18 * head_dim;
 }
 
-extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
-                                  const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
-                                  int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots, int *positions,
-                                  int64_t max_tokens, int *query_start, int *status, void *stream) {
+extern "C" int tn_kv_pages_resize_granted(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
+                                          const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
+                                          int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots,
+                                          int *positions, int64_t max_tokens, int *query_start, int *status,
+                                          int *granted, void *stream) {
     const std::string op("tn_kv_pages_resize");
     const int shift = tn::kv_page_shift(page_size);
     if (shift < 0)
@@ -313,7 +319,7 @@ extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t
         return tn::set_error(TN_ERR_INVALID, op + ": new_lengths must not be lengths");
     tn::Resize p{page_table, table_stride, (int)max_pages, lengths, new_lengths, (int)grow, (int)requests, free_pages,
                  free_count, (int)num_pages, shift, slots, positions, (int)max_tokens, query_start, status,
-                 ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0};
+                 granted, ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0};
     const int smem = (int)((5 * requests + 2) * sizeof(int));
     if (smem > 48 * 1024 - 1024) {
         int st = tn::check_cuda(
@@ -329,4 +335,13 @@ extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t
     if (st || max_tokens <= tn::kSlotsInOne) return st;
     return tn::launch_pdl(tn::kv_pages_slots_kernel, dim3((unsigned)((max_tokens + 1023) / 1024)), dim3(256),
                           (int)((requests + 1) * sizeof(int)), s, "tn_kv_pages_resize", p);
+}
+
+extern "C" int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
+                                  const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
+                                  int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots, int *positions,
+                                  int64_t max_tokens, int *query_start, int *status, void *stream) {
+    return tn_kv_pages_resize_granted(page_table, table_stride, max_pages, lengths, new_lengths, grow, requests, free_pages,
+                                      free_count, num_pages, page_size, slots, positions, max_tokens, query_start, status,
+                                      nullptr, stream);
 }

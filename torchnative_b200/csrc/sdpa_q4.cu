@@ -126,6 +126,13 @@ struct Split {
     int64_t rope_rows;
     int8_t *codes;
     float *scales, *offsets;
+    const int *granted;  // [requests] new tokens that the resize gave, or NULL: one to each
+    // The tokens of request b, its new one among them: none where the resize gave none, so that nothing is appended
+    // over what the cache holds.
+    __device__ __forceinline__ int step_length(int b) const {
+        if (granted && granted[b] <= 0) return 0;
+        return a.c.length(b);
+    }
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -145,13 +152,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 // A place in the line of units: group g of item (b, tile u, head h), whose
 // groups this CTA has from `from` to `upto`. `rel` is the place of the item's
 // group 0 against the first of the CTA's `len` places.
-template <int RT>
+template <int RT, bool STEP>
 struct Cursor {
     int b, u, h, G, rel;
     int S, n, first, tiles;
 
-    __device__ __forceinline__ void load_request(const Attend &p) {
-        S = p.c.length(b);
+    __device__ __forceinline__ void load_request(const Split &s) {
+        const Attend &p = s.a;
+        S = STEP ? s.step_length(b) : p.c.length(b);
         n = p.query_tokens(b, &first);
         tiles = (n * p.rep + RT - 1) / RT;
     }
@@ -169,7 +177,8 @@ struct Cursor {
     __device__ __forceinline__ int from() const { return max(0, -rel); }
     __device__ __forceinline__ int upto(int len) const { return min(G, len - rel); }
     // The next item; past the last one rel is beyond every len.
-    __device__ __forceinline__ void next_item(const Attend &p) {
+    __device__ __forceinline__ void next_item(const Split &s) {
+        const Attend &p = s.a;
         rel += G + kItemCost;
         if (++h < p.c.kv_heads) return;
         h = 0;
@@ -182,7 +191,7 @@ struct Cursor {
                     G = 1;
                     return;
                 }
-                load_request(p);
+                load_request(s);
             } while (tiles == 0);
         }
         G = tile_units(p, u);
@@ -349,7 +358,7 @@ __device__ __forceinline__ void fewer_registers() {
 // One warp: the item's queries; lane (g, t) holds row g, elements 32 b + 8 t ..
 // + 7 of each block.
 template <typename T, int D, int NT, bool STEP>
-__device__ __forceinline__ void load_queries(const Split &p, const Cursor<8 * NT> &at, float (&x)[NT][D / 32][8]) {
+__device__ __forceinline__ void load_queries(const Split &p, const Cursor<8 * NT, STEP> &at, float (&x)[NT][D / 32][8]) {
     const Attend &a = p.a;
     const int lane = threadIdx.x & 31, lt = lane & 3, row0 = at.u * 8 * NT;
 #pragma unroll
@@ -377,8 +386,8 @@ __device__ __forceinline__ void load_queries(const Split &p, const Cursor<8 * NT
 }
 
 // The same warp: into the slot, as the first product's B fragments.
-template <typename T, int D, int NT>
-__device__ __forceinline__ void put_queries(const Split &p, const Cursor<8 * NT> &at, const float (&q)[NT][D / 32][8],
+template <typename T, int D, int NT, bool STEP>
+__device__ __forceinline__ void put_queries(const Split &p, const Cursor<8 * NT, STEP> &at, const float (&q)[NT][D / 32][8],
                                             typename Shape<T, D, NT>::Slot &slot) {
     using H = Shape<T, D, NT>;
     constexpr int NB = H::NB;
@@ -480,14 +489,14 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
     if (warp >= W) {
         fewer_registers<H::PRODUCER_REGS>();
         // ---- a producer: this CTA's part of the line
-        Cursor<RT> at;
+        Cursor<RT, STEP> at;
         long long total = 0, own = 0;
 #pragma unroll 1
         for (int b0 = 0; b0 < a.c.requests; b0 += 32) {
             own = 0;
             at.b = b0 + lane;
             if (at.b < a.c.requests) {
-                at.load_request(a);
+                at.load_request(p);
                 own = at.request_places(a);
             }
             long long w = own;
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                     own = 0;
                     at.b = b0 + lane;
                     if (at.b < a.c.requests) {
-                        at.load_request(a);
+                        at.load_request(p);
                         own = at.request_places(a);
                     }
                 }
@@ -529,7 +538,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                 }
                 place += __shfl_sync(0xffffffffu, upto, 31);
             }
-            at.load_request(a);
+            at.load_request(p);
 #pragma unroll 1
             for (at.u = 0;; ++at.u) {
                 at.G = at.tile_units(a, at.u);
@@ -550,7 +559,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
 #pragma unroll 1
             for (int m = 0;; ++m) {
 #pragma unroll 1
-                while (at.rel < len && at.from() >= at.upto(len)) at.next_item(a);
+                while (at.rel < len && at.from() >= at.upto(len)) at.next_item(p);
                 if (at.rel >= len) return;
                 const bool ok = m < 2 || mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1);
                 if (__any_sync(0xffffffffu, !ok)) {
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                 if (at.upto(len) == at.G) append_new<D>(p, at.b, at.h, at.S - 1, slots[m & 1].added);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&new_full[m & 1]);
-                at.next_item(a);
+                at.next_item(p);
             }
         }
         if (warp > W) {
@@ -578,7 +587,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                         have = false;
                     } else {
                         g -= max(at.from(), at.upto(len));
-                        at.next_item(a);
+                        at.next_item(p);
                         g += at.from();
                     }
                 }
@@ -628,7 +637,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
 #pragma unroll 1
         for (int m = 0;; ++m) {
 #pragma unroll 1
-            while (at.rel < len && at.from() >= at.upto(len)) at.next_item(a);
+            while (at.rel < len && at.from() >= at.upto(len)) at.next_item(p);
             typename H::Slot &slot = slots[m & 1];
             const bool end = at.rel >= len;
             if (m >= 2 && !mbar_wait(&q_empty[m & 1], (m / 2 - 1) & 1)) broken = true;
@@ -640,7 +649,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
                 const int g0 = at.from(), g1 = at.upto(len), row0 = at.u * RT, rows = min(RT, at.n * a.rep - row0);
                 float q[NT][NB][8];
                 load_queries<T, D, NT, STEP>(p, at, q);
-                put_queries<T, D, NT>(p, at, q, slot);
+                put_queries<T, D, NT, STEP>(p, at, q, slot);
                 Item it;
                 it.end = 0;
                 it.g0 = g0, it.g1 = g1, it.i0 = i0;
@@ -663,7 +672,7 @@ __global__ void __launch_bounds__(32 * (Shape<T, D, NT>::W + 4), 1) sdpa_q4_kern
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[m & 1]);
             if (end) return;
-            at.next_item(a);
+            at.next_item(p);
         }
     }
 
@@ -1257,12 +1266,13 @@ extern "C" int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strid
                              : tn::launch_attend<__nv_bfloat16, 64>(p, max_query, workspace, s);
 }
 
-extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t rope_rows, void *pool, int64_t num_pages,
-                                      int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
-                                      const int *page_table, int64_t table_stride, int64_t max_pages, const int *lengths,
-                                      int64_t requests, void *out, float *lse, int8_t *codes, float *scales,
-                                      float *offsets, double scale, void *workspace, int64_t workspace_bytes,
-                                      void *stream) {
+extern "C" int tn_sdpa_q4_decode_step_granted(const void *qkv, const void *rope, int64_t rope_rows, void *pool,
+                                              int64_t num_pages, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t page_size, const int *page_table, int64_t table_stride,
+                                              int64_t max_pages, const int *lengths, int64_t requests, void *out,
+                                              float *lse, int8_t *codes, float *scales, float *offsets, double scale,
+                                              void *workspace, int64_t workspace_bytes, const int *granted,
+                                              void *stream) {
     const char *op = "tn_sdpa_q4_decode_step";
     int st = tn::check_kv_pool(op, pool, num_pages, kv_heads, head_dim, page_size);
     if (st) return st;
@@ -1295,6 +1305,18 @@ extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t
     p.codes = codes;
     p.scales = scales;
     p.offsets = offsets;
+    p.granted = granted;
     return head_dim == 128 ? tn::launch_split<__nv_bfloat16, 128, 1, true>(p, workspace, s, op)
                            : tn::launch_split<__nv_bfloat16, 64, 1, true>(p, workspace, s, op);
+}
+
+extern "C" int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t rope_rows, void *pool, int64_t num_pages,
+                                      int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                      const int *page_table, int64_t table_stride, int64_t max_pages, const int *lengths,
+                                      int64_t requests, void *out, float *lse, int8_t *codes, float *scales,
+                                      float *offsets, double scale, void *workspace, int64_t workspace_bytes,
+                                      void *stream) {
+    return tn_sdpa_q4_decode_step_granted(qkv, rope, rope_rows, pool, num_pages, heads, kv_heads, head_dim, page_size,
+                                          page_table, table_stride, max_pages, lengths, requests, out, lse, codes, scales,
+                                          offsets, scale, workspace, workspace_bytes, nullptr, stream);
 }

@@ -109,6 +109,13 @@ def _table_shape(op: str, page_table: torch.Tensor, lengths: torch.Tensor):
     return page_table.shape
 
 
+def _granted(op: str, device: torch.device, granted: torch.Tensor, lengths: torch.Tensor) -> int:
+    _require(op, device, "granted", granted, _I32)
+    if granted.shape != lengths.shape:
+        raise RuntimeError(f"{op}: granted {list(granted.shape)} does not fit lengths {list(lengths.shape)}")
+    return granted.data_ptr()
+
+
 def _pool_shape(op: str, pool: torch.Tensor):
     """(pages, KV heads, page size, head dimension) of a pool [pages, heads, page_size / 16, 18 D]."""
     shape = pool.shape
@@ -128,7 +135,7 @@ def kv_q4_pool(num_pages: int, kv_heads: int, head_dim: int, page_size: int, dev
 
 def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Tensor,
                     free_count: torch.Tensor, status: torch.Tensor, page_size: int, max_tokens: int, *,
-                    new_lengths: torch.Tensor | None = None, grow: int = 0):
+                    new_lengths: torch.Tensor | None = None, grow: int = 0, granted: torch.Tensor | None = None):
     """Take every request from its length to `new_lengths`, or, without them,
     grow every request that has tokens by `grow`; returns (slots int64 and
     positions int32 [max_tokens], query_start int32 [requests + 1]) of the new
@@ -136,7 +143,9 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     go back to the stack free_pages[:free_count]; page_table, lengths,
     free_pages and free_count are updated in place. Nothing waits for the GPU:
     a call that cannot be met changes nothing, gives no token a slot and sets
-    `status` (see `PagedQ4Cache.check`)."""
+    `status` (see `PagedQ4Cache.check`). `granted` (int32 [requests]) receives
+    each request's new tokens, 0 for all of such a call: what a decode step
+    needs to leave the cache alone then."""
     op = "kv_pages_resize"
     device, index = page_table.device, page_table.get_device()
     if not (index >= 0 and page_table.dtype is lengths.dtype is free_pages.dtype is free_count.dtype is status.dtype is _I32
@@ -160,12 +169,15 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
             _require(op, device, "new_lengths", new_lengths, _I32)
             raise RuntimeError(f"{op}: new_lengths {list(new_lengths.shape)} do not fit lengths {list(lengths.shape)}")
         new = new_lengths.data_ptr()
+    if granted is not None:
+        granted = _granted(op, device, granted, lengths)
     slots = _empty(_I64, index, max_tokens)
     positions = _empty(_I32, index, max_tokens)
     query_start = _empty(_I32, index, requests + 1)
-    _call(index, "tn_kv_pages_resize", page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
+    _call(index, "tn_kv_pages_resize_granted", page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
           int(grow), requests, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size,
-          slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr())
+          slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr(),
+          granted)
     return slots, positions, query_start
 
 
@@ -274,14 +286,18 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
 
 
 def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
-                        lengths: torch.Tensor, heads: int, *, scale: float | None = None, q8=None) -> torch.Tensor:
+                        lengths: torch.Tensor, heads: int, *, scale: float | None = None, q8=None,
+                        granted: torch.Tensor | None = None) -> torch.Tensor:
     """One decode token's attention block of every request, bf16: from the
     projection rows qkv [requests, (heads + 2 kv_heads) D], rotate q and k at
     position lengths - 1 (rows of `rope` [positions, D]: cosines, then sines),
     append k and v there in 4 bits, attend. Returns [requests, heads, D]; q8 =
     (codes int8 [requests, heads D], scales and offsets float32 [requests,
     heads D / 32]) also receives its planar Q8_0, the next linear's
-    activations. A request of length 0 appends nothing and gives zeros."""
+    activations. A request of length 0 appends nothing and gives zeros, and so
+    does one with granted[b] <= 0: pass what the resize before granted. Without
+    it every length counts a new token, and a step behind a resize that could
+    not be met writes over the last cached ones."""
     op = "sdpa_q4_decode_step"
     device, index = qkv.device, qkv.get_device()
     if not (index >= 0 and qkv.dtype is rope.dtype is _BF16 and pool.dtype is _U8
@@ -312,12 +328,14 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
             raise RuntimeError(f"{op}: q8 must be codes [{requests}, {heads * dim}], scales and offsets "
                                f"[{requests}, {heads * dim // 32}]")
         codes, scales, offsets = codes.data_ptr(), scales.data_ptr(), offsets.data_ptr()
+    if granted is not None:
+        granted = _granted(op, device, granted, lengths)
     out = _empty(_BF16, index, requests, heads, dim)
     ws = _workspace(device, index, heads // kv_heads, dim, requests, heads, kv_heads, 1)
-    _call(index, "tn_sdpa_q4_decode_step", qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
+    _call(index, "tn_sdpa_q4_decode_step_granted", qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
           heads, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
           out.data_ptr(), None, codes, scales, offsets, 0.0 if scale is None else float(scale), ws.data_ptr(),
-          ws.numel())
+          ws.numel(), granted)
     return out
 
 
@@ -360,6 +378,8 @@ class PagedQ4Cache:
         self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
         self.free_count = torch.full((1,), num_pages, **i32)
         self.status = torch.zeros(1, **i32)
+        # the new tokens that the last resize gave each request, for the decode steps behind it
+        self.granted = torch.zeros(max_requests, **i32)
 
     def nbytes(self) -> int:
         return sum(p.numel() for p in self.pools)
@@ -367,7 +387,7 @@ class PagedQ4Cache:
     def resize(self, max_tokens: int, *, new_lengths: torch.Tensor | None = None, grow: int = 0):
         """`kv_pages_resize` of this cache: (slots, positions, query_start)."""
         return kv_pages_resize(self.page_table, self.lengths, self.free_pages, self.free_count, self.status,
-                               self.page_size, max_tokens, new_lengths=new_lengths, grow=grow)
+                               self.page_size, max_tokens, new_lengths=new_lengths, grow=grow, granted=self.granted)
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor) -> None:
         kv_q4_append(key, value, self.pools[layer], slots)
@@ -377,8 +397,10 @@ class PagedQ4Cache:
                              max_tokens=max_tokens, scale=scale)
 
     def decode_step(self, layer: int, qkv: torch.Tensor, rope: torch.Tensor, heads: int, *, scale=None, q8=None):
+        """`sdpa_q4_decode_step` of the tokens that the last `resize` granted; a
+        request that it gave none keeps its cache and gives zeros."""
         return sdpa_q4_decode_step(qkv, rope, self.pools[layer], self.page_table, self.lengths, heads, scale=scale,
-                                   q8=q8)
+                                   q8=q8, granted=self.granted)
 
     def check(self) -> None:
         """Wait for the GPU and raise for a resize that could not be met since

@@ -528,11 +528,11 @@ class Q4LlamaDecoder:
         """Pages for the step's token of every sequence that has tokens."""
         c = self.paged
         requests, max_pages = c.page_table.shape
-        N.check(N.lib().tn_kv_pages_resize(
+        N.check(N.lib().tn_kv_pages_resize_granted(
             P(c.page_table.data_ptr()), max_pages, max_pages, P(c.lengths.data_ptr()), None, 1, requests,
             P(c.free_pages.data_ptr()), P(c.free_count.data_ptr()), c.free_pages.shape[0], c.page_size,
             P(self._slots.data_ptr()), P(self._positions.data_ptr()), requests, P(self._query_start.data_ptr()),
-            P(c.status.data_ptr()), stream))
+            P(c.status.data_ptr()), P(c.granted.data_ptr()), stream))
 
     def _attn_paged(self, li, out, stream, q8: bool) -> None:
         """Rotary embedding, append and attention of layer li's new tokens from
@@ -542,15 +542,20 @@ class Q4LlamaDecoder:
         pool = c.pools[li]
         requests, max_pages = c.page_table.shape
         codes = (P(t.data_ptr()) if q8 else None for t in (self.codes, self.scales, self.offsets))
-        N.check(N.lib().tn_sdpa_q4_decode_step(
+        N.check(N.lib().tn_sdpa_q4_decode_step_granted(
             P(self.qkv_out.data_ptr()), P(self.rope.data_ptr()), self.rope.shape[0], P(pool.data_ptr()), pool.shape[0],
             self.hq, self.hkv, s.head_dim, c.page_size, P(c.page_table.data_ptr()), max_pages, max_pages,
             P(c.lengths.data_ptr()), requests, P(out.data_ptr()), None, *codes, 1.0 / math.sqrt(s.head_dim),
-            P(self._attn_ws.data_ptr()), self._attn_ws.numel(), stream))
+            P(self._attn_ws.data_ptr()), self._attn_ws.numel(), P(c.granted.data_ptr()), stream))
 
-    def _advance(self):
-        """The position that the argmax kernel moves on (a paged cache's lengths moved with its pages)."""
-        return None if self.paged is not None else P(self.pos.data_ptr())
+    def _next_tokens(self, h, stream) -> None:
+        """The greedy tokens and their embeddings; the position moves on with them. A paged cache's lengths moved with
+        its pages, and a sequence that they gave no place keeps its token."""
+        s, c = self.s, self.paged
+        N.check(N.lib().tn_llama_argmax_embed_granted(
+            P(self.logits.data_ptr()), self.B, s.vocab, P(self.tokens.data_ptr()), P(self.embed.data_ptr()), s.hidden,
+            P(h.data_ptr()), P(self.pos.data_ptr()) if c is None else None,
+            None if c is None else P(c.granted.data_ptr()), stream))
 
     @staticmethod
     def _stream():
@@ -572,7 +577,10 @@ class Q4LlamaDecoder:
         """One token for every sequence: reads tokens' embeddings in self.h and
         the position self.pos (a paged cache: its lengths); leaves the next
         tokens in self.tokens, their embeddings in self.h, and the position
-        advanced by one. Of an idle sequence of a paged cache they mean nothing."""
+        advanced by one. An idle sequence of a paged cache keeps its token. Where
+        the cache has no place for every sequence's token, none gets one: the step
+        leaves cache, lengths, tokens and embeddings as they were, and
+        self.paged.check() raises."""
         if self._mega is not None:
             return self._step_mega(stream or self._stream())
         if self.paged is not None:
@@ -617,9 +625,7 @@ class Q4LlamaDecoder:
         self._norm(self.delta, self.final_norm, stream)
         self._linear(self.lm_head, self.logits_l, self.v_l, s.hidden, stream)
         self._gather(self.logits_l, self.logits, 4 * self.n_layers, stream)
-        N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
-                                        P(self.embed.data_ptr()), s.hidden, P(self.h.data_ptr()),
-                                        self._advance(), stream))
+        self._next_tokens(self.h, stream)
         self._step_end(stream)
 
     def _fused_linear(self, mode, x, x_stride, delta, h_out, norm_w, w, y, n, k, stream, flags=0, link=None,
@@ -678,9 +684,7 @@ class Q4LlamaDecoder:
         self._fused_linear(N.TN_X_RMSNORM, ha, H, self.delta, hb, self.final_norm, self.lm_head, self.logits_l,
                            self.v_l, H, stream)
         self._gather(self.logits_l, self.logits, 0, stream)
-        N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
-                                        P(self.embed.data_ptr()), s.hidden, P(ha.data_ptr()),
-                                        self._advance(), stream))
+        self._next_tokens(ha, stream)
         self._step_end(stream)
 
     def _step_rowwise_rows(self, stream) -> None:
@@ -722,9 +726,7 @@ class Q4LlamaDecoder:
         self._norm(self.delta, self.final_norm, stream)
         self._linear(self.lm_head, self.logits_l, self.v_l, H, stream)
         self._gather(self.logits_l, self.logits, 0, stream)
-        N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
-                                        P(self.embed.data_ptr()), s.hidden, P(self.h.data_ptr()),
-                                        self._advance(), stream))
+        self._next_tokens(self.h, stream)
         self._step_end(stream)
 
     def _step_fused(self, stream) -> None:
@@ -789,9 +791,7 @@ class Q4LlamaDecoder:
         self._fused_linear(N.TN_X_RMSNORM, ha, H, self.delta, hb, self.final_norm, self.lm_head, self.logits_l,
                            self.v_l, H, stream, link=links[("lm_head", 0)] if fg else None)
         self._gather(self.logits_l, self.logits, 4 * self.n_layers, stream)
-        N.check(L.tn_llama_argmax_embed(P(self.logits.data_ptr()), B, s.vocab, P(self.tokens.data_ptr()),
-                                        P(self.embed.data_ptr()), s.hidden, P(ha.data_ptr()),
-                                        self._advance(), stream))
+        self._next_tokens(ha, stream)
         self._step_end(stream)
 
     def _build_links(self) -> dict:
