@@ -454,7 +454,10 @@ TN_API int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strides, 
  * tn_q8_0_quantize_planar). A request of length 0 appends nothing and gives
  * zeros, and so does one with granted[b] <= 0 (granted: of the resize before;
  * NULL: every request's length counts its new token). Without `granted` a step
- * behind a resize that was refused writes over the last cached tokens.
+ * behind a resize that was refused writes over the last cached tokens. A token
+ * whose position lies outside the page table or the rotary table is left out and
+ * reported, and its request gives zeros; one whose page is not of the pool is
+ * left out and reported, and its request attends its other keys.
  * out [requests][heads][head_dim]; heads / kv_heads <= 8. */
 TN_API int tn_sdpa_q4_decode_step(const void *qkv, const void *rope, int64_t rope_rows, void *pool,
                                   int64_t num_pages, int64_t heads, int64_t kv_heads, int64_t head_dim,

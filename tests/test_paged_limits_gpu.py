@@ -4,6 +4,7 @@ leaves pools, lengths and tokens as they were, and the next call that can be goe
 import pytest
 import torch
 
+from tests.kv_q4_ref import State
 from tests.test_decode_paged_gpu import small, tokens
 from tests.test_kv_cache_gpu import rope_table
 from torchnative_b200 import _native as N
@@ -112,3 +113,33 @@ def test_granted_is_checked(cuda_device):
             kv.kv_pages_resize(*args, grow=1, granted=bad)
         with pytest.raises(error, match=match):
             kv.sdpa_q4_decode_step(*step, granted=bad)
+
+
+@pytest.mark.parametrize("what", ["rope", "table"])
+def test_a_token_without_a_place_is_left_out(cuda_device, what):
+    """Lengths beyond the rotary table, or beyond what the page table can name: nothing is appended, nothing that lies at
+    the place is read, and it is reported; the other requests are as they are without."""
+    st = State([40, 20, 48], 2, 64, 16, cuda_device)
+    qkv = st.randn(3, 8 * 64, dtype=BF)
+    rope = rope_table(50, 64, cuda_device)
+    table, lengths = st.table, st.lengths.clone()
+    if what == "rope":
+        rope, lost = rope[:39].contiguous(), [0, 2]  # positions 39 and 47
+    else:
+        lengths[0], lengths[2], lost = 49, 2**31 - 1, [0, 2]
+    own = st.pool.clone()
+    want = kv.sdpa_q4_decode_step(qkv[1:2].contiguous(), rope, own, table[1:2], lengths[1:2], 4)
+    for fill in (None, 0xff):  # an unwritten place may hold anything: NaN scales among it
+        pool = st.pool.clone()
+        if fill is not None:
+            pool[table[0].long(), :, 0] = fill
+            pool[table[2].long(), :, 0] = fill
+        before = pool.clone()
+        out = kv.sdpa_q4_decode_step(qkv, rope, pool, table, lengths, 4)
+        with pytest.raises(RuntimeError, match="position"):
+            N.device_status()
+        assert (out[lost] == 0).all() and torch.equal(out[1:2], want)
+        for b in (0, 2):
+            pages = table[b].long()
+            assert torch.equal(pool[pages], before[pages])
+        assert torch.equal(pool[table[1, 1]], own[table[1, 1]])

@@ -123,15 +123,20 @@ struct Split {
     uint32_t f16_1024, f16_64;  // 1024 and 64 as half2: here so that the compiler keeps them in registers
     // decode step
     const __nv_bfloat16 *qkv, *rope;
-    int64_t rope_rows;
+    int places;  // positions that a new token may have: the table's, and the rotary table's
     int8_t *codes;
     float *scales, *offsets;
     const int *granted;  // [requests] new tokens that the resize gave, or NULL: one to each
     // The tokens of request b, its new one among them: none where the resize gave none, so that nothing is appended
-    // over what the cache holds.
-    __device__ __forceinline__ int step_length(int b) const {
-        if (granted && granted[b] <= 0) return 0;
-        return a.c.length(b);
+    // over what the cache holds, and none where the new one has no place (`lost`), so that what lies there is not read.
+    __device__ __forceinline__ int step_length(int b, bool *lost) const {
+        const int n = a.c.lengths[b];
+        *lost = n > places;
+        if (granted && granted[b] <= 0) {
+            *lost = false;
+            return 0;
+        }
+        return n < 0 || *lost ? 0 : n;
     }
 };
 
@@ -159,7 +164,8 @@ struct Cursor {
 
     __device__ __forceinline__ void load_request(const Split &s) {
         const Attend &p = s.a;
-        S = STEP ? s.step_length(b) : p.c.length(b);
+        bool lost;
+        S = STEP ? s.step_length(b, &lost) : p.c.length(b);
         n = p.query_tokens(b, &first);
         tiles = (n * p.rep + RT - 1) / RT;
     }
@@ -227,10 +233,13 @@ __device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos
     const Attend &a = p.a;
     const int lane = threadIdx.x & 31, t = lane & 3, block = (lane >> 2) % NB, is_v = (lane >> 2) / NB % 2;
     uint8_t *group = nullptr;
-    if (pos >= p.rope_rows)
-        record_device_error(a.c.err, DEV_ERR_BAD_PAGE);
-    else if (pos >= 0)
+    if (pos >= 0) {
         group = a.c.group<D>(b, h, pos >> 4);
+    } else {
+        bool lost;
+        p.step_length(b, &lost);
+        if (lost) record_device_error(a.c.err, DEV_ERR_BAD_PAGE);
+    }
     if (lane == 0) added.key = group ? pos & 15 : -1;
     if (!group) return;
     const __nv_bfloat16 *row = p.qkv + ((int64_t)b * (a.heads + 2 * a.c.kv_heads) + a.heads + (is_v ? a.c.kv_heads : 0) + h) * D;
@@ -379,8 +388,7 @@ __device__ __forceinline__ void load_queries(const Split &p, const Cursor<8 * NT
             for (int b = 0; b < D / 32; ++b) load8<T>(src + b * 32 + lt * 8, x[nt][b]);
         }
         if constexpr (STEP) {
-            const int64_t pos = max((int64_t)0, min((int64_t)at.S - 1, p.rope_rows - 1));
-            rotate<D>(p.rope + pos * D, lt, x[nt]);
+            rotate<D>(p.rope + (int64_t)max(0, at.S - 1) * D, lt, x[nt]);
         }
     }
 }
@@ -1301,7 +1309,7 @@ extern "C" int tn_sdpa_q4_decode_step_granted(const void *qkv, const void *rope,
     p.a = {nullptr, 0, 0, c, nullptr, out, lse, (int)requests, (int)heads, (int)(heads / kv_heads), sc};
     p.qkv = (const __nv_bfloat16 *)qkv;
     p.rope = (const __nv_bfloat16 *)rope;
-    p.rope_rows = rope_rows;
+    p.places = (int)std::min<int64_t>(max_pages << c.page_shift, rope_rows);
     p.codes = codes;
     p.scales = scales;
     p.offsets = offsets;

@@ -297,7 +297,9 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
     activations. A request of length 0 appends nothing and gives zeros, and so
     does one with granted[b] <= 0: pass what the resize before granted. Without
     it every length counts a new token, and a step behind a resize that could
-    not be met writes over the last cached ones."""
+    not be met writes over the last cached ones. A position outside the page
+    table or `rope` is reported (`PagedQ4Cache.check`); its request appends
+    nothing and gives zeros."""
     op = "sdpa_q4_decode_step"
     device, index = qkv.device, qkv.get_device()
     if not (index >= 0 and qkv.dtype is rope.dtype is _BF16 and pool.dtype is _U8
