@@ -143,3 +143,28 @@ def test_a_token_without_a_place_is_left_out(cuda_device, what):
             pages = table[b].long()
             assert torch.equal(pool[pages], before[pages])
         assert torch.equal(pool[table[1, 1]], own[table[1, 1]])
+
+
+@pytest.mark.parametrize("batch", [2, 6])
+def test_a_capacity_that_ends_inside_a_page(cuda_device, batch):
+    """The last page's places beyond the capacity are places like others: tokens there are those of a larger engine."""
+    from torchnative_b200.llama_decode import LlamaShape, Q4LlamaDecoder
+
+    shape = LlamaShape(hidden=512, inter=1024, heads=8, kv_heads=2, head_dim=64, vocab=2048, layers=2, rope_theta=10000.0)
+    runs = []
+    for capacity in (70, 80):
+        dec = Q4LlamaDecoder(shape, batch=batch, capacity=capacity, device=cuda_device, seed=12, kv_cache="q4_0", page_size=16)
+        dec.fill_prompt_cache([66] + [9] * (batch - 1))
+        dec.start(tokens(batch, cuda_device))
+        runs.append([])
+        for _ in range(14):
+            dec.step()
+            runs[-1].append(dec.tokens.tolist())
+        dec.paged.check()
+        assert dec.paged.lengths.tolist() == [80] + [23] * (batch - 1)
+        runs[-1].append([p.cpu() for p in dec.paged.pools])
+        dec.step()  # the page's end
+        with pytest.raises(RuntimeError, match="length"):
+            dec.paged.check()
+    assert runs[0][:-1] == runs[1][:-1]
+    assert all(torch.equal(a, b) for a, b in zip(runs[0][-1], runs[1][-1]))

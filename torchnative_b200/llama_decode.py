@@ -183,7 +183,8 @@ class Q4LlamaDecoder:
             per_request = -(-capacity // page_size)
             self.paged = PagedQ4Cache(self.n_layers, self.hkv, s.head_dim, batch * per_request, batch, per_request,
                                       page_size, dev)
-            self.rope = rope_table(capacity, s.head_dim, s.rope_theta).to(dev)
+            # of every place that a sequence's pages have: the last page may reach beyond `capacity`
+            self.rope = rope_table(per_request * page_size, s.head_dim, s.rope_theta).to(dev)
             # what a step's resize writes, and the attention's scratch: at fixed addresses, for the captured step
             self._slots = torch.empty(batch, device=dev, dtype=torch.int64)
             self._positions = torch.empty(batch, device=dev, dtype=torch.int32)
