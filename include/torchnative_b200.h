@@ -71,8 +71,9 @@ TN_API int tn_device_info(int device, int *sm_count, int *cc_major, int *cc_mino
 
 /* Synchronises the current device and reads its device-side error word: every
  * spin-wait in these kernels is bounded, and a wait that gives up records a
- * code there and returns instead of hanging. TN_ERR_TIMEOUT if set (cleared
- * when reset != 0). No reference counterpart (candle's kernels never wait). */
+ * code there and returns instead of hanging. TN_ERR_TIMEOUT if set;
+ * TN_ERR_INVALID if a paged KV cache call met an id outside its tables, which
+ * has a word of its own that no wait looks at (both cleared when reset != 0). No reference counterpart (candle's kernels never wait). */
 TN_API int tn_device_status(int reset);
 
 /* The budget (GPU clock cycles, default 2^31, ~1 s) that every bounded wait of

@@ -168,3 +168,62 @@ def test_a_capacity_that_ends_inside_a_page(cuda_device, batch):
             dec.paged.check()
     assert runs[0][:-1] == runs[1][:-1]
     assert all(torch.equal(a, b) for a, b in zip(runs[0][-1], runs[1][-1]))
+
+
+def bad_slot(device):
+    pool = kv.kv_q4_pool(1, 1, 64, 16, device)
+    x = torch.ones((1, 1, 64), device=device)
+    kv.kv_q4_append(x, x, pool, torch.tensor([16], device=device))
+
+
+def test_a_bad_slot_stops_no_other_kernel(cuda_device):
+    """The persistent decode kernel, whose waits end early once one has given up, beside a reported slot."""
+    from torchnative_b200.llama_decode import LLAMA3_8B, Q4LlamaDecoder
+
+    dec = Q4LlamaDecoder(LLAMA3_8B, batch=1, capacity=64, device=cuda_device, seed=3, layers=1, mega=True)
+    runs = []
+    for bad in (False, True):
+        dec.fill_prompt_cache(40)
+        dec.start(torch.tensor([17], device=cuda_device))
+        if bad:
+            bad_slot(cuda_device)
+        runs.append([])
+        for _ in range(3):
+            dec.step()
+            runs[-1].append((dec.tokens.item(), dec.logits.clone()))
+    with pytest.raises(RuntimeError, match="slot"):
+        N.device_status()
+    N.device_status()
+    dec.close()
+    assert all(a[0] == b[0] and torch.equal(a[1], b[1]) for a, b in zip(*runs))
+
+
+def test_a_bad_slot_hides_no_timeout(cuda_device):
+    """A gather whose peer never signals, its wait cut to about 1 ms, behind a slot that was reported: both are told, the
+    timeout by its status, and both are cleared."""
+    import ctypes
+
+    lib = N.lib()
+    N.device_status()
+    regions = []
+    for _ in range(2):
+        base, handle = ctypes.c_void_p(), (ctypes.c_uint8 * 64)()
+        N.check(lib.tn_tp_region_alloc(1 << 16, ctypes.byref(base), handle))
+        regions.append(base)
+    bases = (ctypes.c_void_p * 2)(*[r.value for r in regions])
+    local = torch.ones((1, 64), dtype=BF, device=cuda_device)
+    prev = N.set_wait_budget(2_000_000)
+    try:
+        bad_slot(cuda_device)
+        N.check(lib.tn_tp_allgather(bases, 0, 2, local.data_ptr(), 64, 1, 64, 0, 128, 0,
+                                    torch.cuda.current_stream().cuda_stream))
+        cache = kv.PagedQ4Cache(1, 1, 64, 1, 1, 1, 16, cuda_device)
+        cache.resize(0, new_lengths=i32([17], cuda_device))
+        with pytest.raises(TimeoutError, match="length.*gave up.*slot"):
+            cache.check()
+        cache.check()
+    finally:
+        N.set_wait_budget(prev)
+        torch.cuda.synchronize()
+        for base in regions:
+            lib.tn_tp_region_free(base)

@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads) kv_q4_append_kernel(const Append p) 
     const uint32_t vw2 = __shfl_xor_sync(0xffffffffu, vw, ROW_LANES);
     const int64_t slot2 = __shfl_xor_sync(0xffffffffu, slot, ROW_LANES);
     if (slot >= p.num_slots) {  // never followed
-        record_device_error(p.err, DEV_ERR_BAD_PAGE);
+        record_bad_page(p.err);
         return;
     }
     if (slot < 0) return;

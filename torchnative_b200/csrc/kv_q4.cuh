@@ -66,7 +66,7 @@ struct KvPool {
         return n < 0 ? 0 : (n > cap ? (int)cap : n);
     }
     // The group of tokens [16 group, 16 group + 16) of request b, or NULL (and
-    // the device error word set) where the table names no page of the pool.
+    // the word for bad pages set) where the table names no page of the pool.
     // (A pool holds fewer than 2^31 groups: 4.9 TB.)
     template <int D>
     __device__ __forceinline__ uint8_t *group(int b, int kvh, int group) const {
@@ -76,7 +76,7 @@ struct KvPool {
     __device__ __forceinline__ uint8_t *group_of_row(const int *row, int kvh, int group) const {
         const int shift = page_shift - 4, page = row[group >> shift];
         if ((unsigned)page >= (unsigned)num_pages) {
-            record_device_error(err, DEV_ERR_BAD_PAGE);
+            record_bad_page(err);
             return nullptr;
         }
         return pool + (int64_t)(((page * kv_heads + kvh) << shift) + (group & ((1 << shift) - 1))) * KvQ4<D>::GROUP_BYTES;

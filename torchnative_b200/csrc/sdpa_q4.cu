@@ -238,7 +238,7 @@ __device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos
     } else {
         bool lost;
         p.step_length(b, &lost);
-        if (lost) record_device_error(a.c.err, DEV_ERR_BAD_PAGE);
+        if (lost) record_bad_page(a.c.err);
     }
     if (lane == 0) added.key = group ? pos & 15 : -1;
     if (!group) return;

@@ -52,8 +52,7 @@ enum : int {
     DEV_ERR_NONE = 0,
     DEV_ERR_WAIT_FULL = 1,
     DEV_ERR_WAIT_EMPTY = 2,
-    DEV_ERR_DRAIN = 3,
-    DEV_ERR_BAD_PAGE = 4  // a page id, slot or position outside what the call was given: skipped, never followed
+    DEV_ERR_DRAIN = 3
 };
 
 // ~2^31 cycles (~1 s at 1.9 GHz) before a wait gives up: the default of the
@@ -152,6 +151,9 @@ __device__ __forceinline__ uint64_t policy_evict_first() {
 __device__ __forceinline__ void record_device_error(int *word, int code) {
     if (word) atomicCAS(word, 0, code);
 }
+// A page id, slot or position outside what the call was given: skipped, never followed. It has a word of its own
+// behind the error word, since waits stop where that is set, and this is no reason to.
+__device__ __forceinline__ void record_bad_page(int *err) { record_device_error(err ? err + 1 : nullptr, 1); }
 
 // ---- tensor-parallel exchange regions (tp_comm.cu, and the GEMV epilogue
 // that scatters its output rows straight into every rank's region) --------

@@ -25,11 +25,12 @@ FactsSlot g_facts[kMaxDevices];
 std::mutex g_facts_mu;
 
 // Device-side words of each GPU: the error code set by kernels whose bounded
-// waits gave up, and the wait budget (clock cycles) those waits allow. Kernels
-// reach both through the `int *err` they are given (budget at err + 2).
+// waits gave up, whether a paged KV cache call met an id outside its tables, and
+// the wait budget (clock cycles) those waits allow. Kernels reach them through
+// the `int *err` they are given (bad_page at err + 1, budget at err + 2).
 struct DeviceWords {
     int err;
-    int pad;
+    int bad_page;
     long long wait_budget;
 };
 __device__ DeviceWords g_device_error = {0, 0, tn::kWaitBudgetCycles};
@@ -223,19 +224,19 @@ int tn_device_status(int reset) {
     if (!w) return tn::set_error(TN_ERR_CUDA, "tn_device_status: no device error word");
     int st = tn::check_cuda(cudaDeviceSynchronize(), "tn_device_status", "cudaDeviceSynchronize");
     if (st) return st;
-    int v = 0;
-    st = tn::check_cuda(cudaMemcpy(&v, w, sizeof(int), cudaMemcpyDeviceToHost), "tn_device_status", "read");
+    int v[2] = {0, 0};  // the error word, the bad-page word
+    st = tn::check_cuda(cudaMemcpy(v, w, sizeof(v), cudaMemcpyDeviceToHost), "tn_device_status", "read");
     if (st) return st;
-    if (reset && v) {
-        int zero = 0;
-        cudaMemcpy(w, &zero, sizeof(int), cudaMemcpyHostToDevice);
+    if (reset && (v[0] || v[1])) {
+        const int zero[2] = {0, 0};
+        cudaMemcpy(w, zero, sizeof(zero), cudaMemcpyHostToDevice);
     }
-    if (v == tn::DEV_ERR_BAD_PAGE)
-        return tn::set_error(TN_ERR_INVALID, "torchnative_b200: a paged KV cache call met a page id, slot or position "
-                                             "outside its pool or tables (that token was skipped)");
-    if (v)
+    const std::string page("a paged KV cache call met a page id, slot or position outside its pool or tables (that token "
+                           "was skipped)");
+    if (v[0])
         return tn::set_error(TN_ERR_TIMEOUT, "torchnative_b200: a kernel's bounded wait gave up (device code " +
-                                                 std::to_string(v) + ")");
+                                                 std::to_string(v[0]) + ")" + (v[1] ? "; " + page : ""));
+    if (v[1]) return tn::set_error(TN_ERR_INVALID, "torchnative_b200: " + page);
     return TN_OK;
 }
 

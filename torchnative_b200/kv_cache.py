@@ -405,10 +405,19 @@ class PagedQ4Cache:
                                    q8=q8, granted=self.granted)
 
     def check(self) -> None:
-        """Wait for the GPU and raise for a resize that could not be met since
-        the last check, or a page, slot or position outside its range."""
-        code = int(self.status.item())
-        self.status.zero_()
+        """Wait for the cache's GPU and raise for a resize that could not be met
+        since the last check, a page, slot or position outside its range, or a
+        wait that gave up; all of it is read and cleared before one is raised."""
+        with torch.cuda.device(self.status.device):
+            met = None
+            try:
+                N.device_status()
+            except (RuntimeError, TimeoutError) as e:
+                met = e
+            code = int(self.status.item())
+            self.status.zero_()
+        refused = f"kv_pages_resize: {_STATUS.get(code, code)}; that call changed nothing"
+        if met is not None:
+            raise type(met)(f"{refused}; {met}" if code else str(met))
         if code:
-            raise RuntimeError(f"kv_pages_resize: {_STATUS.get(code, code)}; that call changed nothing")
-        N.device_status()
+            raise RuntimeError(refused)
