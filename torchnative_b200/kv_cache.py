@@ -67,21 +67,7 @@ def _call(index: int, name: str, *args) -> None:
 
 
 _empty_like, _contiguous = torch.empty_like, torch.contiguous_format
-_templates: dict = {}
-
-
-def _empty(dtype: torch.dtype, *place) -> torch.Tensor:
-    """torch.empty on place = (device index, *shape); like a template without
-    memory of its own, it takes half the host's time."""
-    shapes = _templates.get(dtype)
-    if shapes is None:
-        shapes = _templates[dtype] = {}
-    t = shapes.get(place)
-    if t is None:
-        if len(shapes) >= 1024:
-            shapes.clear()
-        t = shapes[place] = torch.empty(1, dtype=dtype, device=torch.device("cuda", place[0])).expand(place[1:])
-    return _empty_like(t, memory_format=_contiguous)
+_empty_strided = torch.empty_strided  # on the host half of torch.empty's time
 
 
 _scratch: dict = {}
@@ -90,14 +76,19 @@ _scratch: dict = {}
 def _workspace(device: torch.device, index: int, rows: int, dim: int, *shape: int) -> torch.Tensor:
     """The attention calls' scratch: one a stream, since calls on a stream run
     one after the other; a captured call gets memory of its graph's own, since
-    graphs captured on one stream may be replayed on several."""
+    graphs captured on one stream may be replayed on several. What a dispatch
+    mode gives instead of memory (a fake tensor) is not kept."""
     key = (index, _current_stream(index), rows > 8, dim)
     ws = _scratch.get(key)
-    capturing = _capturing()
+    if index == _current_device():
+        capturing = _capturing()
+    else:
+        with torch.cuda.device(index):
+            capturing = _capturing()
     if ws is None or capturing:
         tokens, heads, kv_heads, most = shape
         ws = torch.empty(N.lib().tn_sdpa_q4_workspace_bytes(tokens, heads, kv_heads, dim, most), dtype=_U8, device=device)
-        if not capturing:
+        if not capturing and type(ws) is torch.Tensor:
             _scratch[key] = ws
     return ws
 
@@ -113,7 +104,10 @@ def _granted(op: str, device: torch.device, granted: torch.Tensor, lengths: torc
     _require(op, device, "granted", granted, _I32)
     if granted.shape != lengths.shape:
         raise RuntimeError(f"{op}: granted {list(granted.shape)} does not fit lengths {list(lengths.shape)}")
-    return granted.data_ptr()
+    address = granted.data_ptr()
+    if not address and granted.numel():
+        raise RuntimeError(f"{op}: granted has no memory (a fake tensor)")
+    return address
 
 
 def _pool_shape(op: str, pool: torch.Tensor):
@@ -171,9 +165,9 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
         new = new_lengths.data_ptr()
     if granted is not None:
         granted = _granted(op, device, granted, lengths)
-    slots = _empty(_I64, index, max_tokens)
-    positions = _empty(_I32, index, max_tokens)
-    query_start = _empty(_I32, index, requests + 1)
+    slots = _empty_strided((max_tokens,), (1,), dtype=_I64, device=device)
+    positions = _empty_strided((max_tokens,), (1,), dtype=_I32, device=device)
+    query_start = _empty_strided((requests + 1,), (1,), dtype=_I32, device=device)
     _call(index, "tn_kv_pages_resize_granted", page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), new,
           int(grow), requests, free_pages.data_ptr(), free_count.data_ptr(), free_pages.shape[0], page_size,
           slots.data_ptr(), positions.data_ptr(), max_tokens, query_start.data_ptr(), status.data_ptr(),
@@ -277,7 +271,7 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
         most = tokens if max_tokens is None else max(1, min(max_tokens, tokens))
     query = _rows(query)
     out = _empty_like(query, memory_format=_contiguous)
-    lse = _empty(_F32, index, tokens, heads)
+    lse = _empty_strided((tokens, heads), (heads, 1), dtype=_F32, device=device)
     ws = _workspace(device, index, heads // kv_heads * most, dim, tokens, heads, kv_heads, most)
     _call(index, "tn_sdpa_q4_cache", query.data_ptr(), code, _row_strides(query), tokens, heads, pool.data_ptr(),
           pages, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
@@ -332,7 +326,7 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
         codes, scales, offsets = codes.data_ptr(), scales.data_ptr(), offsets.data_ptr()
     if granted is not None:
         granted = _granted(op, device, granted, lengths)
-    out = _empty(_BF16, index, requests, heads, dim)
+    out = _empty_strided((requests, heads, dim), (heads * dim, dim, 1), dtype=_BF16, device=device)
     ws = _workspace(device, index, heads // kv_heads, dim, requests, heads, kv_heads, 1)
     _call(index, "tn_sdpa_q4_decode_step_granted", qkv.data_ptr(), rope.data_ptr(), rope.shape[0], pool.data_ptr(), pages,
           heads, kv_heads, dim, page_size, page_table.data_ptr(), max_pages, max_pages, lengths.data_ptr(), requests,
