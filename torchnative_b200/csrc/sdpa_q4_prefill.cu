@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *where = reinterpret_cast<volatile int *>(tmem_slot + 2);  // request, pair of tiles
+    int *odd_tiles = reinterpret_cast<int *>(tmem_slot + 4);  // first and last with value scales that are not finite
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     pdl_launch_dependents();
@@ -226,6 +227,8 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
         for (int i = 0; i < NINFO; ++i) mbar_init(&info_full[i], 8);
         mbar_init(mma_done, 1);
         *abort = 0;
+        odd_tiles[0] = INT32_MAX;
+        odd_tiles[1] = -1;
         fence_mbar_init();
     }
     __syncthreads();
@@ -263,14 +266,34 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             auto load = [&](int piece) { x.load(a.c, table, head, 4 * (piece >> 3) + (piece & 3), piece & 4, S, lane); };
             if (warp - 9 < pieces) load(warp - 9);
             for (int piece = warp - 9; piece < pieces; piece += UNPACKERS) {
-                const Words<D> y = x;
+                Words<D> y = x;
                 if (piece + UNPACKERS < pieces) load(piece + UNPACKERS);
                 const int j = piece >> 3, w = piece & 3, slot = j % NINFO, ks = j % NK, vs = j % NV;
                 // the group's power of two
                 int e = 1;
 #pragma unroll
                 for (int c = 0; c < NB / 2; ++c) e = most_exponent(most_exponent(e, y.scales[0][c]), y.scales[1][c]);
-                e = min((int)__reduce_max_sync(0xffffffffu, (unsigned)e), 30);
+                e = (int)__reduce_max_sync(0xffffffffu, (unsigned)e);
+                const bool odd = e > 30;
+                if (odd) {
+                    // infinite and NaN scales. A score that is not finite is its own row's matter; a value times 0 would
+                    // reach the rows that do not see it, so it counts as 0 here, and what it adds to the others' results
+                    // comes in at the end.
+                    e = 30;
+                    if (piece & 4) {
+                        e = 1;
+#pragma unroll
+                        for (int c = 0; c < NB / 2; ++c)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t w = y.scales[i][c];
+                                if ((w & 0x7c00u) == 0x7c00u) y.scales[i][c] &= 0xffff0000u;
+                                if ((w & 0x7c000000u) == 0x7c000000u) y.scales[i][c] &= 0xffffu;
+                                e = most_exponent(e, y.scales[i][c]);
+                            }
+                        e = (int)__reduce_max_sync(0xffffffffu, (unsigned)e);
+                    }
+                }
                 const uint32_t power = power_f16x2(e);
                 if (!(piece & 4)) {
                     if (j >= NK && !warp_wait(&k_empty[ks], (j / NK - 1) & 1, abort, a.c.err)) break;
@@ -304,6 +327,10 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                     if (lane == 0) mbar_arrive(&k_full[ks]);
                 } else {
                     if (lane == 0) {
+                        if (odd) {
+                            atomicMin(odd_tiles, j);
+                            atomicMax(odd_tiles + 1, j);
+                        }
                         info[slot].v[w] = (float)(e - 14);
                         info[slot].vinv[w] = __uint_as_float((uint32_t)(141 - e) << 23);
                         mbar_arrive(&info_full[slot]);
@@ -555,6 +582,8 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
             tc05::fence_after();
             const bool live = row < rows;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            // (of this row's tiles all is written: their info_full says so)
+            const int odd0 = *(volatile int *)odd_tiles, odd1 = *(volatile int *)(odd_tiles + 1);
             const int64_t at = (int64_t)(first + tok) * a.heads + head * a.rep + (row - tok * a.rep);
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -565,6 +594,23 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                }
+                if (live && odd1 >= odd0) {
+                    // the block's elements of the keys that were left out, as they are: infinite, or NaN
+                    const int *table = a.c.table + b * a.c.table_stride;
+#pragma unroll 1
+                    for (int key = odd0 * BN; key < min(sees, (odd1 + 1) * BN); ++key) {
+                        const uint8_t *src = a.c.group_of_row<D>(table, head, key >> 4);
+                        if (!src) continue;
+                        const float d = __half2float(*reinterpret_cast<const __half *>(src + KvQ4<D>::v_scale(key & 15, c)));
+                        if (fabsf(d) < INFINITY) continue;
+#pragma unroll
+                        for (int g = 0; g < 8; ++g) {
+                            const uint32_t w = *reinterpret_cast<const uint16_t *>(src + KvQ4<D>::v_half(key & 15, g, c));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[4 * g + i] = fmaf((float)(int)(w >> (4 * i) & 15) - 8.0f, d, v[4 * g + i]);
+                        }
+                    }
                 }
                 if (live) {
                     uint32_t w[16];
