@@ -280,6 +280,7 @@ __device__ __forceinline__ void patch_new(const NewToken<D> &added, uint8_t *buf
         *reinterpret_cast<__half *>(buf + Q::k_scale(key, lane)) = added.ks[lane];
         *reinterpret_cast<__half *>(buf + Q::v_scale(key, lane)) = added.vs[lane];
     }
+    fence_proxy_async_smem();  // before the bulk copy that the stage gets next
     __syncwarp();
 }
 
