@@ -227,3 +227,45 @@ def test_a_bad_slot_hides_no_timeout(cuda_device):
         torch.cuda.synchronize()
         for base in regions:
             lib.tn_tp_region_free(base)
+
+
+def test_caches_of_many_and_of_very_many_requests_at_the_same_time(cuda_device):
+    """Two host threads, whose calls need different amounts of shared memory; and a graph of the larger one that is made
+    before and replayed after a smaller call."""
+    import threading
+
+    caches = [kv.PagedQ4Cache(1, 1, 64, n, n, 1, 16, cuda_device) for n in (8192, 2600)]
+    new = [torch.ones_like(c.lengths) for c in caches]
+    gate, failed = threading.Barrier(2), []
+
+    def work(c, one):
+        try:
+            with torch.cuda.device(cuda_device), torch.cuda.stream(torch.cuda.Stream(cuda_device)):
+                zero = torch.zeros_like(one)
+                gate.wait(timeout=60)
+                for _ in range(300):
+                    c.resize(0, new_lengths=zero)
+                    c.resize(len(one), new_lengths=one)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 -- shown below
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=x) for x in zip(caches, new)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for c in caches:
+        c.check()
+        assert (c.lengths == 1).all() and c.free_count.item() == 0
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        caches[0].resize(8192, grow=1)
+    caches[1].resize(2600, grow=1)
+    graph.instantiate()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (caches[0].lengths == 2).all() and (caches[1].lengths == 2).all()
+    caches[0].check()

@@ -6,6 +6,7 @@
 // packed rows. All of it is prefix sums over the requests (pages given, pages
 // taken, tokens new), so the result does not depend on any order of execution.
 #include <algorithm>
+#include <atomic>
 
 #include "kv_q4.cuh"
 
@@ -322,10 +323,18 @@ extern "C" int tn_kv_pages_resize_granted(int *page_table, int64_t table_stride,
                  granted, ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0};
     const int smem = (int)((5 * requests + 2) * sizeof(int));
     if (smem > 48 * 1024 - 1024) {
-        int st = tn::check_cuda(
-            cudaFuncSetAttribute(tn::kv_pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-            "tn_kv_pages_resize", "cudaFuncSetAttribute");
+        // once a device, for the most requests: the limit is the kernel's, not the call's
+        static std::atomic<uint64_t> ready{0};  // a bit a device
+        int device = 0;
+        int st = tn::check_cuda(cudaGetDevice(&device), "tn_kv_pages_resize", "cudaGetDevice");
         if (st) return st;
+        if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
+            st = tn::check_cuda(cudaFuncSetAttribute(tn::kv_pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     (int)((5 * tn::kMaxRequests + 2) * sizeof(int))),
+                                "tn_kv_pages_resize", "cudaFuncSetAttribute");
+            if (st) return st;
+            ready.fetch_or(1ull << device, std::memory_order_relaxed);
+        }
     }
     cudaStream_t s = tn::stream_of(stream);
     const int64_t moves = new_lengths ? max_pages : std::min(max_pages, (grow >> shift) + 1);
