@@ -269,3 +269,28 @@ def test_caches_of_many_and_of_very_many_requests_at_the_same_time(cuda_device):
     torch.cuda.synchronize()
     assert (caches[0].lengths == 2).all() and (caches[1].lengths == 2).all()
     caches[0].check()
+
+
+def test_the_most_new_tokens_that_a_call_takes(cuda_device):
+    """2^31 - 1 of them (26 GB of slots and positions), into longer buffers whose ends stay as they were."""
+    most, tail = 2**31 - 1, 5
+    cache = kv.PagedQ4Cache(1, 1, 64, 8, 2, 4, 16, cuda_device)
+    slots = torch.full((most + tail,), 7, dtype=torch.int64, device=cuda_device)
+    positions = torch.full((most + tail,), 7, dtype=torch.int32, device=cuda_device)
+    start = torch.empty(3, dtype=torch.int32, device=cuda_device)
+    new = i32([33, 5], cuda_device)
+    for shift in (0, 1):  # in 16-byte vectors, and not
+        ahead = slots[:shift].clone(), positions[:shift].clone()
+        N.check(N.lib().tn_kv_pages_resize(
+            cache.page_table.data_ptr(), 4, 4, cache.lengths.data_ptr(), new.data_ptr(), 0, 2, cache.free_pages.data_ptr(),
+            cache.free_count.data_ptr(), 8, 16, slots.data_ptr() + 8 * shift, positions.data_ptr() + 4 * shift, most,
+            start.data_ptr(), cache.status.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        cache.check()
+        first, last = (x[shift:shift + 38].tolist() for x in (slots, positions))
+        rows = cache.page_table.tolist()
+        at = [(b, p) for b, n in enumerate([33, 5]) for p in range(n)]
+        assert first == [rows[b][p // 16] * 16 + p % 16 for b, p in at] and last == [p for _, p in at]
+        for x, y in zip((slots, positions), ahead):
+            assert (x[shift + 38:shift + 1000] == -1).all() and (x[most + shift - 5:most + shift] == -1).all()
+            assert (x[most + shift:] == 7).all() and torch.equal(x[:shift], y)
+        cache.resize(0, new_lengths=i32([0, 0], cuda_device))

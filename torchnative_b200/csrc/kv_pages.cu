@@ -259,10 +259,10 @@ __global__ void __launch_bounds__(256) kv_pages_slots_kernel(const Resize p) {
     const int B = p.requests;
     for (int b = threadIdx.x; b <= B; b += 256) sm[b] = p.query_start[b];
     __syncthreads();
-    const int r0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t r0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // r0 + 4 may be 2^31
     if (r0 >= p.max_tokens) return;
     const int tokens = sm[B];
-    int b = r0 < tokens ? find(sm, B, r0) : 0;
+    int b = r0 < tokens ? find(sm, B, (int)r0) : 0;
     int64_t slots[4];
     int positions[4];
 #pragma unroll
@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(256) kv_pages_slots_kernel(const Resize p) {
         slots[i] = -1;
         positions[i] = -1;
         if (r0 + i < tokens) {
-            while (sm[b + 1] <= r0 + i) ++b;
-            positions[i] = p.lengths[b] - (sm[b + 1] - (r0 + i));
+            const int r = (int)r0 + i;
+            while (sm[b + 1] <= r) ++b;
+            positions[i] = p.lengths[b] - (sm[b + 1] - r);
             slots[i] = slot_of(p, b, positions[i]);
         }
     }
