@@ -373,7 +373,8 @@ TN_API int tn_sdpa_decode_step_q8(const void *qkv, const float *inv_freq, void *
  * scales, in the order that the attention kernels read (kv_q4.cuh, with the bytes of a
  * group). page_size: a power of two from 16 to 1024; head_dim 64 or 128.
  * page_table: int32 [requests][table_stride], the first max_pages columns of
- * which may be used: the pages of each request in order, -1 where none.
+ * which may be used: the pages of each request in order, -1 where none;
+ * max_pages * page_size <= 2^31 - 1024.
  * lengths: int32 [requests], cached tokens. A length outside [0, max_pages *
  * page_size] counts as the nearer end. Page ids, slots and positions are device
  * data that no host check sees: one outside its range is never followed; its

@@ -307,7 +307,7 @@ extern "C" int tn_kv_pages_resize_granted(int *page_table, int64_t table_stride,
         return tn::set_error(TN_ERR_NOT_IMPLEMENTED, op + ": a page holds 16, 32, 64, 128, 256, 512 or 1024 tokens, got " +
                                                          std::to_string(page_size));
     if (requests < 0 || max_pages < 0 || table_stride < max_pages || num_pages < 0 || num_pages > INT32_MAX ||
-        max_tokens < 0 || max_tokens > INT32_MAX || max_pages > (int64_t)INT32_MAX >> shift)
+        max_tokens < 0 || max_tokens > INT32_MAX || max_pages > tn::kMaxRowTokens >> shift)
         return tn::set_error(TN_ERR_SHAPE, op + ": bad table, pool or token count");
     if (grow < 0 || grow > INT32_MAX)
         return tn::set_error(TN_ERR_SHAPE, op + ": grow must be a token count (new_lengths shrinks requests)");

@@ -29,6 +29,8 @@
 namespace tn {
 
 constexpr int kKvGroup = 16;
+// Tokens that a table's row may name: 32-bit positions with room for a tile behind the last one.
+constexpr int64_t kMaxRowTokens = ((int64_t)1 << 31) - 1024;
 
 template <int D>
 struct KvQ4 {

@@ -1214,7 +1214,7 @@ int check_cache(const char *op, const KvPool &c, int64_t requests, int64_t max_p
                 int64_t heads, int64_t kv_heads, int64_t tokens) {
     const std::string name(op);
     if (requests < 0 || requests > 65535 || max_pages < 0 || table_stride < max_pages ||
-        max_pages > (int64_t)INT32_MAX >> c.page_shift || tokens < 0 || tokens > INT32_MAX / 2)
+        max_pages > kMaxRowTokens >> c.page_shift || tokens < 0 || tokens > INT32_MAX / 2)
         return set_error(TN_ERR_SHAPE, name + ": bad request, table or token count");
     if (heads < 1 || heads > 65535 || heads % kv_heads != 0)
         return set_error(TN_ERR_SHAPE, name + ": query heads (" + std::to_string(heads) +
