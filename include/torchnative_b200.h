@@ -499,7 +499,8 @@ TN_API int tn_llama_rope_append(const void *qkv, const float *inv_freq, const in
                                 int64_t pos_host, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                 void *q_out, void *k_cache, void *v_cache, int64_t cache_b_stride,
                                 int64_t cache_h_stride, void *stream);
-/* tokens[r] = argmax(logits[r]) (first index of the maximum); h[r] = embed[tokens[r]];
+/* tokens[r] = argmax(logits[r]) (first index of the maximum, NaN below every
+ * number; 0 in a row of nothing but NaN); h[r] = embed[tokens[r]];
  * if pos_dev, *pos_dev += 1. With `granted` a row of granted[r] <= 0 keeps its token. */
 TN_API int tn_llama_argmax_embed(const void *logits, int64_t rows, int64_t V, int *tokens,
                                  const void *embed, int64_t H, void *h, int *pos_dev, void *stream);

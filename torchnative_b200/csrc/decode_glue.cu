@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(1024) argmax_embed_kernel(const __nv_bfloat16 
             if (ov > best || (ov == best && oi < idx)) best = ov, idx = oi;
         }
         if (lane == 0) {
+            if (idx >= V) idx = 0;  // a row of nothing but NaN has no maximum
             if (granted && granted[row] <= 0)
                 idx = tokens[row];
             else

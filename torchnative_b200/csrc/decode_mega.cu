@@ -1281,7 +1281,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_mega_kernel(const MegaPara
             if (ov > bv || (ov == bv && oi < bi)) bv = ov, bi = oi;
         }
         if (lane == 0) {
-            p.tokens[0] = bi;
+            p.tokens[0] = bi < p.V ? bi : 0;  // logits of nothing but NaN have no maximum
             p.pos[0] = pos + 1;
             __threadfence();
             atomicAdd(p.epoch, 1u);
