@@ -1179,6 +1179,7 @@ int launch_split(Split &p, void *workspace, cudaStream_t stream, const char *op)
         if (st) return st;
         ready.fetch_or(1ull << device, std::memory_order_relaxed);
     }
+    __atomic_fetch_add(&counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * (Shape<T, D, NT>::W + 4)), Shape<T, D, NT>::SMEM, stream, op, p);
 }
 
@@ -1264,7 +1265,6 @@ extern "C" int tn_sdpa_q4_cache(const void *q, int dtype, const int64_t *q_strid
     tn::Split p{};
     p.a = {q, q_strides[0], q_strides[1], c, query_start, out, lse, (int)tokens, (int)heads, (int)(heads / kv_heads), sc};
     __atomic_fetch_add(&tn::counters().sdpa_calls, 1ull, __ATOMIC_RELAXED);
-    __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     cudaStream_t s = tn::stream_of(stream);
     if (head_dim == 128)
         return dtype == TN_F32   ? tn::launch_attend<float, 128>(p, max_query, workspace, s)
@@ -1305,7 +1305,6 @@ extern "C" int tn_sdpa_q4_decode_step_granted(const void *qkv, const void *rope,
     if ((uintptr_t)workspace % 16)
         return tn::set_error(TN_ERR_INVALID, std::string(op) + ": the workspace must be 16-byte aligned");
     __atomic_fetch_add(&tn::counters().sdpa_calls, 1ull, __ATOMIC_RELAXED);
-    __atomic_fetch_add(&tn::counters().sdpa_decode_launches, 1ull, __ATOMIC_RELAXED);
     tn::Split p{};
     p.a = {nullptr, 0, 0, c, nullptr, out, lse, (int)requests, (int)heads, (int)(heads / kv_heads), sc};
     p.qkv = (const __nv_bfloat16 *)qkv;
