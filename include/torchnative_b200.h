@@ -394,7 +394,9 @@ TN_API int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t p
  * (request by request, packed): slots[r] = page * page_size + offset,
  * positions[r] = place in the request, and -1 for r from the last new token to
  * max_tokens; query_start [requests + 1] the first of each request's new
- * tokens. lengths, page_table, free_pages and *free_count are updated.
+ * tokens. lengths, page_table, free_pages and *free_count are updated. A new
+ * token whose page, in the table or from the stack, is not one of the pool's
+ * gets the slot -1 and is reported (tn_device_status).
  * A call that cannot be met changes none of them, gives no token a slot
  * (slots and positions -1, query_start 0) and sets *status, if that is 0, to
  * 1: not enough pages, 2: a length outside [0, max_pages * page_size], 3: more

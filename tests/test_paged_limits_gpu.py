@@ -294,3 +294,25 @@ def test_the_most_new_tokens_that_a_call_takes(cuda_device):
             assert (x[shift + 38:shift + 1000] == -1).all() and (x[most + shift - 5:most + shift] == -1).all()
             assert (x[most + shift:] == 7).all() and torch.equal(x[:shift], y)
         cache.resize(0, new_lengths=i32([0, 0], cuda_device))
+
+
+@pytest.mark.parametrize("tokens", [40, 5000])
+@pytest.mark.parametrize("bad", [-1, -7, 8, 1 << 30])
+def test_new_tokens_in_pages_that_are_none_are_reported(cuda_device, tokens, bad):
+    """A page id on the stack, or in the table, that is not one of the pool's: its tokens get no slot; the others theirs."""
+    for where in ("stack", "table"):
+        cache = kv.PagedQ4Cache(1, 1, 64, 8, 2, 4, 16, cuda_device)
+        cache.resize(40, new_lengths=i32([0, 20], cuda_device))
+        if where == "stack":
+            cache.free_pages[5] = bad  # the page that the first request takes
+        else:
+            cache.page_table[1, 1] = bad
+        slots, positions, _ = cache.resize(tokens, new_lengths=i32([5, 23], cuda_device))
+        first = [2 * 16 + i for i in range(5)] if where == "table" else [-1] * 5
+        second = [16 + i for i in range(4, 7)] if where == "stack" else [-1] * 3
+        assert slots[:8].tolist() == first + second
+        assert positions[:8].tolist() == [0, 1, 2, 3, 4, 20, 21, 22]
+        assert (slots[8:] == -1).all()
+        with pytest.raises(RuntimeError, match="page id"):
+            cache.check()
+        cache.check()

@@ -65,6 +65,7 @@ struct Resize {
     int *query_start, *status;
     int *granted;  // [requests] or NULL
     int aligned;  // slots and positions may be written in 16-byte vectors
+    int *err;
 };
 
 // Every thread of the cluster's CTAs, and what they wrote to global memory before; one CTA needs its own barrier only.
@@ -92,8 +93,13 @@ __device__ __forceinline__ int find(const int *starts, int n, int x) {
     return lo;
 }
 
+// A token's slot; -1, and reported, where the table names no page of the pool.
 __device__ __forceinline__ int64_t slot_of(const Resize &p, int b, int position) {
     const int page = p.table[b * p.table_stride + (position >> p.page_shift)];
+    if ((unsigned)page >= (unsigned)p.num_pages) {
+        record_bad_page(p.err);
+        return -1;
+    }
     return ((int64_t)page << p.page_shift) + (position & ((1 << p.page_shift) - 1));
 }
 
@@ -321,7 +327,7 @@ extern "C" int tn_kv_pages_resize_granted(int *page_table, int64_t table_stride,
         return tn::set_error(TN_ERR_INVALID, op + ": new_lengths must not be lengths");
     tn::Resize p{page_table, table_stride, (int)max_pages, lengths, new_lengths, (int)grow, (int)requests, free_pages,
                  free_count, (int)num_pages, shift, slots, positions, (int)max_tokens, query_start, status,
-                 granted, ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0};
+                 granted, ((uintptr_t)slots | (uintptr_t)positions) % 16 == 0, tn::device_error_word()};
     const int smem = (int)((5 * requests + 2) * sizeof(int));
     if (smem > 48 * 1024 - 1024) {
         // once a device, for the most requests: the limit is the kernel's, not the call's
