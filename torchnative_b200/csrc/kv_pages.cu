@@ -39,9 +39,11 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kMaxRequests = 8192;
-// Where more pages than this may move, a cluster of CTAs shares the moves; all of them compute the sums. It costs 1.2 us
-// (a step of 128 requests: 3.4 us, 4.5 in the cluster). 512 requests of up to 256 pages, of which 13,300 are taken and
-// 5,800 given, take 17.7 us in one CTA, 10.8 in the cluster; 256 requests of up to 64 pages 8.1 and 8.7, 512 10.5 and 9.2.
+// Where more pages than this may move, a cluster of CTAs shares the moves; all of them compute the sums. Two calls, there
+// and back, in one CTA and in the cluster: 512 requests of up to 256 pages, of which 13,300 are taken and 5,800 given, 42.7
+// and 20.1 us; 512 of up to 64 pages 21.9 and 18.0, 256 of them 16.4 and 17.0; a step of 128 requests 6.4 and 8.9. (A
+// thread moves one page at a time: four at once, for their loads, took 21.4 us where this takes 20.1, and 13.7 for 13.2
+// with 16 requests of 1000 pages in one CTA.)
 constexpr int64_t kMovesInOne = 16384;
 constexpr int kCtas = 8;
 // Up to here the launch that moves the pages writes the slots too; above, a second one over the whole GPU does (210,000
@@ -209,37 +211,17 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
         *p.free_count = top - (int)takes;
     }
     __syncthreads();
-    // Pages given back, the last one first, so that a roll-back leaves the stack as it was; then the pages taken. Of
-    // many, four neighbours a thread: one search, and four loads on their way at once.
-    const int each_give = gives > all ? 4 : 1, each_take = takes > all ? 4 : 1;
-    for (int i0 = me * each_give; i0 < (int)gives; i0 += all * each_give) {
-        int b = find(give_at, B, i0), page[4];
-        int64_t at[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k >= each_give || i0 + k >= (int)gives) continue;
-            while (give_at[b + 1] <= i0 + k) ++b;
-            at[k] = b * p.table_stride + pages_of(new_len[b], p.page_shift) + (i0 + k - give_at[b]);
-            page[k] = p.table[at[k]];
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k >= each_give || i0 + k >= (int)gives) continue;
-            p.free_pages[top - 1 - i0 - k] = page[k];
-            p.table[at[k]] = -1;
-        }
+    // Pages given back, the last one first, so that a roll-back leaves the stack as it was; then the pages taken.
+    for (int i = me; i < (int)gives; i += all) {
+        const int b = find(give_at, B, i);
+        int *at = p.table + b * p.table_stride + pages_of(new_len[b], p.page_shift) + (i - give_at[b]);
+        p.free_pages[top - 1 - i] = *at;
+        *at = -1;
     }
     sync_all(ctas);
-    for (int i0 = me * each_take; i0 < (int)takes; i0 += all * each_take) {
-        int b = find(take_at, B, i0), page[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) page[k] = k < each_take && i0 + k < (int)takes ? p.free_pages[top - 1 - i0 - k] : -1;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k >= each_take || i0 + k >= (int)takes) continue;
-            while (take_at[b + 1] <= i0 + k) ++b;
-            p.table[b * p.table_stride + pages_of(old_len[b], p.page_shift) + (i0 + k - take_at[b])] = page[k];
-        }
+    for (int i = me; i < (int)takes; i += all) {
+        const int b = find(take_at, B, i);
+        p.table[b * p.table_stride + pages_of(old_len[b], p.page_shift) + (i - take_at[b])] = p.free_pages[top - 1 - i];
     }
     if (p.max_tokens > kSlotsInOne) return;
     sync_all(ctas);
