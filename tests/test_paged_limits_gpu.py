@@ -316,3 +316,16 @@ def test_new_tokens_in_pages_that_are_none_are_reported(cuda_device, tokens, bad
         with pytest.raises(RuntimeError, match="page id"):
             cache.check()
         cache.check()
+
+
+def test_a_pool_without_heads_is_refused(cuda_device):
+    pool = torch.zeros((4, 0, 1, 18 * 64), dtype=torch.uint8, device=cuda_device)
+    table, lengths = i32([[0], [1]], cuda_device), i32([3, 4], cuda_device)
+    with pytest.raises(RuntimeError, match="multiple of"):
+        kv.sdpa_q4_cache(torch.zeros((2, 4, 64), device=cuda_device), pool, table, lengths)
+    with pytest.raises(RuntimeError, match="multiple of"):
+        kv.sdpa_q4_decode_step(torch.zeros((2, 256), dtype=BF, device=cuda_device), rope_table(9, 64, cuda_device), pool, table,
+                               lengths, 4)
+    x = torch.zeros((2, 0, 64), device=cuda_device)
+    with pytest.raises(RuntimeError, match="head count"):
+        kv.kv_q4_append(x, x, pool, torch.zeros(2, dtype=torch.int64, device=cuda_device))

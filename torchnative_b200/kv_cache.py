@@ -240,7 +240,8 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
     its lengths[b] cached tokens, and each sees the tokens up to its own. A
     token that sees none gives zeros and logsumexp 0; rows behind the last
     request's are not written. `max_tokens`, a bound on one request's query
-    tokens, chooses the kernel (None: all of them)."""
+    tokens, chooses the kernel (None: all of them). A `scale` of 0 or less, as
+    none, is 1 / sqrt(D), as in the dense operator; gradients do not pass."""
     op = "sdpa_q4_cache"
     device, index = query.device, query.get_device()
     code = _CODE.get(query.dtype)
@@ -258,7 +259,7 @@ def sdpa_q4_cache(query: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
     if query.dim() != 3 or query.shape[2] != dim:
         raise RuntimeError(f"{op}: query {list(query.shape)} must be [tokens, heads, {dim}]")
     tokens, heads, _ = query.shape
-    if heads == 0 or heads % kv_heads:
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
     start, most = None, 1
     if query_start is not None:
@@ -308,7 +309,7 @@ def sdpa_q4_decode_step(qkv: torch.Tensor, rope: torch.Tensor, pool: torch.Tenso
         _require(op, device, "lengths", lengths, _I32)
     pages, kv_heads, page_size, dim = _pool_shape(op, pool)
     requests, max_pages = _table_shape(op, page_table, lengths)
-    if heads <= 0 or heads % kv_heads:
+    if heads <= 0 or kv_heads == 0 or heads % kv_heads:
         raise RuntimeError(f"{op}: query heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
     if qkv.shape != (requests, (heads + 2 * kv_heads) * dim):
         raise RuntimeError(f"{op}: qkv {list(qkv.shape)} must be [{requests}, {(heads + 2 * kv_heads) * dim}]")
