@@ -402,9 +402,10 @@ TN_API int64_t tn_kv_q4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t p
  * 1: not enough pages, 2: a length outside [0, max_pages * page_size], 3: more
  * new tokens than max_tokens, 4: more free pages than num_pages. *status is
  * never cleared here. requests <= 8192.
- * tn_kv_pages_resize_granted also writes granted [requests]: each request's new
- * tokens, 0 for all of a call that cannot be met. Decode steps that follow read
- * it, so that they append nothing where no slot was given. */
+ * tn_kv_pages_resize_granted also keeps granted [requests], zeroed once: a
+ * request's new tokens of the last call that changed its length (0 if that took
+ * tokens away), and 0 for all after a call that cannot be met. Decode steps that
+ * follow read it, so that they append nothing where no slot was given. */
 TN_API int tn_kv_pages_resize(int *page_table, int64_t table_stride, int64_t max_pages, int *lengths,
                               const int *new_lengths, int64_t grow, int64_t requests, int *free_pages,
                               int *free_count, int64_t num_pages, int64_t page_size, int64_t *slots,

@@ -329,3 +329,31 @@ def test_a_pool_without_heads_is_refused(cuda_device):
     x = torch.zeros((2, 0, 64), device=cuda_device)
     with pytest.raises(RuntimeError, match="head count"):
         kv.kv_q4_append(x, x, pool, torch.zeros(2, dtype=torch.int64, device=cuda_device))
+
+
+def test_grants_outlast_resizes_of_other_requests(cuda_device):
+    """A request that grew steps although another one ended or came in since; one that ended, or did not grow, does not."""
+    cache = kv.PagedQ4Cache(1, 2, 64, 12, 3, 4, 16, cuda_device)
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn((50, 2, 64), generator=g).to(cuda_device)
+    slots, _, _ = cache.resize(50, new_lengths=i32([20, 30, 0], cuda_device))
+    cache.append(0, x, x.flip(0), slots)
+    qkv = torch.randn((3, 8 * 64), generator=g).to(BF).to(cuda_device)
+    rope = rope_table(64, 64, cuda_device)
+    cache.resize(2, grow=1)
+    cache.resize(0, new_lengths=i32([21, 0, 0], cuda_device))
+    assert cache.granted.tolist() == [1, 0, 0]
+    want_pool = cache.pools[0].clone()
+    want = kv.sdpa_q4_decode_step(qkv, rope, want_pool, cache.page_table, cache.lengths, 4)
+    out = cache.decode_step(0, qkv, rope, 4)
+    assert torch.equal(out, want) and torch.equal(cache.pools[0], want_pool) and (out[0] != 0).any()
+    assert (out[1:] == 0).all()
+    cache.resize(40, new_lengths=i32([21, 0, 40], cuda_device))
+    assert cache.granted.tolist() == [1, 0, 40]
+    cache.resize(400, new_lengths=i32([21, 0, 400], cuda_device))
+    assert cache.granted.tolist() == [0, 0, 0]
+    with pytest.raises(RuntimeError, match="length"):
+        cache.check()
+    cache.resize(0, new_lengths=i32([20, 0, 40], cuda_device))
+    assert cache.granted.tolist() == [0, 0, 0]
+    cache.check()

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize 
         if (blockIdx.x == 0) {
             p.query_start[b] = tok_at[b];
             p.lengths[b] = n;
-            if (p.granted) p.granted[b] = max(0, n - o);
+            if (p.granted && n != o) p.granted[b] = max(0, n - o);
         }
     }
     const int top = top0 + (int)gives;

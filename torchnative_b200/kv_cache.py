@@ -137,8 +137,9 @@ def kv_pages_resize(page_table: torch.Tensor, lengths: torch.Tensor, free_pages:
     go back to the stack free_pages[:free_count]; page_table, lengths,
     free_pages and free_count are updated in place. Nothing waits for the GPU:
     a call that cannot be met changes nothing, gives no token a slot and sets
-    `status` (see `PagedQ4Cache.check`). `granted` (int32 [requests]) receives
-    each request's new tokens, 0 for all of such a call: what a decode step
+    `status` (see `PagedQ4Cache.check`). `granted` (int32 [requests], zeroed
+    once) keeps each request's new tokens of the last call that changed its
+    length, and 0 for all after one that could not be met: what a decode step
     needs to leave the cache alone then."""
     op = "kv_pages_resize"
     device, index = page_table.device, page_table.get_device()
@@ -375,7 +376,7 @@ class PagedQ4Cache:
         self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
         self.free_count = torch.full((1,), num_pages, **i32)
         self.status = torch.zeros(1, **i32)
-        # the new tokens that the last resize gave each request, for the decode steps behind it
+        # the new tokens that resizes gave each request, 0 behind one that was refused: for the decode steps
         self.granted = torch.zeros(max_requests, **i32)
 
     def nbytes(self) -> int:
@@ -394,8 +395,9 @@ class PagedQ4Cache:
                              max_tokens=max_tokens, scale=scale)
 
     def decode_step(self, layer: int, qkv: torch.Tensor, rope: torch.Tensor, heads: int, *, scale=None, q8=None):
-        """`sdpa_q4_decode_step` of the tokens that the last `resize` granted; a
-        request that it gave none keeps its cache and gives zeros."""
+        """`sdpa_q4_decode_step` of the tokens that `resize` granted; a request
+        that has none, and every one behind a `resize` that could not be met,
+        keeps its cache and gives zeros."""
         return sdpa_q4_decode_step(qkv, rope, self.pools[layer], self.page_table, self.lengths, heads, scale=scale,
                                    q8=q8, granted=self.granted)
 
