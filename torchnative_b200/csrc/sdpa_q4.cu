@@ -32,10 +32,14 @@ namespace {
 // last ones ended alone (127 us for 82 at 2 x 100,000 tokens of 8 heads, then).
 // The first producer warp prepares each item's queries.
 //
-// What bounds it: instruction issue, ~550 instructions a unit (bf16, D 128) at
-// 0.6 to 0.69 a cycle and scheduler; 2 x 100,000 tokens of 8 heads of 128 take 57
-// us, 4.05 TB/s, 62% of a copy's rate; one request of 2048 10.4 us, nearly all of
-// it latency: ~3 us to the first products, ~4 us for the join.
+// What bounds it: the consumers' own latencies. A unit (bf16, D 128) is ~580
+// instructions, 26 us of issue at one a cycle for 2 x 100,000 tokens of 8 heads of
+// 128, which take 55 us (4.2 TB/s, 65% of a copy's rate): a scheduler issues in
+// 54% of the cycles, and its three consumer warps wait for their chain of scores,
+// vote, exponents and products, for the tensor and conversion pipes, and at an
+// item's end for one another. Of shorter lines start and join take more: issue in
+// 46% of the cycles for 32 ragged requests, 34% for drafts of 5 in float32; one
+// request of 2048 takes 10.4 us, ~3 us to the first products, ~4 us for the join.
 //
 // Per 16 tokens a warp computes, with m16n8k16 tensor instructions,
 //   S^T[16 tokens, 8 rows] = sum over blocks b of d_k[token, b] * (codes_b . q_b)
@@ -50,16 +54,22 @@ namespace {
 //
 // p is 2^(s - ref) times 2^10, f16, where ref follows the row's maximum by more
 // than 2^5 only (a vote per unit; out = O / l holds for any ref), and goes down
-// when the value scales are above 1, so that p * d_v stays in f16's range.
+// when the value scales are above 1, so that p * d_v stays in f16's range. For a
+// bf16 result p is one f16 term, and rounded again after its value's scale: each
+// time by 2^-11 at most, random from key to key, where the result's own rounding
+// is 2^-8. That shows as other neighbours of a result near the middle between two
+// (9e-4 of its norm), not as error: 0.0017 of it against 64 bits, as with float32
+// probabilities rounded once. For f16 and float32 results p * d_v has two terms.
+// The sums l and the products' accumulators are float32.
 constexpr int kMaxGrid = 148;  // CTAs whose parts a workspace holds
 constexpr int kUnitGroups = 2, kUnit = kUnitGroups * kKvGroup;
 constexpr float kBias = 10.0f, kSlack = 5.0f;
 // What an item costs besides its units (queries, the warps' results joined), in units: with 8, 12, 16, 20 the ragged
-// batch of 32 up to 8192 tokens (heads of 128, 8 of them) takes 47.6, 43.8, 42.0, 42.1 us, one request of 8192 12.9,
-// 13.0, 12.5, 13.1.
+// batch of 32 up to 8192 tokens (heads of 128, 8 of them) takes 47.4, 43.5, 41.8, 41.8 us, one request of 8192 12.7,
+// 12.9, 12.4, 12.9.
 constexpr int kItemCost = 16;
 // A CTA has 2^kMinPlaces places of the line before another one is used: with 8, 16, 32 of them one request of 2048
-// takes 10.3, 10.7, 13.9 us, 8192 tokens 13.4, 13.0, 15.1.
+// takes 10.1, 10.4, 11.6 us, of 8192 tokens 13.3, 12.4, 13.0.
 constexpr int kMinPlaces = 4;
 
 // What the producer tells the consumers of an item.
@@ -128,15 +138,10 @@ struct Split {
     float *scales, *offsets;
     const int *granted;  // [requests] new tokens that the resize gave, or NULL: one to each
     // The tokens of request b, its new one among them: none where the resize gave none, so that nothing is appended
-    // over what the cache holds, and none where the new one has no place (`lost`), so that what lies there is not read.
-    __device__ __forceinline__ int step_length(int b, bool *lost) const {
-        const int n = a.c.lengths[b];
-        *lost = n > places;
-        if (granted && granted[b] <= 0) {
-            *lost = false;
-            return 0;
-        }
-        return n < 0 || *lost ? 0 : n;
+    // over what the cache holds, and none where the new one has no place, so that what lies there is not read.
+    __device__ __forceinline__ int step_length(int b) const {
+        const int n = a.c.lengths[b], new_tokens = granted ? granted[b] : 1;
+        return new_tokens > 0 && (unsigned)n <= (unsigned)places ? n : 0;
     }
 };
 
@@ -164,8 +169,7 @@ struct Cursor {
 
     __device__ __forceinline__ void load_request(const Split &s) {
         const Attend &p = s.a;
-        bool lost;
-        S = STEP ? s.step_length(b, &lost) : p.c.length(b);
+        S = STEP ? s.step_length(b) : p.c.length(b);
         n = p.query_tokens(b, &first);
         tiles = (n * p.rep + RT - 1) / RT;
     }
@@ -235,10 +239,8 @@ __device__ __forceinline__ void append_new(const Split &p, int b, int h, int pos
     uint8_t *group = nullptr;
     if (pos >= 0) {
         group = a.c.group<D>(b, h, pos >> 4);
-    } else {
-        bool lost;
-        p.step_length(b, &lost);
-        if (lost) record_bad_page(a.c.err);
+    } else if (a.c.lengths[b] > p.places && (!p.granted || p.granted[b] > 0)) {
+        record_bad_page(a.c.err);
     }
     if (lane == 0) added.key = group ? pos & 15 : -1;
     if (!group) return;
