@@ -426,7 +426,9 @@ TN_API int tn_kv_q4_append(const void *k, const void *v, int dtype, const int64_
 
 /* Scratch bytes of the two attention calls below (device memory of the
  * caller's, 16-byte aligned, any contents; two calls that can run at the same
- * time need one each). max_query: a bound on one request's query tokens. */
+ * time need one each). max_query: a bound on one request's query tokens. Behind
+ * a call that recorded a timeout (tn_device_status) it must be cleared before a
+ * captured call that uses it runs again. */
 TN_API int64_t tn_sdpa_q4_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                           int64_t max_query);
 

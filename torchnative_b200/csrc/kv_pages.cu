@@ -106,8 +106,8 @@ __device__ __forceinline__ int64_t slot_of(const Resize &p, int b, int position)
 }
 
 // Latency bounds it: a launch, and inside it a chain of dependent loads
-// (lengths, prefix sums, stack entries). A decode step of 32 requests, and of
-// 700: 3.0 and 4.0 us.
+// (lengths, prefix sums, stack entries). A decode step and its way back, two calls:
+// 6.3 us of 32 requests, 9.0 of 700.
 __global__ void __launch_bounds__(kThreads) kv_pages_resize_kernel(const Resize p) {
     extern __shared__ int sm[];
     const int B = p.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;

@@ -25,7 +25,8 @@ struct Append {
 // One warp: 256 / D neighbouring tokens of one head, keys and values; a lane has
 // eight elements of a row. 2 D elements read and 9 D / 8 bytes written
 // a token and head; bound by the quantiser's instructions where there are many: 8192 tokens of 8 x 128 bf16 take 13.7
-// us, 3.1 TB/s (half a copy's rate), and 32 tokens 1.8 us, a launch.
+// us, 3.1 TB/s (half a copy's rate), 342 instructions a warp, issue active in 79% of the cycles; 32 tokens take 1.8 us,
+// a launch.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv_q4_append_kernel(const Append p) {
     using Q = KvQ4<D>;

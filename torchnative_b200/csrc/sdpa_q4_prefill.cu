@@ -26,12 +26,17 @@
 // as float32 sums are; a value's and a probability's roundings to 2^-11 are an
 // eighth of the bf16 result's own. (bf16 operands would lose 2^-8 three times
 // over. For f16 results those roundings would be as large as the result's: they
-// take the other kernel.)
+// take the other kernel.) A key is exact where its block's scale lies above 2^-14
+// of its group's largest: a smaller one is below f16's normal numbers here, and
+// rounded to a multiple of 2^-24 of at most twice that largest scale.
+// An infinite or NaN value scale counts as 0 in the products, since 0 times it
+// would be NaN in the rows that do not see its token; the rows that do add it at
+// the end, from the cache.
 // What bounds it: the stream of products, of which hardly a moment is without one,
 // but each of 128 x 128 x 16 takes 110 to 160 cycles for the 64 of the pipe's peak
 // (which was active 41% of the cycles at 866 us); two terms of K make half as many
 // again; and the last wave of items (384 on 148 SMs), an eighth. 2 x 1536 tokens at
-// 9728, 32/8 heads of 128: 820 us, 550 TFLOP/s.
+// 9728, 32/8 heads of 128: 824 us, 547 TFLOP/s.
 // Every wait is bounded; one that gives up raises a CTA-wide abort flag.
 #include <algorithm>
 #include <atomic>
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) sdpa_q4_prefill_kernel(const Atten
         const int all_see = S - n + (row_first + BM * k) / a.rep + 1;       // keys of every row of the tile
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tO = tmem + lane_off + TO + k * 128;
-        // ---- this row's queries, in f16 into TMEM: the largest magnitude taken to [2^13, 2^14) by a power of two
+        // ---- this row's queries, in f16 into shared memory: the largest magnitude taken to [2^13, 2^14) by a power of two
         float inv_q = 1.0f;
         {
             uint4 q[D / 8];
