@@ -20,7 +20,8 @@ BF = torch.bfloat16
 def calls(st, q, qkv, rope):
     """Every call that allocates, on copies of what it changes."""
     table, lengths = st.table.clone(), st.lengths.clone()
-    free, count, status = (torch.arange(9, dtype=torch.int32, device=q.device), torch.full_like(lengths[:1], 9),
+    pages = st.pool.shape[0]  # the table's ids are of these
+    free, count, status = (torch.arange(pages, dtype=torch.int32, device=q.device), torch.full_like(lengths[:1], 9),
                            torch.zeros_like(lengths[:1]))
     attend = kv.sdpa_q4_cache(q, st.pool, st.table, st.lengths)
     step = kv.sdpa_q4_decode_step(qkv, rope, st.pool.clone(), st.table, st.lengths, q.shape[1])
@@ -87,3 +88,4 @@ def test_a_first_call_in_a_capture_or_in_inference_mode(cuda_device):
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     assert torch.cuda.memory_stats()["reserved_bytes.all.current"] <= before  # no block of the graph's pool is held
+    N.device_status()
