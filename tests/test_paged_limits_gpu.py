@@ -357,3 +357,25 @@ def test_grants_outlast_resizes_of_other_requests(cuda_device):
     cache.resize(0, new_lengths=i32([20, 0, 40], cuda_device))
     assert cache.granted.tolist() == [0, 0, 0]
     cache.check()
+
+
+@pytest.mark.parametrize("requests, width", [(3, 5), (40, 500), (2600, 8)])
+def test_grants_follow_the_last_change_of_a_length(cuda_device, requests, width):
+    """In one CTA and in a cluster, up and down, with calls that cannot be met between."""
+    import random
+
+    rng = random.Random(requests)
+    cache = kv.PagedQ4Cache(1, 1, 64, requests * width, requests, width, 16, cuda_device)
+    want = [0] * requests
+    for turn in range(8):
+        old = cache.lengths.tolist()
+        new = [rng.choice([n, n, 0, min(n + 1, 16 * width), rng.randint(0, 16 * width)]) for n in old]
+        if turn in (3, 6):
+            new[rng.randrange(requests)] = 16 * width + 1
+            want = [0] * requests
+        else:
+            want = [w if n == o else max(0, n - o) for w, n, o in zip(want, new, old)]
+        cache.resize(requests * width * 16, new_lengths=i32(new, cuda_device))
+        assert cache.granted.tolist() == want
+        assert cache.status.item() == (2 if turn in (3, 6) else 0)
+        cache.status.zero_()
